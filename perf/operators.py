@@ -1,0 +1,352 @@
+"""Timing cases of the training-side operators: group norm with an activation on channels-last maps, class log probabilities
+of given labels, and distillation from a teacher's kept logits.
+
+`run` computes a case with elementary torch operations in 32 bits (`own = False`) or with the package's kernels (`own = True`);
+`exact` gives the same outputs from the definitions in 64 bits."""
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+EPS = 1e-5
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+SIZE = {"fp32": 4, "bf16": 2, "fp16": 2}
+MOST_BYTES = 6.0e8          # what the largest listed case has to move
+
+
+def listed():
+    return [
+        # the stride-4 map of a small (48 x 24 x 48) chunk at inference: latency
+        _gn("norm_small_map", (12, 6, 12), 128, 16, "relu", "fp32", "fwd"),
+        # a 64-channel stride-2 map at inference in half precision
+        _gn("norm_stride2_bf16", (48, 24, 48), 64, 8, "silu", "bf16", "fwd"),
+        # the 128-channel stride-4 map of a 96 x 48 x 96 chunk in a training step
+        _gn("norm_level_train", (24, 12, 24), 128, 32, "relu", "fp32", "train"),
+        # 32 channels at the full resolution of a chunk in a training step: the largest activation a chunk has
+        _gn("norm_full_train", (96, 48, 96), 32, 8, "relu", "fp32", "train"),
+        # the mask head's crops of 16 boxes (9 to 20 voxels on an edge), each with its own statistics
+        _gn_ragged("norm_crops_train", 16, 9, 20, 64, 16, "relu", "fp32", "train"),
+        # the RoI classifier's rows: confidence of the labels and three alternatives
+        _lp("logp_roi", "rows", 200, 19, 3, "fp32", "fwd"),
+        # per-voxel class scores of the 41 image classes on a stride-2 map, planar, in a training step
+        _lp("logp_voxels_train", "planar", 48 * 24 * 48, 41, 1, "fp32", "train"),
+        # a long list of class names (open vocabulary), an odd count, eight alternatives
+        _lp("logp_names", "rows", 2000, 20011, 8, "bf16", "fwd"),
+        # few objects against a long list: the class axis has to be split
+        _lp("logp_few", "rows", 3, 65536, 5, "fp32", "fwd"),
+        # a small RoI head learning from a larger one's four best classes
+        _kd("distill_roi_train", 200, 19, 4, 2.0, "fp32", "train"),
+        # per-voxel student with a thousand classes
+        _kd("distill_rows_train", 40000, 1203, 8, 1.5, "fp16", "train"),
+        # a long list of classes, many kept: the largest case
+        _kd("distill_names_train", 4096, 32768, 32, 1.0, "bf16", "train"),
+    ]
+
+
+def _gn(name, dims, c, g, act, dtype, way):
+    return dict(name=name, op="norm", ragged=False, n=1, nx=dims[0], ny=dims[1], nz=dims[2], c=c, g=g, act=act, dtype=dtype, way=way)
+
+
+def _gn_ragged(name, crops, lo, hi, c, g, act, dtype, way):
+    return dict(name=name, op="norm", ragged=True, crops=crops, lo=lo, hi=hi, mix=crops * 1000 + hi, c=c, g=g, act=act, dtype=dtype, way=way)
+
+
+def _lp(name, layout, rows, classes, top, dtype, way):
+    return dict(name=name, op="logp", layout=layout, rows=rows, classes=classes, top=top, dtype=dtype, way=way)
+
+
+def _kd(name, rows, classes, kept, temperature, dtype, way):
+    return dict(name=name, op="distill", rows=rows, classes=classes, kept=kept, temperature=temperature, dtype=dtype, way=way)
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    while True:
+        op = rng.choice(["norm", "crops", "logp", "distill"])
+        dtype, way = rng.choice(sorted(DTYPES)), rng.choice(["fwd", "train"])
+        if op in ("norm", "crops"):
+            g = rng.choice([1, 2, 4, 8, 16, 32])
+            c = g * rng.choice([1, 2, 3, 4, 5, 8, 16])
+            act = rng.choice(["none", "relu", "silu"])
+            if not 16 <= c <= 256:
+                continue
+            if op == "norm":
+                e = _log(rng, 5, 96)
+                case = _gn("", (e, max(2, e // 2 + rng.randint(-1, 1)), e + rng.randint(-2, 2)), c, g, act, dtype, way)
+                case["n"] = rng.choice([1, 1, 2, 3])
+            else:
+                lo = rng.randint(2, 10)
+                case = _gn_ragged("", _log(rng, 1, 100), lo, lo + rng.randint(1, 14), c, g, act, dtype, way)
+        elif op == "logp":
+            layout = rng.choice(["rows", "rows", "planar"])
+            rows = _log(rng, 1, 100000)
+            classes = _log(rng, 2, 200 if layout == "planar" else 65536)
+            case = _lp("", layout, rows, classes, min(classes, rng.randint(0, 10)), dtype, way)
+        else:
+            rows, classes = _log(rng, 1, 100000), _log(rng, 5, 65536)
+            case = _kd("", rows, classes, min(classes, _log(rng, 1, 64)), rng.choice([1.0, 1.5, 2.0, 4.0]), dtype, way)
+        del case["name"]
+        if work(case)["bytes"] <= MOST_BYTES * (0.5 if case["op"] == "norm" else 1.0):
+            return case
+
+
+def _crop_rows(case):
+    r = random.Random(case["mix"])
+    return [r.randint(case["lo"], case["hi"]) * r.randint(case["lo"], case["hi"]) * r.randint(case["lo"], case["hi"]) for _ in range(case["crops"])]
+
+
+def work(case):
+    s, train = SIZE[case["dtype"]], case["way"] == "train"
+    if case["op"] == "norm":
+        rows = sum(_crop_rows(case)) if case["ragged"] else case["n"] * case["nx"] * case["ny"] * case["nz"]
+        n = rows * case["c"]
+        return {"bytes": n * s * (4 if train else 2) + case["c"] * (16 if train else 8), "flops": n * (30 if train else 9)}
+    r, k = case["rows"], case["classes"]
+    if case["op"] == "logp":
+        out = r * (8 + 8 + 12 * case["top"])
+        return {"bytes": r * k * s * (2 if train else 1) + out + (8 * r if train else 0), "flops": r * k * (12 if train else 6)}
+    kept = case["kept"] * r * (8 + 4)
+    return {"bytes": r * k * s * (2 if train else 1) + kept + r * (8 if train else 4), "flops": r * k * (8 if train else 4)}
+
+
+# ------------------------------------------------------------------ inputs --
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(int(seed))
+
+    def normal(*shape):
+        return torch.randn(*shape, device="cuda", generator=gen)
+
+    def chance(*shape):
+        return torch.rand(*shape, device="cuda", generator=gen)
+
+    dt = DTYPES[case["dtype"]]
+    st = dict(case)
+    if case["op"] == "norm":
+        c = case["c"]
+        scale, shift = 0.5 + chance(c), 0.5 * normal(c)                 # a convolution's output: channels differ in size and place
+        if case["ragged"]:
+            rows = _crop_rows(case)
+            st["offsets"] = torch.tensor([0] + rows, device="cuda").cumsum(0)
+            st["x"] = (normal(sum(rows), c) * scale + shift).to(dt)
+            st["dy"] = normal(sum(rows), c).to(dt) if case["way"] == "train" else None
+        else:
+            dims = (case["n"], case["nx"], case["ny"], case["nz"], c)
+            st["offsets"] = None
+            st["x"] = (normal(*dims) * scale + shift).to(dt).permute(0, 4, 1, 2, 3)
+            st["dy"] = normal(*dims).to(dt).permute(0, 4, 1, 2, 3) if case["way"] == "train" else None
+        st["weight"], st["bias"] = 1 + 0.2 * normal(c), 0.2 * normal(c)
+        return st
+    r, k = case["rows"], case["classes"]
+    truth = torch.randint(0, k, (r,), device="cuda", generator=gen)
+    score = 2.0 * normal(r, k)
+    score.scatter_add_(1, truth[:, None], 3.0 + 2.0 * normal(r, 1))     # a trained head prefers the right class
+    st["grad"] = normal(r)                                              # of a loss scaled up for half precision
+    if case["op"] == "logp":
+        st["labels"] = torch.where(chance(r) < 0.05, torch.full_like(truth, -1), truth)     # some rows carry no label
+        st["grad_entropy"] = 0.1 * normal(r)
+        if case["layout"] == "planar":
+            st["score"] = score.t().contiguous()[None].to(dt)           # (1, classes, rows)
+            for name in ("labels", "grad", "grad_entropy"):
+                st[name] = st[name][None]
+        else:
+            st["score"] = score.to(dt)
+        return st
+    teacher = score + normal(r, k)
+    kept, st["classes_kept"] = teacher.topk(case["kept"], 1)
+    st["kept"] = kept.contiguous()
+    if case["kept"] > 1:                                                # some teachers kept one class fewer
+        st["classes_kept"][:, -1] = torch.where(chance(r) < 0.1, torch.full_like(truth, -1), st["classes_kept"][:, -1])
+    st["score"] = score.to(dt)
+    return st
+
+
+# ------------------------------------------------------------- the package --
+_package = None
+
+
+def _ops():
+    global _package
+    if _package is None:
+        sys.path.insert(0, os.path.join(ROOT, "3d-sis_amd"))
+        from sis3d import ops
+        _package = ops
+    return _package
+
+
+def run(state):
+    if own:
+        return _run_package(state)
+    return {"norm": _plain_norm, "logp": _plain_logp, "distill": _plain_distill}[state["op"]](state)
+
+
+def _run_package(st):
+    ops = _ops()
+    train = st["way"] == "train"
+    if st["op"] == "norm":
+        if not train:
+            return {"y": ops.group_norm(st["x"], st["g"], st["weight"], st["bias"], EPS, act=st["act"], offsets=st["offsets"])}
+        y, mean, rstd = ops.group_norm(st["x"], st["g"], st["weight"], st["bias"], EPS, act=st["act"], offsets=st["offsets"], want_stats=True)
+        dx, dw, db = ops.group_norm_backward(st["dy"], st["x"], mean, rstd, st["g"], st["weight"], st["bias"], act=st["act"], offsets=st["offsets"])
+        return {"y": y, "dx": dx, "dweight": dw, "dbias": db}
+    if st["op"] == "logp":
+        logp, entropy, lse, top_logp, top_class = ops.class_logprobs(st["score"], st["labels"], top=st["top"])
+        out = {"logp": logp, "entropy": entropy, "top_logp": top_logp, "top_class": top_class}
+        if train:
+            out["dscore"] = ops.class_logprobs_backward(st["score"], st["labels"], lse, entropy, st["grad"], st["grad_entropy"])
+        return out
+    loss, lse = ops.distill_loss(st["score"], st["kept"], st["classes_kept"], st["temperature"])
+    out = {"loss": loss}
+    if train:
+        out["dscore"] = ops.distill_loss_backward(st["score"], st["kept"], st["classes_kept"], lse, st["grad"], st["temperature"])
+    return out
+
+
+# ------------------------------------------------------------- plain forms --
+def _act(z, act):
+    return torch.clamp_min(z, 0) if act == "relu" else z / (1 + torch.exp(-z)) if act == "silu" else z
+
+
+def _act_slope(z, act):
+    if act == "relu":
+        return (z > 0).to(z.dtype)
+    if act == "silu":
+        s = 1 / (1 + torch.exp(-z))
+        return s * (1 + z * (1 - s))
+    return torch.ones_like(z)
+
+
+def _plain_norm(st):
+    x, g, c, off = st["x"], st["g"], st["c"], st["offsets"]
+    rows = x if off is not None else x.permute(0, 2, 3, 4, 1).reshape(st["n"], -1, c)
+    shape = rows.shape
+    a = rows.float().reshape(*shape[:-1], g, c // g)
+
+    if off is not None:                                     # sums of each crop's rows: differences of a running sum in 64 bits
+        count = (off[1:] - off[:-1]).double()[:, None] * (c // g)
+        sample = torch.searchsorted(off[1:], torch.arange(shape[0], device=x.device), right=True)
+
+        def mean_of(t):
+            run_ = torch.cat([t.new_zeros(g, 1, dtype=torch.float64), t.sum(-1).t().double().contiguous().cumsum(1)], 1)
+            return ((run_[:, off[1:]] - run_[:, off[:-1]]).t() / count).float()[sample][..., None]
+    else:
+        def mean_of(t):
+            return t.mean((1, 3), keepdim=True)
+
+    mean = mean_of(a)
+    d = a - mean
+    rstd = 1 / torch.sqrt(mean_of(d * d) + EPS)
+    h = d * rstd
+    w, b = st["weight"].reshape(g, -1), st["bias"].reshape(g, -1)
+    z = h * w + b
+
+    def back(t):
+        t = t.reshape(shape).to(x.dtype)
+        return t if off is not None else t.reshape(st["n"], st["nx"], st["ny"], st["nz"], c).permute(0, 4, 1, 2, 3)
+
+    y = back(_act(z, st["act"]))
+    if st["way"] == "fwd":
+        return {"y": y}
+    dy = st["dy"] if off is not None else st["dy"].permute(0, 2, 3, 4, 1).reshape(shape)
+    dz = dy.float().reshape(a.shape) * _act_slope(z, st["act"])
+    dh = dz * w
+    dx = rstd * (dh - mean_of(dh) - h * mean_of(dh * h))
+    return {"y": y, "dx": back(dx), "dweight": (dz * h).reshape(-1, c).sum(0), "dbias": dz.reshape(-1, c).sum(0)}
+
+
+def _plain_logp(st):
+    l = st["score"].float()
+    if st["layout"] == "planar":
+        l = l.permute(0, 2, 1)
+    labels, k = st["labels"], st["top"]
+    m = l.max(-1, keepdim=True)[0]
+    lse = m + torch.log(torch.exp(l - m).sum(-1, keepdim=True))
+    logs = l - lse
+    p = torch.exp(logs)
+    entropy = -(p * logs).sum(-1)
+    has = labels >= 0
+    logp = torch.where(has, logs.gather(-1, labels.clamp_min(0)[..., None])[..., 0], 0.0)
+    # the largest scores, the lowest class first among equal ones: whole numbers in the order of (score, -class)
+    bits = (l + 0.0).contiguous().view(torch.int32).long()
+    key = torch.where(bits >= 0, bits, -(bits & 0x7FFFFFFF)) * (1 << 32) - torch.arange(l.shape[-1], device=l.device)
+    top_class = key.topk(k, -1)[1]
+    out = {"logp": logp, "entropy": entropy, "top_logp": logs.gather(-1, top_class), "top_class": top_class}
+    if st["way"] == "train":
+        a = torch.where(has, st["grad"], 0.0)[..., None]
+        e = st["grad_entropy"][..., None]
+        d = -p * (a + e * (logs + entropy[..., None]))
+        d = d.scatter_add(-1, labels.clamp_min(0)[..., None], a)
+        d = d.to(st["score"].dtype)
+        out["dscore"] = d.permute(0, 2, 1).contiguous() if st["layout"] == "planar" else d
+    return out
+
+
+def _plain_distill(st):
+    temp, cls = st["temperature"], st["classes_kept"]
+    l = st["score"].float() / temp
+    m = l.max(-1, keepdim=True)[0]
+    logs = l - (m + torch.log(torch.exp(l - m).sum(-1, keepdim=True)))
+    has = cls >= 0
+    t = torch.where(has, st["kept"] / temp, float("-inf"))
+    e = torch.exp(t - t.max(-1, keepdim=True)[0])
+    q = e / e.sum(-1, keepdim=True)
+    at = cls.clamp_min(0)
+    loss = temp * temp * torch.where(q > 0, q * (torch.log(q) - logs.gather(-1, at)), 0.0).sum(-1)
+    out = {"loss": loss}
+    if st["way"] == "train":
+        out["dscore"] = (temp * st["grad"][:, None] * torch.exp(logs).scatter_add(-1, at, -q)).to(st["score"].dtype)
+    return out
+
+
+# ------------------------------------------------------ 64-bit definitions --
+def exact(case, seed):
+    st = prepare(case, seed)
+    train = case["way"] == "train"
+    with torch.enable_grad():
+        if case["op"] == "norm":
+            x = st["x"].double().detach().requires_grad_(train)
+            w, b = (st[n].double().requires_grad_(train) for n in ("weight", "bias"))
+            parts = [x] if st["offsets"] is None else [x[int(u):int(v)].t()[None] for u, v in zip(st["offsets"], st["offsets"][1:])]
+            ys = []
+            for part in parts:
+                n, c = part.shape[:2]
+                flat = part.reshape(n, case["g"], -1)
+                var, mu = torch.var_mean(flat, -1, unbiased=False, keepdim=True)
+                z = ((flat - mu) * (var + EPS).rsqrt()).reshape(n, c, -1) * w[:, None] + b[:, None]
+                z = z.relu() if case["act"] == "relu" else z * z.sigmoid() if case["act"] == "silu" else z
+                ys.append(z.reshape(part.shape) if st["offsets"] is None else z[0].t())
+            y = ys[0] if st["offsets"] is None else torch.cat(ys)
+            if not train:
+                return {"y": y.detach()}
+            dx, dw, db = torch.autograd.grad(y, [x, w, b], st["dy"].double())
+            return {"y": y.detach(), "dx": dx, "dweight": dw, "dbias": db}
+        if case["op"] == "logp":
+            s = st["score"].double().detach().requires_grad_(train)
+            logs = torch.log_softmax(s, 1)
+            rows = logs.movedim(1, -1)
+            labels = st["labels"]
+            logp = torch.where(labels >= 0, rows.gather(-1, labels.clamp_min(0)[..., None])[..., 0], 0.0)
+            entropy = -(rows * rows.exp()).sum(-1)
+            top = rows.detach().sort(dim=-1, descending=True, stable=True)[0][..., :case["top"]] if rows.numel() < 3e7 else rows.detach().topk(case["top"], -1)[0]
+            out = {"logp": logp.detach(), "entropy": entropy.detach(), "top_logp": top, "top_class": None}
+            if train:
+                out["dscore"], = torch.autograd.grad((logp * st["grad"].double()).sum() + (entropy * st["grad_entropy"].double()).sum(), s)
+            return out
+        temp, cls = case["temperature"], st["classes_kept"]
+        s = st["score"].double().detach().requires_grad_(train)
+        logs = torch.log_softmax(s / temp, 1)
+        logq = torch.log_softmax((st["kept"].double() / temp).masked_fill(cls < 0, float("-inf")), 1)
+        q = logq.exp()
+        term = q * (logq.masked_fill(q == 0, 0.0) - logs.gather(1, cls.clamp_min(0)))
+        loss = temp * temp * term.sum(1)
+        out = {"loss": loss.detach()}
+        if train:
+            out["dscore"], = torch.autograd.grad((loss * st["grad"].double()).sum(), s)
+        return out
