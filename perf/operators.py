@@ -197,15 +197,15 @@ def _run_package(st):
         dx, dw, db = ops.group_norm_backward(st["dy"], st["x"], mean, rstd, st["g"], st["weight"], st["bias"], act=st["act"], offsets=st["offsets"])
         return {"y": y, "dx": dx, "dweight": dw, "dbias": db}
     if st["op"] == "logp":
-        logp, entropy, lse, top_logp, top_class = ops.class_logprobs(st["score"], st["labels"], top=st["top"])
+        logp, entropy, norm, top_logp, top_class = ops.class_logprobs(st["score"], st["labels"], top=st["top"])
         out = {"logp": logp, "entropy": entropy, "top_logp": top_logp, "top_class": top_class}
         if train:
-            out["dscore"] = ops.class_logprobs_backward(st["score"], st["labels"], lse, entropy, st["grad"], st["grad_entropy"])
+            out["dscore"] = ops.class_logprobs_backward(st["score"], st["labels"], norm, entropy, st["grad"], st["grad_entropy"])
         return out
-    loss, lse = ops.distill_loss(st["score"], st["kept"], st["classes_kept"], st["temperature"])
+    loss, norm = ops.distill_loss(st["score"], st["kept"], st["classes_kept"], st["temperature"])
     out = {"loss": loss}
     if train:
-        out["dscore"] = ops.distill_loss_backward(st["score"], st["kept"], st["classes_kept"], lse, st["grad"], st["temperature"])
+        out["dscore"] = ops.distill_loss_backward(st["score"], st["kept"], st["classes_kept"], norm, st["grad"], st["temperature"])
     return out
 
 
