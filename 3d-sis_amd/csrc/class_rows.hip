@@ -1,0 +1,853 @@
+// Rows of class scores: log probabilities of given labels with entropy and top alternatives, distillation from a teacher's kept
+// logits, and the gradients of both with respect to the scores.
+//
+// Row l of K scores, temperature T (1 for the log probabilities):  L = log sum_j exp(l_j / T),  p_j = exp(l_j / T - L)
+//     log probabilities:  logp = l_y - L,  H = L - sum_j p_j l_j,  the k largest l_j - L (equal scores: the lowest class first)
+//     their gradient:     dl_j = a (1[j = y] - p_j) - e p_j (l_j - L + H)
+//     distillation:       q = softmax of the kept teacher logits / T,  loss = T^2 sum_i q_i (log q_i - l_ci / T + L)
+//     its gradient:       dl_j = g T (p_j - sum over i with c_i = j of q_i)
+//
+// All of it is bound by reading the scores once (and writing the gradient once).  Forward keeps a running maximum m and the sums
+// s = sum e^((l - m) / T) and t = sum (l - m) e^((l - m) / T) per lane, rescaled when m grows, so a row is read once whatever its length;
+// H = log s - t / s needs no second pass.  Everything is held in 32 bits.
+// A row's L is kept as the pair (m, log s): p = exp((l - m) / T - log s) then has no rounding of a large L in it, and rows of the
+// type's lowest value come out as what they are (all classes alike).
+//
+// Three forms, by the number of classes:
+//   K <= 1024        a group of 1 .. 64 lanes holds a row in registers; class-strided (planar) scores give neighbouring rows to
+//                    neighbouring lanes, contiguous rows give neighbouring classes to them
+//   longer rows      a wave (K <= 4096) or a workgroup streams a row with 16-byte loads from its first aligned element on
+//   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
+//
+// Alternatives of a long row without sorting it: every lane knows the largest (score, class) of its own vectors.  The lanes are put
+// into >= k groups; the smallest of the group maxima is a bound that at least k elements reach, so only lanes whose maximum
+// reaches it are read again (from cache) and their elements at or above it -- k log k of them or so -- are ranked by counting.
+#include "elem.h"
+
+namespace {
+
+constexpr int TOP_MAX = 32, KEPT_MAX = 128, K_SMALL = 1024, K_WAVE = 4096;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, LOWEST = -3.402823466e38f;
+constexpr int LP = 0, KD = 1;
+
+struct RowArgs {
+    const void *score;
+    void *dscore;
+    int64_t s_n, s_v, s_c, d_n, d_v, d_c;      // element strides: outer index, row inside it, class
+    int64_t V, R;                              // row r = n * V + v
+    int K, N;
+    const int32_t *num;                        // live rows, or NULL
+    const int64_t *labels;
+    int top;
+    float *logp, *entropy, *top_logp;
+    float2 *norm;                              // (m, log s) of each row
+    int64_t *top_class;
+    const float *kept;                         // (R, nk)
+    const int64_t *cls;
+    int nk;
+    float tau, inv, inv_lo, c2;                // T, 1 / T in two parts, log2(e) / T
+    float *loss;
+    const float *g1, *g2;                      // gradients: of logp and entropy, or of the loss
+    const float2 *norm_in;
+    const float *entropy_in;
+    int lpr_log, planar, parts;
+    float *part;                               // [R * parts][4]
+    uint64_t *part_keys;                       // [R * parts][top]
+};
+
+__device__ inline int64_t live_rows(const RowArgs &a)
+{
+    if (!a.num) return a.R;
+    const int64_t n = a.num[0];
+    return n < 0 ? 0 : (n < a.R ? n : a.R);
+}
+__device__ inline int64_t row_at(const RowArgs &a, int64_t r, int64_t sn, int64_t sv)
+{
+    if (a.N == 1) return r * sv;
+    const int64_t n = r / a.V;
+    return n * sn + (r - n * a.V) * sv;
+}
+
+__device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// (score, class) as one number: larger score first, then the lower class; -0 counts as 0, NaN as -inf
+__device__ inline uint64_t key_of(float v, int c)
+{
+    v = v != v ? -INFINITY : v + 0.f;
+    const uint32_t b = __float_as_uint(v);
+    const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    return ((uint64_t)o << 32) | (uint32_t)~c;
+}
+__device__ inline int key_class(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ inline float key_score(uint64_t k)
+{
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xffffffffu));
+}
+__device__ inline uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__shfl_xor((unsigned long long)v, o); }
+__device__ inline uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ inline uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
+
+// running sums of a softmax: m in score units (never below LOWEST), s = sum 2^x, t = sum x 2^x, x = (l - m) c2
+struct Soft {
+    float m, s, t;
+    __device__ void init() { m = LOWEST; s = t = 0.f; }
+    __device__ void raise(float to, float c2)
+    {
+        const float x = (m - to) * c2, f = exp2_(x);
+        t = f * fmaf(fmaxf(x, -200.f), s, t);          // -200: 2^x is 0 from there on, and 0 * inf is not wanted
+        s *= f;
+        m = to;
+    }
+    __device__ void add(float l, float c2)             // l <= m
+    {
+        const float x = (l - m) * c2, e = exp2_(x);
+        s += e;
+        t = fmaf(fmaxf(x, -200.f), e, t);
+    }
+    __device__ void join(float m2, float s2, float t2, float c2)
+    {
+        Soft o{m2, s2, t2};
+        const float to = fmaxf(m, m2);
+        raise(to, c2);
+        o.raise(to, c2);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ void join_xor(int o, float c2)
+    {
+        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o), t2 = __shfl_xor(t, o);
+        // the same order on both sides, so that every lane ends with the same bits
+        if (threadIdx.x & o) { Soft a{m2, s2, t2}; a.join(m, s, t, c2); *this = a; }
+        else join(m2, s2, t2, c2);
+    }
+    __device__ float2 norm() const { return make_float2(m, s == 0.f ? -INFINITY : logf(s)); }      // s = 0: a row of nothing but -inf
+    __device__ float entropy() const { return s == 0.f ? 0.f : logf(s) - LN2 * (t / s); }
+};
+
+// l / T - L, -inf where L is
+__device__ inline float log_p(float l, float2 norm, float inv, float inv_lo)
+{
+    const float d = l - norm.x;
+    return norm.y == -INFINITY ? -INFINITY : fmaf(d, inv, fmaf(fmaxf(d, LOWEST), inv_lo, -norm.y));
+}
+
+__device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, float2 norm)
+{
+    const int64_t y = a.labels[r];
+    return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, norm, 1.f, 0.f));
+}
+
+__device__ inline float lp_grad(float l, float2 norm, float h, float ga, float ge)
+{
+    const float lp = log_p(l, norm, 1.f, 0.f), p = exp2_(lp * LOG2E);
+    return -p * (ga + ge * (fmaxf(lp, -200.f) + h));
+}
+__device__ inline float kd_p(const RowArgs &a, float l, float2 norm) { return exp2_(log_p(l, norm, a.inv, a.inv_lo) * LOG2E); }
+
+// a teacher's entry: 0 = absent, 1 = present, 2 = no such class
+__device__ inline int entry(const RowArgs &a, int64_t c) { return c < 0 ? 0 : (c >= a.K ? 2 : 1); }
+
+// ---------------------------------------------------------------- K <= 1024: a row in the registers of 1 .. 64 lanes --
+struct Group {
+    int64_t r, at;                             // row; the row that may be read (0 where r is none: such lanes take part in the shuffles only)
+    int sub, lpr, step;                        // lane of the row, lanes per row, distance of neighbouring row lanes
+    bool in, live;                             // a row of the call; a live one
+};
+__device__ inline Group group_of(const RowArgs &a)
+{
+    Group g;
+    const int lane = threadIdx.x & 63, rpw_log = 6 - a.lpr_log;
+    g.lpr = 1 << a.lpr_log;
+    const int64_t wave = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    int row;
+    if (a.planar) {
+        row = lane & ((1 << rpw_log) - 1);
+        g.sub = lane >> rpw_log;
+        g.step = 1 << rpw_log;
+    } else {
+        row = lane >> a.lpr_log;
+        g.sub = lane & (g.lpr - 1);
+        g.step = 1;
+    }
+    g.r = (wave << rpw_log) + row;
+    g.in = g.r < a.R;
+    g.live = g.in && g.r < live_rows(a);
+    g.at = g.live ? g.r : 0;
+    return g;
+}
+__device__ inline float group_sum(float v, const Group &g)
+{
+    for (int o = g.lpr >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o * g.step);
+    return v;
+}
+__device__ inline float group_max(float v, const Group &g)
+{
+    for (int o = g.lpr >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o * g.step));
+    return v;
+}
+
+// largest kept logit, sum of exponentials of a row's kept logits, and whether an entry names no class; lanes share the entries
+struct Teacher { float m, s; bool any, bad; };
+__device__ inline Teacher group_teacher(const RowArgs &a, const Group &g)
+{
+    Teacher t{-INFINITY, 0.f, false, false};
+    const float *kept = a.kept + g.at * a.nk;
+    const int64_t *cls = a.cls + g.at * a.nk;
+    float bad = 0.f;
+    for (int i = g.sub; i < a.nk; i += g.lpr) {
+        const int e = entry(a, cls[i]);
+        if (e) t.m = fmaxf(t.m, kept[i]);
+        if (e == 2 || (e && kept[i] != kept[i])) bad = 1.f;
+    }
+    t.m = group_max(t.m, g);
+    t.bad = group_max(bad, g) > 0.f;
+    t.any = t.m > -INFINITY;
+    if (t.any)
+        for (int i = g.sub; i < a.nk; i += g.lpr)
+            if (entry(a, cls[i])) t.s += exp2_((kept[i] - t.m) * a.c2);
+    t.s = group_sum(t.s, g);
+    return t;
+}
+// the part of the loss that one lane's entries of a row give; q log q is 0 at q = 0
+template <typename T> __device__ inline float teacher_loss(const RowArgs &a, const Group &g, const Teacher &t, const T *row, float2 norm)
+{
+    float loss = 0.f;
+    if (!t.any) return loss;
+    const float ls = logf(t.s);
+    for (int i = g.sub; i < a.nk; i += g.lpr) {
+        const int64_t c = a.cls[g.at * a.nk + i];
+        if (entry(a, c) != 1) continue;
+        const float x = (a.kept[g.at * a.nk + i] - t.m) * a.c2, q = exp2_(x) / t.s;
+        if (q != 0.f) loss += q * (x * LN2 - ls - log_p(sis3d_f32(row[c * a.s_c]), norm, a.inv, a.inv_lo));
+    }
+    return loss;
+}
+
+template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void small_forward(RowArgs a)
+{
+    const Group g = group_of(a);
+    const T *p = (const T *)a.score + row_at(a, g.at, a.s_n, a.s_v);
+    float v[E];
+    Soft so;
+    so.init();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = g.sub + e * g.lpr;
+        v[e] = c < a.K && g.live ? sis3d_f32(p[c * a.s_c]) : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) so.m = fmaxf(so.m, v[e]);
+    so.m = group_max(so.m, g);
+#pragma unroll
+    for (int e = 0; e < E; ++e) so.add(v[e], a.c2);
+    so.s = group_sum(so.s, g);
+    so.t = group_sum(so.t, g);
+    const float2 norm = so.norm();
+    if constexpr (MODE == KD) {
+        const Teacher t = group_teacher(a, g);
+        const float loss = a.tau * a.tau * group_sum(g.live ? teacher_loss(a, g, t, p, norm) : 0.f, g);
+        if (g.sub == 0 && g.in) {
+            a.loss[g.r] = !g.live ? 0.f : (t.bad ? NAN : loss);
+            a.norm[g.r] = g.live ? norm : make_float2(0.f, 0.f);
+        }
+        return;
+    }
+    if (g.sub == 0 && g.in) {
+        const int64_t y = a.labels[g.at];
+        a.logp[g.r] = g.live ? label_logp(a, g.r, y >= 0 && y < a.K ? sis3d_f32(p[y * a.s_c]) : 0.f, norm) : 0.f;
+        a.entropy[g.r] = g.live ? so.entropy() : 0.f;
+        a.norm[g.r] = g.live ? norm : make_float2(0.f, 0.f);
+    }
+    uint32_t taken = 0;
+    for (int i = 0; i < a.top; ++i) {
+        uint64_t best = 0;
+        int at = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int c = g.sub + e * g.lpr;
+            const uint64_t k = c < a.K && !(taken >> e & 1) ? key_of(v[e], c) : 0;
+            if (k > best) { best = k; at = e; }
+        }
+        uint64_t all = best;
+        for (int o = g.lpr >> 1; o > 0; o >>= 1) all = max64(all, shfl_xor64(all, o * g.step));
+        if (best == all) taken |= 1u << at;
+        if (g.sub == 0 && g.in) {
+            a.top_class[g.r * a.top + i] = g.live ? key_class(all) : 0;
+            a.top_logp[g.r * a.top + i] = g.live ? log_p(key_score(all), norm, 1.f, 0.f) : 0.f;
+        }
+    }
+}
+
+template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void small_backward(RowArgs a)
+{
+    const Group g = group_of(a);
+    const T *p = (const T *)a.score + row_at(a, g.at, a.s_n, a.s_v);
+    T *d = (T *)a.dscore + row_at(a, g.in ? g.r : 0, a.d_n, a.d_v);
+    float q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] = 0.f;
+    float ga = 0.f, ge = 0.f, h = 0.f;
+    float2 norm = a.norm_in[g.at];
+    if constexpr (MODE == LP) {
+        const int64_t y = a.labels[g.at];
+        h = a.entropy_in[g.at];
+        ga = y < 0 ? 0.f : (y >= a.K ? NAN : a.g1[g.at]);
+        ge = a.g2 ? a.g2[g.at] : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (g.sub + e * g.lpr == y) q[e] = ga;
+    } else {
+        const Teacher t = group_teacher(a, g);
+        ga = t.bad ? NAN : (t.any ? a.g1[g.at] * a.tau : 0.f);
+        if (t.any)
+            for (int i = 0; i < a.nk; ++i) {
+                const int64_t c = a.cls[g.at * a.nk + i];
+                const float w = entry(a, c) == 1 ? exp2_((a.kept[g.at * a.nk + i] - t.m) * a.c2) / t.s : 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (g.sub + e * g.lpr == c) q[e] += w;
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = g.sub + e * g.lpr;
+        if (c >= a.K || !g.in) continue;
+        const float l = sis3d_f32(p[c * a.s_c]);
+        float o;
+        if constexpr (MODE == LP) o = lp_grad(l, norm, h, ga, ge) + q[e];
+        else o = ga * (kd_p(a, l, norm) - q[e]);
+        d[c * a.d_c] = sis3d_from_f32<T>(g.live ? o : 0.f);
+    }
+}
+
+// ---------------------------------------------------------------------------- long rows, classes contiguous --
+// A team of W waves (1: four teams to a workgroup; 4: the workgroup) has a row or a part of one.
+template <int W> __device__ inline void team_sync()
+{
+    if constexpr (W == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    } else __syncthreads();
+}
+
+// [k0, k1) of a row: elements in front of the first 16-byte boundary and behind the last whole vector are taken one by one
+template <typename T> struct Span {
+    static constexpr int VEC = 16 / sizeof(T);
+    const T *row, *body;
+    int k0, head, nvec, tail;
+    __device__ Span(const T *row_, int k0_, int k1) : row(row_), k0(k0_)
+    {
+        const int n = k1 - k0;
+        head = (int)((16 - ((uintptr_t)(row + k0) & 15)) & 15) / (int)sizeof(T);
+        if (head > n) head = n;
+        nvec = (n - head) / VEC;
+        tail = n - head - nvec * VEC;
+        body = row + k0 + head;
+    }
+    __device__ int first_class(int v) const { return k0 + head + v * VEC; }
+    // the i-th of the single elements, i < head + tail
+    __device__ int edge_class(int i) const { return i < head ? k0 + i : k0 + head + nvec * VEC + (i - head); }
+    __device__ int edges() const { return head + tail; }
+};
+
+template <typename T, int W, int MODE> struct Long {
+    static constexpr int NL = 64 * W, CAP = W == 1 ? 512 : 1024, VEC = 16 / sizeof(T);
+    struct Shared {
+        uint64_t cand[CAP], bound[W];
+        float red[W][3];
+        int lanes[W][64], count;
+    };
+    static __device__ int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
+
+    // one pass over the span: the team's sums in every lane, and this lane's largest (score, class) among its vectors
+    static __device__ Soft pass(const RowArgs &a, const Span<T> &sp, Shared &sh, uint64_t &best_key)
+    {
+        Soft so;
+        so.init();
+        float best = -INFINITY;
+        int at = lane();
+        for (int v = lane(); v < sp.nvec; v += NL) {
+            float x[VEC];
+            sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
+            float mx = x[0];
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) mx = fmaxf(mx, x[i]);
+            if constexpr (MODE == LP) at = mx > best ? v : at;
+            best = fmaxf(best, mx);
+            so.raise(fmaxf(so.m, mx), a.c2);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) so.add(x[i], a.c2);
+        }
+        // the key of a vector: its first class stands for the place of its maximum, vectors being disjoint ranges of classes
+        best_key = lane() < sp.nvec ? key_of(best, sp.first_class(at) + VEC - 1) : 0;
+        if (lane() < sp.edges()) {
+            const float l = sis3d_f32(sp.row[sp.edge_class(lane())]);
+            so.raise(fmaxf(so.m, l), a.c2);
+            so.add(l, a.c2);
+        }
+        for (int o = 32; o > 0; o >>= 1) so.join_xor(o, a.c2);
+        if constexpr (W > 1) {
+            if ((threadIdx.x & 63) == 0) {
+                sh.red[threadIdx.x >> 6][0] = so.m;
+                sh.red[threadIdx.x >> 6][1] = so.s;
+                sh.red[threadIdx.x >> 6][2] = so.t;
+            }
+            __syncthreads();
+            so = Soft{sh.red[0][0], sh.red[0][1], sh.red[0][2]};
+#pragma unroll
+            for (int w = 1; w < W; ++w) so.join(sh.red[w][0], sh.red[w][1], sh.red[w][2], a.c2);
+        }
+        return so;
+    }
+
+    // the `top` largest keys of the span, out(rank, key) once for each rank that exists
+    template <typename F> static __device__ void alternatives(const RowArgs &a, const Span<T> &sp, Shared &sh, uint64_t best_key, F out)
+    {
+        const int n = sp.nvec * VEC + sp.edges(), want = a.top < n ? a.top : n;
+        int groups = 1;
+        while (groups < want) groups *= 2;
+        // a bound that at least `want` elements of this wave's vectors reach; 0 where a group has no vector
+        uint64_t b = best_key;
+        for (int o = 32; o >= groups; o >>= 1) b = max64(b, shfl_xor64(b, o));
+        for (int o = groups >> 1; o > 0; o >>= 1) b = min64(b, shfl_xor64(b, o));
+        if (lane() == 0) sh.count = 0;
+        if constexpr (W > 1) {
+            if ((threadIdx.x & 63) == 0) sh.bound[threadIdx.x >> 6] = b;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < W; ++w) b = max64(b, sh.bound[w]);
+        } else team_sync<W>();
+        // lanes of this wave that have to be read again
+        const int w = W == 1 ? 0 : threadIdx.x >> 6, ln = threadIdx.x & 63;
+        const bool again = best_key != 0 && best_key >= b;
+        const uint64_t mask = __ballot(again);
+        if (again) sh.lanes[w][__popcll(mask & ((1ull << ln) - 1))] = ln;
+        team_sync<W>();
+        auto offer = [&](uint64_t k) {
+            if (k >= b) {
+                const int i = atomicAdd(&sh.count, 1);
+                if (i < CAP) sh.cand[i] = k;
+            }
+        };
+        const int per = (sp.nvec + NL - 1) / NL, items = __popcll(mask) * per;
+        for (int i = ln; i < items; i += 64) {
+            const int j = i / per, v = sh.lanes[w][j] + w * 64 + (i - j * per) * NL;
+            if (v >= sp.nvec) continue;
+            float x[VEC];
+            sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) offer(key_of(x[e], sp.first_class(v) + e));
+        }
+        if (lane() < sp.edges()) {
+            const int c = sp.edge_class(lane());
+            offer(key_of(sis3d_f32(sp.row[c]), c));
+        }
+        team_sync<W>();
+        const int m = sh.count;
+        if (m <= CAP) {
+            for (int i = lane(); i < m; i += NL) {
+                const uint64_t k = sh.cand[i];
+                int rank = 0;
+                for (int j = 0; j < m; ++j) rank += sh.cand[j] > k;
+                if (rank < want) out(rank, k);
+            }
+            team_sync<W>();
+            return;
+        }
+        // more elements at the bound than there is room for (rows made for it): the largest below the last one, `want` times
+        uint64_t last = ~0ull;
+        for (int r = 0; r < want; ++r) {
+            uint64_t k = 0;
+            for (int c = sp.k0 + lane(); c < sp.k0 + n; c += NL) {
+                const uint64_t q = key_of(sis3d_f32(sp.row[c]), c);
+                if (q < last) k = max64(k, q);
+            }
+            for (int o = 32; o > 0; o >>= 1) k = max64(k, shfl_xor64(k, o));
+            if constexpr (W > 1) {
+                __syncthreads();
+                if (ln == 0) sh.bound[w] = k;
+                __syncthreads();
+                for (int i = 0; i < W; ++i) k = max64(k, sh.bound[i]);
+            }
+            if (lane() == 0) out(r, k);
+            last = k;
+        }
+        team_sync<W>();
+    }
+};
+
+// a wave as the lanes of one row
+__device__ inline Group wave_group(int64_t r)
+{
+    Group g;
+    g.r = g.at = r;
+    g.sub = threadIdx.x & 63;
+    g.lpr = 64;
+    g.step = 1;
+    g.in = g.live = true;
+    return g;
+}
+
+template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t r, const T *row, float2 norm)
+{
+    const Group g = wave_group(r);
+    const Teacher t = group_teacher(a, g);
+    const float loss = a.tau * a.tau * group_sum(teacher_loss(a, g, t, row, norm), g);
+    if (g.sub == 0) {
+        a.loss[r] = t.bad ? NAN : loss;
+        a.norm[r] = norm;
+    }
+}
+
+template <typename T> __device__ inline void row_outputs(const RowArgs &a, int64_t r, const T *row, const Soft &so, float2 norm)
+{
+    const int64_t y = a.labels[r];
+    a.logp[r] = label_logp(a, r, y >= 0 && y < a.K ? sis3d_f32(row[y]) : 0.f, norm);
+    a.entropy[r] = so.entropy();
+    a.norm[r] = norm;
+}
+
+// outputs of a row past the live count, by a team of `n` lanes
+template <int MODE> __device__ inline void zero_row(const RowArgs &a, int64_t r, int lane, int n)
+{
+    if (lane == 0) {
+        a.norm[r] = make_float2(0.f, 0.f);
+        if constexpr (MODE == KD) a.loss[r] = 0.f;
+        else a.logp[r] = a.entropy[r] = 0.f;
+    }
+    if constexpr (MODE == LP)
+        for (int i = lane; i < a.top; i += n) {
+            a.top_logp[r * a.top + i] = 0.f;
+            a.top_class[r * a.top + i] = 0;
+        }
+}
+
+template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void long_forward(RowArgs a)
+{
+    using L = Long<T, W, MODE>;
+    __shared__ typename L::Shared shared[4 / W];
+    auto &sh = shared[W == 1 ? threadIdx.x >> 6 : 0];
+    const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (r >= a.R) return;                                  // the whole team
+    if (r >= live_rows(a)) { zero_row<MODE>(a, r, L::lane(), L::NL); return; }
+    const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
+    const Span<T> sp(row, 0, a.K);
+    uint64_t best;
+    const Soft so = L::pass(a, sp, sh, best);
+    const float2 norm = so.norm();
+    if constexpr (MODE == KD) {
+        if (W == 1 || threadIdx.x < 64) wave_loss(a, r, row, norm);
+    } else {
+        if (L::lane() == 0) row_outputs(a, r, row, so, norm);
+        if (a.top)
+            L::alternatives(a, sp, sh, best, [&](int rank, uint64_t k) {
+                a.top_class[r * a.top + rank] = key_class(k);
+                a.top_logp[r * a.top + rank] = log_p(key_score(k), norm, 1.f, 0.f);
+            });
+    }
+}
+
+// one part of a row to a workgroup
+template <typename T, int MODE> __global__ __launch_bounds__(256) void split_forward(RowArgs a)
+{
+    using L = Long<T, 4, MODE>;
+    __shared__ typename L::Shared sh;
+    const int64_t r = blockIdx.x / a.parts;
+    const int part = blockIdx.x - (int)(r * a.parts);
+    if (r >= live_rows(a)) return;
+    const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
+    const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
+    const Span<T> sp(row, k0, k1);
+    uint64_t best;
+    const Soft so = L::pass(a, sp, sh, best);
+    if (threadIdx.x == 0) *(float4 *)(a.part + (size_t)blockIdx.x * 4) = make_float4(so.m, so.s, so.t, 0.f);
+    if constexpr (MODE == LP)
+        if (a.top) L::alternatives(a, sp, sh, best, [&](int rank, uint64_t k) { a.part_keys[(size_t)blockIdx.x * a.top + rank] = k; });
+}
+
+// joins the parts of a row: one wave
+template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join(RowArgs a)
+{
+    __shared__ uint64_t cand[64 * TOP_MAX];
+    __shared__ int count;
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x;
+    if (r >= live_rows(a)) { zero_row<MODE>(a, r, lane, 64); return; }
+    const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
+    Soft so;
+    so.init();
+    if (lane < a.parts) {
+        const float4 v = *(const float4 *)(a.part + ((size_t)r * a.parts + lane) * 4);
+        so = Soft{v.x, v.y, v.z};
+    }
+    for (int o = 32; o > 0; o >>= 1) so.join_xor(o, a.c2);
+    const float2 norm = so.norm();
+    if constexpr (MODE == KD) {
+        wave_loss(a, r, row, norm);
+    } else {
+        if (lane == 0) row_outputs(a, r, row, so, norm);
+        if (!a.top) return;
+        // a part's last alternative bounds the row's from below: only keys that reach the largest of these bounds are ranked
+        const uint64_t *keys = a.part_keys + (size_t)r * a.parts * a.top;
+        uint64_t b = lane < a.parts ? keys[lane * a.top + a.top - 1] : 0;
+        for (int o = 32; o > 0; o >>= 1) b = max64(b, shfl_xor64(b, o));
+        if (lane == 0) count = 0;
+        __syncthreads();
+        for (int i = lane; i < a.parts * a.top; i += 64)
+            if (keys[i] >= b) cand[atomicAdd(&count, 1)] = keys[i];
+        __syncthreads();
+        for (int i = lane; i < count; i += 64) {
+            const uint64_t k = cand[i];
+            int rank = 0;
+            for (int j = 0; j < count; ++j) rank += cand[j] > k;
+            if (rank < a.top) {
+                a.top_class[r * a.top + rank] = key_class(k);
+                a.top_logp[r * a.top + rank] = log_p(key_score(k), norm, 1.f, 0.f);
+            }
+        }
+    }
+}
+
+// gradient of a row's part; `parts` workgroups or one team to a row
+template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void long_backward(RowArgs a)
+{
+    constexpr int NL = 64 * W, VEC = 16 / sizeof(T);
+    __shared__ float q_s[4 / W][KEPT_MAX];
+    __shared__ int c_s[4 / W][KEPT_MAX];
+    const int team = W == 1 ? threadIdx.x >> 6 : 0, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t item = W == 1 ? (int64_t)blockIdx.x * 4 + team : blockIdx.x, r = item / a.parts;
+    if (r >= a.R) return;
+    const int part = (int)(item - r * a.parts);
+    const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
+    const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
+    T *out = (T *)a.dscore + row_at(a, r, a.d_n, a.d_v);
+    if (r >= live_rows(a)) {
+        for (int c = k0 + lane; c < k1; c += NL) out[c] = sis3d_from_f32<T>(0.f);
+        return;
+    }
+    const float2 norm = a.norm_in[r];
+    float ga, ge = 0.f, h = 0.f;
+    int y = -1;
+    if constexpr (MODE == LP) {
+        const int64_t label = a.labels[r];
+        h = a.entropy_in[r];
+        ga = label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[r]);
+        ge = a.g2 ? a.g2[r] : 0.f;
+        y = label >= 0 && label < a.K ? (int)label : -1;
+    } else {
+        const Teacher t = group_teacher(a, wave_group(r));
+        if (W == 1 || threadIdx.x < 64)
+            for (int i = lane; i < a.nk; i += 64) {
+                const int64_t c = a.cls[r * a.nk + i];
+                const bool on = t.any && entry(a, c) == 1;
+                c_s[team][i] = on ? (int)c : -1;
+                q_s[team][i] = on ? exp2_((a.kept[r * a.nk + i] - t.m) * a.c2) / t.s : 0.f;
+            }
+        ga = t.bad ? NAN : (t.any ? a.g1[r] * a.tau : 0.f);
+    }
+    const Span<T> sp(row, k0, k1);
+    auto grad = [&](float l, int c) {
+        if constexpr (MODE == LP) return lp_grad(l, norm, h, ga, ge) + (c == y ? ga : 0.f);
+        else return ga * kd_p(a, l, norm);
+    };
+    const bool wide = ((uintptr_t)(out + k0 + sp.head) & 15) == 0;
+    for (int v = lane; v < sp.nvec; v += NL) {
+        float x[VEC];
+        sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
+        const int c = sp.first_class(v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[i] = grad(x[i], c + i);
+        if (wide) sis3d_store<T, VEC>(out + c, x);
+        else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) out[c + i] = sis3d_from_f32<T>(x[i]);
+        }
+    }
+    if (lane < sp.edges()) {
+        const int c = sp.edge_class(lane);
+        out[c] = sis3d_from_f32<T>(grad(sis3d_f32(row[c]), c));
+    }
+    if constexpr (MODE == KD) {
+        // the kept classes of this part again, with the teacher's share: written behind the team's own stores.  A class that is kept
+        // twice is written by its first entry with the sum of both.
+        team_sync<W>();
+        for (int i = lane; i < a.nk; i += NL) {
+            const int c = c_s[team][i];
+            if (c < k0 || c >= k1) continue;
+            float q = 0.f;
+            bool first = true;
+            for (int j = 0; j < a.nk; ++j)
+                if (c_s[team][j] == c) {
+                    q += q_s[team][j];
+                    first = first && j >= i;
+                }
+            if (first) out[c] = sis3d_from_f32<T>(ga * (kd_p(a, sis3d_f32(row[c]), norm) - q));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ host --
+// few long rows: parts of at least 4096 classes, enough for two workgroups per CU, at most one per lane of the joining wave
+int parts_of(int64_t R, int K, int64_t s_c)
+{
+    if (K <= K_WAVE || s_c != 1 || R >= 256) return 1;
+    int64_t p = (512 + R - 1) / R;
+    if (p > K / 4096) p = K / 4096;
+    return (int)(p > 64 ? 64 : (p < 1 ? 1 : p));
+}
+
+template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
+{
+    if (a.K <= K_SMALL) {
+        const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
+        const dim3 grid((unsigned)((waves + 3) / 4));
+        const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
+        if (e <= 2) hipLaunchKernelGGL((small_forward<T, 2, MODE>), grid, dim3(256), 0, st, a);
+        else if (e <= 4) hipLaunchKernelGGL((small_forward<T, 4, MODE>), grid, dim3(256), 0, st, a);
+        else if (e <= 8) hipLaunchKernelGGL((small_forward<T, 8, MODE>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((small_forward<T, 16, MODE>), grid, dim3(256), 0, st, a);
+        return sis3d_check_launch();
+    }
+    if (a.parts > 1) {
+        hipLaunchKernelGGL((split_forward<T, MODE>), dim3((unsigned)(a.R * a.parts)), dim3(256), 0, st, a);
+        const int rc = sis3d_check_launch();
+        if (rc) return rc;
+        hipLaunchKernelGGL((split_join<T, MODE>), dim3((unsigned)a.R), dim3(64), 0, st, a);
+    } else if (a.K <= K_WAVE) hipLaunchKernelGGL((long_forward<T, 1, MODE>), dim3((unsigned)((a.R + 3) / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((long_forward<T, 4, MODE>), dim3((unsigned)a.R), dim3(256), 0, st, a);
+    return sis3d_check_launch();
+}
+
+template <typename T, int MODE> int run_backward(RowArgs &a, hipStream_t st)
+{
+    if (a.K <= K_SMALL) {
+        const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
+        const dim3 grid((unsigned)((waves + 3) / 4));
+        const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
+        if (e <= 2) hipLaunchKernelGGL((small_backward<T, 2, MODE>), grid, dim3(256), 0, st, a);
+        else if (e <= 4) hipLaunchKernelGGL((small_backward<T, 4, MODE>), grid, dim3(256), 0, st, a);
+        else if (e <= 8) hipLaunchKernelGGL((small_backward<T, 8, MODE>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((small_backward<T, 16, MODE>), grid, dim3(256), 0, st, a);
+        return sis3d_check_launch();
+    }
+    if (a.K <= K_WAVE) hipLaunchKernelGGL((long_backward<T, 1, MODE>), dim3((unsigned)((a.R + 3) / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((long_backward<T, 4, MODE>), dim3((unsigned)(a.R * a.parts)), dim3(256), 0, st, a);
+    return sis3d_check_launch();
+}
+
+template <int MODE> int run(RowArgs &a, int dtype, bool backward, hipStream_t st)
+{
+    switch (dtype) {
+    case SIS3D_F32: return backward ? run_backward<float, MODE>(a, st) : run_forward<float, MODE>(a, st);
+    case SIS3D_BF16: return backward ? run_backward<__bf16, MODE>(a, st) : run_forward<__bf16, MODE>(a, st);
+    default: return backward ? run_backward<_Float16, MODE>(a, st) : run_forward<_Float16, MODE>(a, st);
+    }
+}
+
+// the arguments that all four entry points share; EUNSUPPORTED for scores that are neither short nor contiguous along the classes
+int fill(RowArgs &a, const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c, const int32_t *num)
+{
+    if (!sis3d_elem_bytes(dtype) || N < 0 || V < 0 || K <= 0) return SIS3D_EINVAL;
+    if (V && N > ((int64_t)1 << 40) / V) return SIS3D_EUNSUPPORTED;
+    a.score = score; a.N = N; a.V = V; a.R = N * V; a.K = K; a.s_n = s_n; a.s_v = s_v; a.s_c = s_c; a.num = num;
+    if (K > K_SMALL && s_c != 1) return SIS3D_EUNSUPPORTED;
+    if (((uintptr_t)score) % sis3d_elem_bytes(dtype)) return SIS3D_EINVAL;
+    a.planar = s_c != 1 && s_v < s_c;
+    a.lpr_log = 0;
+    while (a.lpr_log < 6 && (8 << a.lpr_log) < K) ++a.lpr_log;
+    a.parts = parts_of(a.R, K, s_c);
+    if (a.R * a.parts > 0x7fffffff) return SIS3D_EUNSUPPORTED;
+    return SIS3D_OK;
+}
+
+void temperature(RowArgs &a, float t)
+{
+    const double inv = 1.0 / t;
+    a.tau = t;
+    a.inv = (float)inv;
+    a.inv_lo = (float)(inv - a.inv);
+    a.c2 = (float)(1.4426950408889634 * inv);
+}
+
+size_t ws_of(int64_t R, int parts, int top) { return parts > 1 ? (size_t)R * parts * (16 + 8 * (size_t)top) : 0; }
+
+} // namespace
+
+extern "C" size_t sis3d_class_rows_workspace_bytes(int64_t rows, int K, int64_t s_c, int top)
+{
+    return rows > 0 && K > 0 ? ws_of(rows, parts_of(rows, K, s_c), top > 0 ? top : 0) : 0;
+}
+
+extern "C" int sis3d_class_logprobs_forward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,
+                                            const int64_t *labels, const int32_t *num_rows, int top, float *logp, float *entropy,
+                                            float *norm, float *top_logp, int64_t *top_class, void *workspace, size_t workspace_bytes,
+                                            sis3d_stream_t stream)
+{
+    RowArgs a{};
+    const int rc = fill(a, score, dtype, N, V, K, s_n, s_v, s_c, num_rows);
+    if (rc) return rc;
+    if (top < 0 || top > TOP_MAX || top > K) return SIS3D_EINVAL;
+    if (a.R == 0) return SIS3D_OK;
+    if (!score || !labels || !logp || !entropy || !norm || (top && (!top_logp || !top_class))) return SIS3D_EINVAL;
+    if (workspace_bytes < ws_of(a.R, a.parts, top)) return SIS3D_EWORKSPACE;
+    if (a.parts > 1 && (!workspace || ((uintptr_t)workspace & 15))) return SIS3D_EINVAL;
+    a.labels = labels; a.top = top; a.logp = logp; a.entropy = entropy; a.norm = (float2 *)norm; a.top_logp = top_logp; a.top_class = top_class;
+    a.part = (float *)workspace;
+    a.part_keys = (uint64_t *)((char *)workspace + (size_t)a.R * a.parts * 16);
+    temperature(a, 1.f);
+    return run<LP>(a, dtype, false, as_stream(stream));
+}
+
+extern "C" int sis3d_class_logprobs_backward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,
+                                             const int64_t *labels, const int32_t *num_rows, const float *norm, const float *entropy,
+                                             const float *grad_logp, const float *grad_entropy, void *dscore, int64_t d_n, int64_t d_v,
+                                             int64_t d_c, sis3d_stream_t stream)
+{
+    RowArgs a{};
+    const int rc = fill(a, score, dtype, N, V, K, s_n, s_v, s_c, num_rows);
+    if (rc) return rc;
+    if (K > K_SMALL && d_c != 1) return SIS3D_EUNSUPPORTED;
+    if (a.R == 0) return SIS3D_OK;
+    if (!score || !labels || !norm || !entropy || !grad_logp || !dscore) return SIS3D_EINVAL;
+    a.labels = labels; a.norm_in = (const float2 *)norm; a.entropy_in = entropy; a.g1 = grad_logp; a.g2 = grad_entropy;
+    a.dscore = dscore; a.d_n = d_n; a.d_v = d_v; a.d_c = d_c;
+    temperature(a, 1.f);
+    return run<LP>(a, dtype, true, as_stream(stream));
+}
+
+extern "C" int sis3d_distill_forward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,
+                                     const float *kept, const int64_t *classes, int nkept, const int32_t *num_rows, float temp, float *loss,
+                                     float *norm, void *workspace, size_t workspace_bytes, sis3d_stream_t stream)
+{
+    RowArgs a{};
+    const int rc = fill(a, score, dtype, N, V, K, s_n, s_v, s_c, num_rows);
+    if (rc) return rc;
+    if (nkept < 1 || nkept > KEPT_MAX || !(temp >= 1e-3f && temp <= 1e3f)) return SIS3D_EINVAL;
+    if (a.R == 0) return SIS3D_OK;
+    if (!score || !kept || !classes || !loss || !norm) return SIS3D_EINVAL;
+    if (workspace_bytes < ws_of(a.R, a.parts, 0)) return SIS3D_EWORKSPACE;
+    if (a.parts > 1 && (!workspace || ((uintptr_t)workspace & 15))) return SIS3D_EINVAL;
+    a.kept = kept; a.cls = classes; a.nk = nkept; a.loss = loss; a.norm = (float2 *)norm;
+    a.part = (float *)workspace;
+    temperature(a, temp);
+    return run<KD>(a, dtype, false, as_stream(stream));
+}
+
+extern "C" int sis3d_distill_backward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,
+                                      const float *kept, const int64_t *classes, int nkept, const int32_t *num_rows, float temp,
+                                      const float *norm, const float *grad_loss, void *dscore, int64_t d_n, int64_t d_v, int64_t d_c,
+                                      sis3d_stream_t stream)
+{
+    RowArgs a{};
+    const int rc = fill(a, score, dtype, N, V, K, s_n, s_v, s_c, num_rows);
+    if (rc) return rc;
+    if (nkept < 1 || nkept > KEPT_MAX || !(temp >= 1e-3f && temp <= 1e3f)) return SIS3D_EINVAL;
+    if (K > K_SMALL && d_c != 1) return SIS3D_EUNSUPPORTED;
+    if (a.R == 0) return SIS3D_OK;
+    if (!score || !kept || !classes || !norm || !grad_loss || !dscore) return SIS3D_EINVAL;
+    a.kept = kept; a.cls = classes; a.nk = nkept; a.norm_in = (const float2 *)norm; a.g1 = grad_loss;
+    a.dscore = dscore; a.d_n = d_n; a.d_v = d_v; a.d_c = d_c;
+    temperature(a, temp);
+    return run<KD>(a, dtype, true, as_stream(stream));
+}

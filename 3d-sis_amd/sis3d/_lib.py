@@ -114,6 +114,20 @@ SIGNATURES = {
     "sis3d_enet_conv1": (c_int, [c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "sis3d_enet_block": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int,
                                  c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_vp]),
+    "sis3d_group_norm_workspace_bytes": (c_sz, [c_int, c_int, c_i64, c_int, c_int, c_int, c_int]),
+    "sis3d_group_norm_forward": (c_int, [c_vp, c_int, c_int, c_i64, c_vp, c_i64, c_i64, c_int, c_int, c_vp, c_vp, c_f32, c_int, c_vp, c_i64,
+                                         c_i64, c_int, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "sis3d_group_norm_backward": (c_int, [c_vp, c_i64, c_i64, c_vp, c_int, c_int, c_i64, c_vp, c_i64, c_i64, c_int, c_int, c_vp, c_vp, c_vp,
+                                          c_vp, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "sis3d_class_rows_workspace_bytes": (c_sz, [c_i64, c_int, c_i64, c_int]),
+    "sis3d_class_logprobs_forward": (c_int, [c_vp, c_int, c_int, c_i64, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp,
+                                             c_vp, c_vp, c_sz, c_vp]),
+    "sis3d_class_logprobs_backward": (c_int, [c_vp, c_int, c_int, c_i64, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                              c_i64, c_i64, c_i64, c_vp]),
+    "sis3d_distill_forward": (c_int, [c_vp, c_int, c_int, c_i64, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_f32, c_vp, c_vp, c_vp,
+                                      c_sz, c_vp]),
+    "sis3d_distill_backward": (c_int, [c_vp, c_int, c_int, c_i64, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_f32, c_vp, c_vp, c_vp,
+                                       c_i64, c_i64, c_i64, c_vp]),
     "sis3d_planar_to_cl": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp]),
     "sis3d_cl_to_planar": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp]),
 }

@@ -1,0 +1,28 @@
+"""Autograd form of ops.group_norm."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+
+class GroupNormAct(torch.autograd.Function):
+    """`GroupNormAct.apply(x, weight, bias, groups, eps, act, offsets)` -> y: ops.group_norm with gradients for x, weight and bias."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps=1e-5, act=None, offsets=None):
+        y, mean, rstd = ops.group_norm(x, groups, weight, bias, eps, act=act, offsets=offsets, want_stats=True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd, offsets)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd, offsets = ctx.saved_tensors
+        try:
+            ops._channel_rows(dy, "dy", offsets)
+        except ops._lib.Sis3dError:                 # autograd may hand in any layout (an expanded sum's gradient, a planar one)
+            d = ops._like_rows(x, offsets)
+            dy = d.copy_(dy)
+        dx, dw, db = ops.group_norm_backward(dy, x, mean, rstd, ctx.groups, weight, bias, act=ctx.act, offsets=offsets)
+        return dx, dw, db, None, None, None, None

@@ -10,6 +10,7 @@ import torch.nn as nn
 
 from .. import ops
 from ..config import cfg as _default_cfg
+from ..layer_utils.group_norm import GroupNormAct
 from .network import Network
 
 
@@ -62,6 +63,19 @@ class HipMaxPool3d(nn.Module):
 
     def forward(self, x, out=None, out_coff=0):
         return ops.maxpool3(ops.to_cl(x), out, out_coff)
+
+
+class HipGroupNorm(nn.GroupNorm):
+    """nn.GroupNorm parameters and state_dict keys on channels-last activations, with the activation behind it fused (act: None,
+    'relu', 'silu'): the normalisation for training on one chunk per GPU.  Differentiable; `offsets` (RaggedBatch.offsets) normalises
+    every crop of a packed (voxels, C) batch by itself."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, act=None):
+        super().__init__(num_groups, num_channels, eps=eps, affine=affine)
+        self.act = act
+
+    def forward(self, x, offsets=None):
+        return GroupNormAct.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.act, offsets)
 
 
 class Bottleneck(nn.Module):

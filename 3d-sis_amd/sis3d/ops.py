@@ -1600,6 +1600,17 @@ class RaggedBatch:
               "sis3d_conv3d_k3t16_ragged")
         return out
 
+    def offsets(self):
+        """first row of every crop and the row count, int64 on the device: what group_norm takes to normalise each crop by itself"""
+        hit = self._tables.get("offsets")
+        if hit is None:
+            hit = self._tables["offsets"] = torch.from_numpy(self.voffs).to(self.device)
+        return hit
+
+    def group_norm(self, src, groups, weight=None, bias=None, eps=1e-5, act=None):
+        """(voxels, C) -> (voxels, C): every crop normalised by its own statistics"""
+        return group_norm(src, groups, weight, bias, eps, act=act, offsets=self.offsets())
+
     def views(self, out):
         res = []
         NC = out.shape[1]
@@ -1631,3 +1642,296 @@ def maxpool3(x, out=None, out_coff=0):
         raise _lib.Sis3dError("maxpool3: bad `out`")
     check(lib().sis3d_maxpool3d_3x3x3(_ptr(x), X, Y, Z, C, _ptr(out), out.shape[1], int(out_coff), _stream()), "sis3d_maxpool3d_3x3x3")
     return out
+
+
+# ------------------------------------------------- normalisation and class rows --
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/sis3d.h SIS3D_F32 / SIS3D_BF16 / SIS3D_F16
+_ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2}
+
+
+def _on_device(fn):
+    """run on the device of the first tensor argument (and on that device's current stream), whatever the current device is"""
+    import functools
+
+    @functools.wraps(fn)
+    def call(x, *args, **kwargs):
+        if isinstance(x, torch.Tensor) and x.is_cuda and x.device.index != torch.cuda.current_device():
+            with torch.cuda.device(x.device):
+                return fn(x, *args, **kwargs)
+        return fn(x, *args, **kwargs)
+    return call
+
+
+def _elem(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise _lib.Sis3dError("%s must be a CUDA/ROCm tensor (sis3d has no CPU path)" % name)
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise _lib.Sis3dError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return code
+
+
+def _side(t, name, like, dtype, shape, optional=True):
+    """a contiguous companion tensor of `like`: type, shape and device are checked"""
+    if t is None and optional:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != dtype:
+        raise _lib.Sis3dError("%s must be a %s tensor on %s" % (name, dtype, like.device))
+    if tuple(t.shape) != tuple(shape):
+        raise _lib.Sis3dError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _one_stride(sizes, strides):
+    """element stride of dimensions that are walked as one (0 elements or one: any), or None if no single stride does it"""
+    step, expect = 1, None
+    for n, s in zip(reversed(sizes), reversed(strides)):
+        if n == 1:
+            continue
+        if expect is None:
+            step = expect = s
+        elif s != expect:
+            return None
+        expect *= n
+    return step
+
+
+def _channel_rows(t, name, offsets):
+    """(samples, rows, channels, sample stride, row stride) of (N,C,*spatial) in channels-last memory, or of (rows, C) with offsets"""
+    shape, stride = t.shape, t.stride()
+    if offsets is not None:
+        if t.dim() != 2:
+            raise _lib.Sis3dError("%s must be (rows, C) with offsets" % name)
+        S, V, C = offsets.numel() - 1, shape[0], shape[1]
+        sn, sv, sc = 0, stride[0] if V > 1 else max(C, 1), stride[1]
+    else:
+        if t.dim() < 2:
+            raise _lib.Sis3dError("%s must be (N, C, ...)" % name)
+        S, C, sc = shape[0], shape[1], stride[1]
+        sn = stride[0] if S > 1 else 0
+        V = 1
+        for n in shape[2:]:
+            V *= n
+        sv = _one_stride(shape[2:], stride[2:])
+    if V == 1:
+        sv = C
+    if t.numel() and ((C > 1 and sc != 1) or sv is None or (V > 1 and sv < C)):
+        raise _lib.Sis3dError("%s must be channels-last in memory (or a channel range of such a tensor), got strides %s" % (name, tuple(stride)))
+    return S, V, C, sn, sv if sv is not None else C
+
+
+def _like_rows(x, offsets):
+    """an uninitialised tensor of x's shape and type, dense channels-last"""
+    if offsets is not None or x.dim() == 2:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = x.dim()
+    return torch.empty((x.shape[0],) + tuple(x.shape[2:]) + (x.shape[1],), dtype=x.dtype, device=x.device).permute(0, n - 1, *range(1, n - 1))
+
+
+def _norm_args(x, groups, weight, bias, act, offsets):
+    code = _elem(x, "x")
+    if offsets is not None:
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 1:
+            raise _lib.Sis3dError("offsets must be (samples + 1,) row offsets")
+        offsets = _side(offsets, "offsets", x, torch.int64, offsets.shape)
+    S, V, C, sn, sv = _channel_rows(x, "x", offsets)
+    groups = int(groups)
+    if groups < 1 or C < 1 or C % groups:
+        raise _lib.Sis3dError("group norm: %d channels do not split into %d groups" % (C, groups))
+    if act not in _ACTS:
+        raise _lib.Sis3dError("group norm: act must be one of 'none', 'relu', 'silu', got %r" % (act,))
+    weight = _side(weight, "weight", x, torch.float32, (C,))
+    bias = _side(bias, "bias", x, torch.float32, (C,))
+    return code, S, V, C, sn, sv, groups, weight, bias, offsets
+
+
+def _norm_check(rc, what, C, groups):
+    if rc == -4:
+        raise Sis3dUnsupported("%s: %d channels in %d groups are more than a workgroup takes" % (what, C, groups))
+    check(rc, what)
+
+
+@_on_device
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act=None, offsets=None, out=None, want_stats=False):
+    """act(group norm of x) in channels-last memory (sis3d_group_norm_forward): the normalisation for one chunk per GPU.
+
+    x: (N,C,*spatial), fp32 / bf16 / fp16, channels-last (dense, or a channel range of a wider tensor), statistics per sample and
+    group; or, with offsets (S+1,) int64 on the device, (rows, C) of which sample s is [offsets[s], offsets[s+1]) -- the packing of
+    RaggedBatch.  weight / bias (C,) fp32 or None; act: None / 'none', 'relu', 'silu'.  out: where to write (x itself is allowed, any
+    other overlap is not); rows behind offsets[-1] are left as they are in `out`, and zero without it.
+    -> y, or (y, mean, rstd) with want_stats: (samples, groups) fp32 for group_norm_backward."""
+    code, S, V, C, sn, sv, groups, weight, bias, offsets = _norm_args(x, groups, weight, bias, act, offsets)
+    if out is None:
+        y, yn, yv = _like_rows(x, offsets), V * C, C
+    else:
+        y = out
+        if _elem(out, "out") != code or out.shape != x.shape or out.device != x.device:
+            raise _lib.Sis3dError("group norm: `out` must have x's shape, type and device")
+        _, _, _, yn, yv = _channel_rows(out, "out", offsets)
+        if offsets is None and S > 1 and V > 0 and yn < (V - 1) * yv + C and (yn < C or yv < (S - 1) * yn + C):
+            raise _lib.Sis3dError("group norm: the samples of `out` overlap in memory")
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty(S, groups, dtype=torch.float32, device=x.device), torch.empty(S, groups, dtype=torch.float32, device=x.device)
+    ragged = 0 if offsets is None else 1
+    wsb = lib().sis3d_group_norm_workspace_bytes(code, S, V, ragged, C, groups, 0)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
+    _norm_check(lib().sis3d_group_norm_forward(_ptr(x), code, S, V, _ptr(offsets), sn, sv, C, groups, _ptr(weight), _ptr(bias), float(eps),
+                                               _ACTS[act], _ptr(y), yn, yv, 1 if out is None else 0, _ptr(mean), _ptr(rstd), _ptr(ws), wsb,
+                                               _stream()), "sis3d_group_norm_forward", C, groups)
+    return (y, mean, rstd) if want_stats else y
+
+
+@_on_device
+def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, act=None, offsets=None):
+    """gradients of group_norm (sis3d_group_norm_backward): dy like y, the call's own x, mean, rstd, weight, bias, act, offsets
+    -> (dx, dweight, dbias), the last two fp32, None where the parameter is None.  Sums are deterministic."""
+    code, S, V, C, sn, sv, groups, weight, bias, offsets = _norm_args(x, groups, weight, bias, act, offsets)
+    if _elem(dy, "dy") != code or dy.shape != x.shape or dy.device != x.device:
+        raise _lib.Sis3dError("group norm: dy must have x's shape, type and device")
+    _, _, _, dn, dv = _channel_rows(dy, "dy", offsets)
+    mean = _side(mean, "mean", x, torch.float32, (S, groups), optional=False)
+    rstd = _side(rstd, "rstd", x, torch.float32, (S, groups), optional=False)
+    dx = _like_rows(x, offsets)
+    dw = torch.empty(C, dtype=torch.float32, device=x.device) if weight is not None else None
+    db = torch.empty(C, dtype=torch.float32, device=x.device) if bias is not None else None
+    wsb = lib().sis3d_group_norm_workspace_bytes(code, S, V, 0 if offsets is None else 1, C, groups, 1)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
+    _norm_check(lib().sis3d_group_norm_backward(_ptr(dy), dn, dv, _ptr(x), code, S, V, _ptr(offsets), sn, sv, C, groups, _ptr(mean), _ptr(rstd),
+                                                _ptr(weight), _ptr(bias), _ACTS[act], _ptr(dx), V * C, C, _ptr(dw), _ptr(db), _ptr(ws), wsb,
+                                                _stream()), "sis3d_group_norm_backward", C, groups)
+    return dx, dw, db
+
+
+def _score_rows(score):
+    """(type, shape of the rows, outer count, rows, classes, three element strides) of (R,K) or (N,K,*spatial) class scores"""
+    code = _elem(score, "score")
+    if score.dim() < 2:
+        raise _lib.Sis3dError("score must be (rows, classes) or (N, classes, ...)")
+    shape, st = tuple(score.shape), score.stride()
+    K = shape[1]
+    if K < 1:
+        raise _lib.Sis3dError("score must have at least one class")
+    if score.dim() == 2:
+        N, V, sn, sv, rows = 1, shape[0], 0, st[0], shape[:1]
+    else:
+        N, sn, rows = shape[0], st[0], shape[:1] + shape[2:]
+        V = 1
+        for n in shape[2:]:
+            V *= n
+        sv = _one_stride(shape[2:], st[2:])
+        if sv is None:
+            raise _lib.Sis3dError("score: the dimensions behind the classes must be dense among themselves, got strides %s" % (tuple(st),))
+    sc = st[1] if K > 1 else 1
+    if K > 1024 and sc != 1:
+        raise Sis3dUnsupported("score: more than 1024 classes must be contiguous in memory (class stride %d)" % sc)
+    return code, rows, N, V, K, sn, sv, sc
+
+
+def _num_rows(num, like):
+    if num is None:
+        return None
+    if num.numel() != 1:
+        raise _lib.Sis3dError("num must hold one int32: the live rows")
+    return _side(num, "num", like, torch.int32, num.shape)
+
+
+def _like_score(score, sc):
+    """an uninitialised dense tensor of score's shape with the classes where they are in score: last in memory, or second"""
+    n, dev = score.dim(), score.device
+    shape = tuple(score.shape)
+    if n == 2:
+        return torch.empty(shape, dtype=score.dtype, device=dev) if sc == 1 else torch.empty(shape[::-1], dtype=score.dtype, device=dev).t()
+    if sc == 1 and shape[1] > 1:
+        return torch.empty(shape[:1] + shape[2:] + shape[1:2], dtype=score.dtype, device=dev).permute(0, n - 1, *range(1, n - 1))
+    return torch.empty(shape, dtype=score.dtype, device=dev)
+
+
+@_on_device
+def class_logprobs(score, labels, top=0, num=None):
+    """log probability of the given classes, entropy and the best alternatives of every row (sis3d_class_logprobs_forward).
+
+    score (R,K), or (N,K,*spatial) planar or channels-last, fp32 / bf16 / fp16; labels int64 (R,) or (N,*spatial): a negative label is
+    none (log probability 0).  num: int32 tensor with the number of live rows (detection passes pad theirs): outputs behind are 0.
+    -> (logp, entropy, norm, top_logp, top_class): logp / entropy fp32 like labels; norm (...,2) for the backward pass (a row's
+    largest score and the log of its sum relative to it: they add up to the row's log-sum-exp); top_logp fp32 / top_class int64
+    (...,top), best first, the lowest class first among equal scores; top <= min(32, K)."""
+    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    top = int(top)
+    if not 0 <= top <= min(32, K):
+        raise _lib.Sis3dError("class_logprobs: top must be 0 to %d, got %d" % (min(32, K), top))
+    labels = _side(labels, "labels", score, torch.int64, rows, optional=False)
+    num = _num_rows(num, score)
+    dev = score.device
+    logp, ent, norm, tl = (torch.empty(rows + tail, dtype=torch.float32, device=dev) for tail in ((), (), (2,), (top,)))
+    tc = torch.empty(rows + (top,), dtype=torch.int64, device=dev)
+    wsb = lib().sis3d_class_rows_workspace_bytes(N * V, K, sc, top)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    check(lib().sis3d_class_logprobs_forward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(labels), _ptr(num), top, _ptr(logp), _ptr(ent),
+                                             _ptr(norm), _ptr(tl), _ptr(tc), _ptr(ws), wsb, _stream()), "sis3d_class_logprobs_forward")
+    return logp, ent, norm, tl, tc
+
+
+@_on_device
+def class_logprobs_backward(score, labels, norm, entropy, grad_logp, grad_entropy=None, num=None):
+    """gradient of class_logprobs with respect to the scores, in the scores' type and layout (sis3d_class_logprobs_backward);
+    grad_logp / grad_entropy fp32 like labels"""
+    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    labels = _side(labels, "labels", score, torch.int64, rows, optional=False)
+    norm = _side(norm, "norm", score, torch.float32, rows + (2,), optional=False)
+    entropy = _side(entropy, "entropy", score, torch.float32, rows, optional=False)
+    grad_logp = _side(grad_logp, "grad_logp", score, torch.float32, rows, optional=False)
+    grad_entropy = _side(grad_entropy, "grad_entropy", score, torch.float32, rows)
+    num = _num_rows(num, score)
+    d = _like_score(score, sc)
+    _, _, _, _, _, dn, dv, dc = _score_rows(d)
+    check(lib().sis3d_class_logprobs_backward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(labels), _ptr(num), _ptr(norm), _ptr(entropy),
+                                              _ptr(grad_logp), _ptr(grad_entropy), _ptr(d), dn, dv, dc, _stream()),
+          "sis3d_class_logprobs_backward")
+    return d
+
+
+def _teacher(score, kept, classes, rows, temperature):
+    if not isinstance(kept, torch.Tensor) or kept.dim() != len(rows) + 1 or not 1 <= kept.shape[-1] <= 128:
+        raise _lib.Sis3dError("kept must be %s + (1 to 128 logits,)" % (tuple(rows),))
+    shape = rows + (kept.shape[-1],)
+    temperature = float(temperature)
+    if not 1e-3 <= temperature <= 1e3:
+        raise _lib.Sis3dError("temperature must be within 1e-3 and 1e3, got %r" % temperature)
+    return (_side(kept, "kept", score, torch.float32, shape, optional=False), _side(classes, "classes", score, torch.int64, shape, optional=False),
+            temperature)
+
+
+@_on_device
+def distill_loss(score, kept, classes, temperature=1.0, num=None):
+    """T^2 KL(teacher || student) of every row against a teacher's kept top logits (sis3d_distill_forward).
+
+    score: the student's scores, as class_logprobs takes them; kept (R,k) / (N,*spatial,k) fp32 teacher logits of `classes` (same shape,
+    int64; negative = absent, equal classes add up), k <= 128.  The teacher's distribution is the softmax of kept / T over the entries
+    that are present, the student's the softmax of score / T over all classes; a row without entries has loss 0.
+    -> (loss fp32 (R,) / (N,*spatial), norm for the backward pass)."""
+    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    kept, classes, temperature = _teacher(score, kept, classes, rows, temperature)
+    num = _num_rows(num, score)
+    loss, norm = (torch.empty(rows + tail, dtype=torch.float32, device=score.device) for tail in ((), (2,)))
+    wsb = lib().sis3d_class_rows_workspace_bytes(N * V, K, sc, 0)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=score.device) if wsb else None
+    check(lib().sis3d_distill_forward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(kept), _ptr(classes), kept.shape[-1], _ptr(num), temperature,
+                                      _ptr(loss), _ptr(norm), _ptr(ws), wsb, _stream()), "sis3d_distill_forward")
+    return loss, norm
+
+
+@_on_device
+def distill_loss_backward(score, kept, classes, norm, grad_loss, temperature=1.0, num=None):
+    """gradient of distill_loss with respect to the scores, in the scores' type and layout (sis3d_distill_backward); grad_loss fp32
+    like the loss"""
+    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    kept, classes, temperature = _teacher(score, kept, classes, rows, temperature)
+    norm = _side(norm, "norm", score, torch.float32, rows + (2,), optional=False)
+    grad_loss = _side(grad_loss, "grad_loss", score, torch.float32, rows, optional=False)
+    num = _num_rows(num, score)
+    d = _like_score(score, sc)
+    _, _, _, _, _, dn, dv, dc = _score_rows(d)
+    check(lib().sis3d_distill_backward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(kept), _ptr(classes), kept.shape[-1], _ptr(num), temperature,
+                                       _ptr(norm), _ptr(grad_loss), _ptr(d), dn, dv, dc, _stream()), "sis3d_distill_backward")
+    return d

@@ -35,6 +35,11 @@ extern "C" {
 
 typedef void *sis3d_stream_t; /* hipStream_t */
 
+/* element types of the entry points that take a `dtype` (everything else is fp32) */
+#define SIS3D_F32 0
+#define SIS3D_BF16 1
+#define SIS3D_F16 2
+
 int sis3d_abi_version(void);
 const char *sis3d_strerror(int code);
 /* last HIP error string recorded by a failing launch on this thread */
@@ -552,6 +557,64 @@ int sis3d_bottleneck_wino(const float *y1, int X, int Y, int Z, int planes, cons
  * range of a wider tensor = the torch.cat of backbones.py:109 done in place). */
 int sis3d_maxpool3d_3x3x3(const float *in, int X, int Y, int Z, int C, float *out, int out_stride, int out_coff,
                           sis3d_stream_t stream);
+
+/* Group norm with an activation on channels-last rows (csrc/group_norm.hip): the normalisation of a network that trains on ONE chunk
+ * per GPU.  Per (sample, group of C / G channels): mean and rstd = (var + eps)^-1/2 over the sample's rows and the group's channels
+ * (biased variance), y = act((x - mean) * rstd * weight + bias); act: SIS3D_ACT_*.
+ * x, y, dy, dx: `dtype` elements, row r of sample s at  s * sample stride + r * row stride  (elements), its C channels contiguous (a
+ * channel range of a wider tensor: the row stride is the wider one).  Dense (offsets NULL): S samples of `rows` rows.  Ragged: `rows`
+ * rows in one buffer, sample s = rows [offsets[s], offsets[s+1]), offsets [S+1] int64 on the DEVICE, ascending from 0; rows from
+ * offsets[S] on are left as they are (zero_tail = 0) or zeroed (1; what backward does with dx).  Samples may be empty (mean = rstd = 0).
+ * weight / bias [C] fp32, each may be NULL (1 / 0).  mean / rstd [S][G] fp32: forward writes them (both may be NULL), backward reads them.
+ * Statistics: 32-bit sums of differences to a nearby value per thread, 64-bit across threads; no atomics, results do not vary.
+ * backward also writes dweight / dbias [C] fp32 (each may be NULL), summed over all samples.  y may be x (in place); dx may be dy, not x.
+ * SIS3D_EUNSUPPORTED: more than 512 * (16 bytes / element) channels per group (512 where a pointer, a stride or C is not a multiple of
+ * 16 bytes).  workspace: 16-byte aligned, sis3d_group_norm_workspace_bytes (ragged: 0 / 1), any content. */
+#define SIS3D_ACT_NONE 0
+#define SIS3D_ACT_RELU 1
+#define SIS3D_ACT_SILU 2
+size_t sis3d_group_norm_workspace_bytes(int dtype, int S, int64_t rows, int ragged, int C, int G, int backward);
+int sis3d_group_norm_forward(const void *x, int dtype, int S, int64_t rows, const int64_t *offsets, int64_t x_sample, int64_t x_row,
+                             int C, int G, const float *weight, const float *bias, float eps, int act, void *y, int64_t y_sample,
+                             int64_t y_row, int zero_tail, float *mean, float *rstd, void *workspace, size_t workspace_bytes,
+                             sis3d_stream_t stream);
+int sis3d_group_norm_backward(const void *dy, int64_t dy_sample, int64_t dy_row, const void *x, int dtype, int S, int64_t rows,
+                              const int64_t *offsets, int64_t x_sample, int64_t x_row, int C, int G, const float *mean,
+                              const float *rstd, const float *weight, const float *bias, int act, void *dx, int64_t dx_sample,
+                              int64_t dx_row, float *dweight, float *dbias, void *workspace, size_t workspace_bytes,
+                              sis3d_stream_t stream);
+
+/* Rows of class scores (csrc/class_rows.hip): what the softmax / arg-max of the heads leaves out -- the log probability of GIVEN classes,
+ * entropy, the best alternatives -- and distillation from a teacher's kept logits, each with its gradient (the cross entropies of
+ * lib/nets/network.py:319-501 are -logp with the gradient of sis3d_class_logprobs_backward).
+ * score: `dtype` elements; N * V rows, row r = n * V + v at n * s_n + v * s_v, class c of it c * s_c further (element strides): rows
+ * (1, R, s_v = K, s_c = 1), channels-last and planar maps ((N,K,...) with s_c = V) alike.  K > 1024 needs s_c = 1 (else EUNSUPPORTED).
+ * num_rows: device int32, live rows (NULL: all); the rows behind are not read and their outputs are zero.
+ * norm [R][2]: the row's largest score m and log sum exp((l - m) / T); their sum (m / T + ...) is the row's log-sum-exp.
+ *   sis3d_class_logprobs_forward   logp [R] = log p(labels[r]) (0 where the label is negative, NaN where it is >= K), entropy [R] (nat),
+ *                                  top_logp / top_class [R][top] the largest scores in descending order, the lowest class first among equal
+ *                                  ones, NaN ranked with -inf.  top <= min(32, K), 0: none.  -inf scores have p = 0; a row of nothing but
+ *                                  -inf has logp = -inf, entropy 0, gradient 0 apart from the label's.
+ *   sis3d_class_logprobs_backward  dscore = grad_logp (1[c = label] - p) - grad_entropy p (log p + entropy); grad_entropy may be NULL
+ *   sis3d_distill_forward          loss [R] = T^2 KL(q || softmax(score / T)), q = softmax(kept / T) over the row's present entries: kept
+ *                                  [R][nkept] fp32 teacher logits of classes [R][nkept] int64, negative = absent, >= K makes the row NaN,
+ *                                  equal classes add up; no present entry: loss 0.  nkept <= 128, 1e-3 <= T <= 1e3.
+ *   sis3d_distill_backward         dscore = grad_loss T (p - q)
+ * workspace: 16-byte aligned, sis3d_class_rows_workspace_bytes(N * V, K, s_c, top) (0 for most calls; top = 0 for distillation). */
+size_t sis3d_class_rows_workspace_bytes(int64_t rows, int K, int64_t s_c, int top);
+int sis3d_class_logprobs_forward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,
+                                 const int64_t *labels, const int32_t *num_rows, int top, float *logp, float *entropy, float *norm,
+                                 float *top_logp, int64_t *top_class, void *workspace, size_t workspace_bytes, sis3d_stream_t stream);
+int sis3d_class_logprobs_backward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,
+                                  const int64_t *labels, const int32_t *num_rows, const float *norm, const float *entropy,
+                                  const float *grad_logp, const float *grad_entropy, void *dscore, int64_t d_n, int64_t d_v, int64_t d_c,
+                                  sis3d_stream_t stream);
+int sis3d_distill_forward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c, const float *kept,
+                          const int64_t *classes, int nkept, const int32_t *num_rows, float temp, float *loss, float *norm,
+                          void *workspace, size_t workspace_bytes, sis3d_stream_t stream);
+int sis3d_distill_backward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c, const float *kept,
+                           const int64_t *classes, int nkept, const int32_t *num_rows, float temp, const float *norm,
+                           const float *grad_loss, void *dscore, int64_t d_n, int64_t d_v, int64_t d_c, sis3d_stream_t stream);
 
 /* layout helpers: planar (C,X,Y,Z) <-> channels-last (X,Y,Z,C) */
 int sis3d_planar_to_cl(const float *in, int C, int64_t nvox, float *out, sis3d_stream_t stream);

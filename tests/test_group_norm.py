@@ -1,0 +1,447 @@
+"""Group norm with an activation on channels-last rows (csrc/group_norm.hip) against the formulas in 64 bits.
+
+Tolerances (u = 2^-24, the rounding of a 32-bit operation; half = eps(type) / 2, the rounding of a result):
+  h    (x - mu) r with mu and r rounded once: th = 4 u (|mu| r + |h|)
+  y    (x - mu) sc + b, sc = r w: ty = 16 u (|mu| r |w| + |h w| + |z| + |b|), which also holds the few roundings of a smooth activation
+       (its slope is at most 1.1); + half |y|
+  d    dy act'(z): SiLU's slope changes by at most 0.5 a unit of z: td = 0.5 ty |dy|, 0 for the others; te = td |w| for e = d w
+  dx   r (e - m1 - h m2): its own roundings, the errors of e, h, m1, m2, and sums of at most L rows a thread in m1 and m2; + half |dx|
+  dw   sum d h: a thread's chain of at most L additions, 64 bits behind it: sum (L u |d h| + td |h| + |d| th); db alike: sum (L u |d| + td)
+ReLU's slope jumps at 0: dy is 0 where |z| < 1e-3, so that a rounding of z cannot decide it."""
+import ctypes
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+EPS = 1e-5
+
+
+def reference(x, dy, offsets, groups, w, b, act, eps=EPS):
+    """x, dy: (rows, C) float64, offsets: list -> dict of float64 tensors, dy's zeroing near ReLU's corner included"""
+    C = x.shape[1]
+    c = C // groups
+    w = torch.ones(C, dtype=x.dtype, device=x.device) if w is None else w.double()
+    b = torch.zeros(C, dtype=x.dtype, device=x.device) if b is None else b.double()
+    out = {k: torch.zeros_like(x) for k in ("y", "z", "hw", "dx", "ty", "tdx")}
+    out["mean"], out["rstd"] = (torch.zeros(len(offsets) - 1, groups, dtype=x.dtype, device=x.device) for _ in range(2))
+    for k in ("dw", "db", "tdw", "tdb"):
+        out[k] = torch.zeros(C, dtype=x.dtype, device=x.device)
+    for s, (lo, hi) in enumerate(zip(offsets, offsets[1:])):
+        if hi == lo:
+            continue
+        v = x[lo:hi].reshape(hi - lo, groups, c)
+        mu = v.mean((0, 2), keepdim=True)
+        r = 1 / torch.sqrt(((v - mu) ** 2).mean((0, 2), keepdim=True) + eps)
+        h = (v - mu) * r
+        ws, bs = w.view(groups, c), b.view(groups, c)
+        z = h * ws + bs
+        sig = torch.sigmoid(z)
+        y = {"none": z, "relu": z.clamp_min(0), "silu": z * sig}[act]
+        slope = {"none": torch.ones_like(z), "relu": (z > 0).double(), "silu": sig * (1 + z * (1 - sig))}[act]
+        d = dy[lo:hi].reshape(v.shape) * slope
+        e = d * ws
+        m1, m2 = e.mean((0, 2), keepdim=True), (e * h).mean((0, 2), keepdim=True)
+        L = 16 + min(hi - lo, 4096)
+        put = lambda k, t: out[k].__setitem__(slice(lo, hi), t.reshape(hi - lo, C))       # noqa: E731
+        mean = lambda t: t.mean((0, 2), keepdim=True)                                    # noqa: E731
+        th = 4 * U * (mu.abs() * r + h.abs())
+        ty = 16 * U * (mu.abs() * r * ws.abs() + (h * ws).abs() + z.abs() + bs.abs())
+        td = 0.5 * ty * dy[lo:hi].reshape(v.shape).abs() * (act == "silu")
+        te = td * ws.abs()
+        put("y", y)
+        put("z", z)
+        put("dx", r * (e - m1 - h * m2))
+        put("ty", ty)
+        put("tdx", r * (32 * U * (e.abs() + m1.abs() + (h * m2).abs()) + te + m2.abs() * th + mean(te) + L * U * mean(e.abs())
+                        + h.abs() * (mean(te * h.abs() + e.abs() * th) + L * U * mean((e * h).abs()))))
+        out["mean"][s], out["rstd"][s] = mu.flatten(), r.flatten()
+        out["dw"] += (d * h).sum(0).flatten()
+        out["db"] += d.sum(0).flatten()
+        out["tdw"] += (L * U * (d * h).abs() + td * h.abs() + d.abs() * th).sum(0).flatten()
+        out["tdb"] += (L * U * d.abs() + td).sum(0).flatten()
+    return out
+
+
+def check_close(got, want, tol, name):
+    got = got.double()
+    bad = (got - want).abs() > tol
+    assert torch.isfinite(got).all(), name
+    assert not bad.any(), "%s: %d off, worst %.3g of its tolerance" % (name, int(bad.sum()), float(((got - want).abs() / (tol + 1e-30)).max()))
+
+
+def half_of(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def make(shape_rows, C, dtype, seed=0, shift=0.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g)                            # noqa: E731
+    x = (n(shape_rows, C) * (0.5 + torch.rand(C, device="cuda", generator=g)) + shift * n(C)).to(dtype)
+    return x, n(shape_rows, C).to(dtype), 1 + 0.3 * n(C), 0.3 * n(C)
+
+
+def away_from_corner(x, dy, offsets, groups, w, b, act):
+    z = reference(x.double(), dy.double(), offsets, groups, w, b, act)["z"]
+    return torch.where(z.abs() < 1e-3, torch.zeros_like(dy), dy)
+
+
+def run_rows(x, dy, offsets, groups, w, b, act):
+    from sis3d import ops
+    off = torch.tensor(offsets, device="cuda")
+    y, mean, rstd = ops.group_norm(x, groups, w, b, EPS, act=act, offsets=off, want_stats=True)
+    dx, dw, db = ops.group_norm_backward(dy, x, mean, rstd, groups, w, b, act=act, offsets=off)
+    return y, mean, rstd, dx, dw, db
+
+
+def compare_rows(got, want, dtype, has_w=True, has_b=True):
+    y, mean, rstd, dx, dw, db = got
+    h = half_of(dtype)
+    check_close(y, want["y"], want["ty"] + h * want["y"].abs(), "y")
+    check_close(dx, want["dx"], want["tdx"] + h * want["dx"].abs() + 1e-7 * (dtype == torch.float16), "dx")     # fp16: its smallest step
+    check_close(mean, want["mean"], 4 * U * (want["mean"].abs() + 1 / want["rstd"].clamp_min(1e-30) * (want["rstd"] > 0)), "mean")
+    check_close(rstd, want["rstd"], 8 * U * want["rstd"] * 4, "rstd")
+    if has_w:
+        check_close(dw, want["dw"], want["tdw"], "dw")
+    if has_b:
+        check_close(db, want["db"], want["tdb"], "db")
+
+
+CHANNELS = [(128, 32), (128, 1), (64, 8), (32, 32), (24, 8), (20, 4), (19, 19), (6, 3), (5, 1), (2, 1), (1, 1), (256, 2), (514, 2), (1024, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("C,G", CHANNELS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_ragged_rows_match_formula(dtype, C, G, act):
+    lens = [0, 1, 700, 0, 3, 129, 0]
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    x, dy, w, b = make(offsets[-1], C, dtype, seed=C * 7 + G)
+    dy = away_from_corner(x, dy, offsets, G, w, b, act)
+    compare_rows(run_rows(x, dy, offsets, G, w, b, act), reference(x.double(), dy.double(), offsets, G, w, b, act), dtype)
+
+
+def cl(rows, N, dims):
+    """(N*V, C) rows -> (N,C,*dims) in channels-last memory"""
+    t = rows.view((N,) + tuple(dims) + (rows.shape[1],))
+    n = t.dim()
+    return t.permute(0, n - 1, *range(1, n - 1))
+
+
+def rows_of(t):
+    n = t.dim()
+    return t.permute(0, *range(2, n), 1).reshape(-1, t.shape[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,dims,C,G,act", [(1, (12, 6, 12), 128, 16, "relu"), (1, (24, 12, 24), 64, 8, "silu"), (3, (5, 3, 7), 48, 16, "relu"),
+                                            (2, (33, 17), 20, 5, "silu"), (4, (), 32, 8, "none"), (1, (1, 1, 1), 64, 8, "relu"),
+                                            (2, (1, 1, 1), 8, 8, "silu"), (1, (96, 48, 96), 32, 8, "relu"), (7, (9,), 3, 1, "none")])
+@pytest.mark.parametrize("affine", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_dense_maps_match_formula(N, dims, C, G, act, affine, dtype):
+    from sis3d import ops
+    V = 1
+    for d in dims:
+        V *= d
+    offsets = [i * V for i in range(N + 1)]
+    x, dy, w, b = make(N * V, C, dtype, seed=V)
+    if not affine:
+        w = b = None
+    dy = away_from_corner(x, dy, offsets, G, w, b, act)
+    want = reference(x.double(), dy.double(), offsets, G, w, b, act)
+    xm, dm = cl(x, N, dims), cl(dy, N, dims)
+    y, mean, rstd = ops.group_norm(xm, G, w, b, EPS, act=act, want_stats=True)
+    dx, dw, db = ops.group_norm_backward(dm, xm, mean, rstd, G, w, b, act=act)
+    assert y.shape == xm.shape and dx.shape == xm.shape and (dw is None) == (w is None)
+    compare_rows((rows_of(y), mean, rstd, rows_of(dx), dw, db), want, dtype, affine, affine)
+    assert torch.equal(ops.group_norm(xm, G, w, b, EPS, act=act), y)           # without statistics, and the same bits again
+
+
+@pytest.mark.gpu
+def test_strides_slices_alignment_and_out():
+    """a channel range of a wider tensor, a view that starts off 16 bytes, interleaved samples, writing into a range and in place"""
+    from sis3d import ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn(2, 6, 5, 4, 96, device="cuda", generator=g).permute(0, 4, 1, 2, 3)
+    dyw = torch.randn(2, 6, 5, 4, 96, device="cuda", generator=g).permute(0, 4, 1, 2, 3)
+    for lo, hi, G in ((32, 64, 8), (1, 33, 4), (90, 96, 3)):
+        x, dy = wide[:, lo:hi], dyw[:, lo:hi]
+        dense = x.permute(0, 2, 3, 4, 1).contiguous()
+        n = hi - lo
+        w, b = torch.rand(n, device="cuda", generator=g), torch.rand(n, device="cuda", generator=g)
+        want = reference(dense.view(-1, n).double(), dy.permute(0, 2, 3, 4, 1).reshape(-1, n).double(), [0, 120, 240], G, w, b, "silu")
+        y, mean, rstd = ops.group_norm(x, G, w, b, act="silu", want_stats=True)
+        grads = ops.group_norm_backward(dy, x, mean, rstd, G, w, b, act="silu")
+        compare_rows((rows_of(y), mean, rstd, rows_of(grads[0])) + grads[1:], want, torch.float32)
+        target = torch.full_like(wide, 7.0)
+        before = target.clone()
+        assert ops.group_norm(x, G, w, b, act="silu", out=target[:, lo:hi]) .data_ptr() == target[:, lo:hi].data_ptr()
+        check_close(rows_of(target[:, lo:hi]), want["y"], want["ty"] + half_of(torch.float32) * want["y"].abs(), "out")
+        target[:, lo:hi] = 7.0
+        assert torch.equal(target, before)                                     # nothing beside the range
+        inplace = x.clone(memory_format=torch.preserve_format)
+        inplace = cl(rows_of(inplace).contiguous(), 2, (6, 5, 4))
+        ops.group_norm(inplace, G, w, b, act="silu", out=inplace)
+        check_close(rows_of(inplace), want["y"], want["ty"] + half_of(torch.float32) * want["y"].abs(), "in place")
+    # samples interleaved in memory: (voxels, samples, channels)
+    m = torch.randn(50, 3, 16, device="cuda", generator=g)
+    x = m.permute(1, 2, 0)
+    want = reference(m.permute(1, 0, 2).reshape(-1, 16).double(), torch.zeros(150, 16, device="cuda", dtype=torch.float64), [0, 50, 100, 150], 4, None, None, "none")
+    check_close(ops.group_norm(x, 4).permute(0, 2, 1).reshape(-1, 16), want["y"], want["ty"] + half_of(torch.float32) * want["y"].abs(), "interleaved")
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_sample_and_empty_batches():
+    from sis3d import ops
+    x, dy, w, b = make(1000, 32, torch.float32)
+    off = torch.tensor([0, 40, 40, 900], device="cuda")
+    out = torch.full((1000, 32), 3.0, device="cuda")
+    y, mean, rstd = ops.group_norm(x, 8, w, b, offsets=off, out=out, want_stats=True)
+    assert (y[900:] == 3.0).all()
+    assert (mean[1] == 0).all() and (rstd[1] == 0).all()
+    fresh = ops.group_norm(x, 8, w, b, offsets=off)
+    assert torch.equal(fresh[:900], y[:900]) and (fresh[900:] == 0).all()
+    dirty = dy.clone()
+    dirty[900:] = float("nan")
+    dx, dw, db = ops.group_norm_backward(dirty, x, mean, rstd, 8, w, b, offsets=off)
+    assert (dx[900:] == 0).all() and torch.isfinite(dw).all() and torch.isfinite(dx).all()
+    # no samples, no rows
+    none = torch.tensor([0], device="cuda")
+    assert (ops.group_norm(x, 8, w, b, offsets=none) == 0).all()
+    m0 = torch.empty(0, 8, device="cuda")
+    dx, dw, db = ops.group_norm_backward(dy, x, m0, m0, 8, w, b, offsets=none)
+    assert (dx == 0).all() and (dw == 0).all() and (db == 0).all()
+    e = torch.empty(0, 32, device="cuda")
+    y, mean, rstd = ops.group_norm(e, 8, w, b, offsets=torch.zeros(3, dtype=torch.int64, device="cuda"), want_stats=True)
+    assert y.shape == (0, 32) and (mean == 0).all() and mean.shape == (2, 8)
+    dx, dw, db = ops.group_norm_backward(e, e, mean, rstd, 8, w, b, offsets=torch.zeros(3, dtype=torch.int64, device="cuda"))
+    assert (dw == 0).all() and (db == 0).all()
+    e5 = ops.new_act(32, (0, 4, 4), "cuda")
+    y, mean, rstd = ops.group_norm(e5, 8, w, b, want_stats=True)
+    assert y.numel() == 0 and (rstd == 0).all()
+    # offsets that decrease or leave the buffer are empty / cut samples, never rows outside it
+    y = ops.group_norm(x, 8, w, b, offsets=torch.tensor([0, 500, 20, 5000], device="cuda"))
+    assert y.shape == (1000, 32)
+
+
+@pytest.mark.gpu
+def test_many_samples_and_one_row_each():
+    lens = [(i * 37) % 5 for i in range(5000)]
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    from sis3d import ops
+    x, dy, w, b = make(offsets[-1], 16, torch.float32)
+    y, mean, rstd = ops.group_norm(x, 4, w, b, offsets=torch.tensor(offsets, device="cuda"), want_stats=True)
+    pick = [i for i in range(0, 5000, 97)]
+    for s in pick:
+        lo, hi = offsets[s], offsets[s + 1]
+        want = reference(x[lo:hi].double(), dy[lo:hi].double(), [0, hi - lo], 4, w, b, "none")
+        check_close(y[lo:hi], want["y"], want["ty"] * 4 + half_of(torch.float32) * want["y"].abs(), "sample %d" % s)
+
+
+@pytest.mark.gpu
+def test_large_mean_constant_and_non_finite_inputs():
+    from sis3d import ops
+    g = torch.Generator(device="cuda").manual_seed(0)
+    # deviation 1 around a mean of 4096: the variance must not cancel (u * 4096 is the rounding of the mean itself)
+    x = 4096 + torch.randn(5000, 16, device="cuda", generator=g)
+    y, mean, rstd = ops.group_norm(x, 2, offsets=torch.tensor([0, 5000], device="cuda"), want_stats=True)
+    want = reference(x.double(), torch.zeros_like(x).double(), [0, 5000], 2, None, None, "none")
+    assert ((rstd.double() - want["rstd"]).abs() <= 64 * U * want["rstd"]).all()
+    check_close(y, want["y"], want["ty"], "y")
+    # a constant map has variance 0 exactly: y is the bias
+    b = torch.randn(16, device="cuda", generator=g)
+    c = torch.full((300, 16), 1.7, device="cuda")
+    assert torch.equal(ops.group_norm(c, 4, None, b, offsets=torch.tensor([0, 300], device="cuda")), b.expand(300, 16))
+    # a NaN or an infinity stays in its own sample and group
+    x = torch.randn(2, 4, 4, 4, 16, device="cuda", generator=g)
+    clean = ops.group_norm(x.permute(0, 4, 1, 2, 3), 4, act="relu")
+    for v in (float("nan"), float("inf")):
+        d = x.clone()
+        d[1, 2, 1, 3, 5] = v
+        y = ops.group_norm(d.permute(0, 4, 1, 2, 3), 4, act="relu")
+        assert torch.isnan(y[1, 4:8]).all()
+        y[1, 4:8] = clean[1, 4:8]
+        assert torch.equal(y, clean)
+
+
+@pytest.mark.gpu
+def test_streams_graph_and_determinism():
+    from sis3d import ops
+    x, dy, w, b = make(3456, 64, torch.float32)
+    off = torch.tensor([0, 1000, 3456], device="cuda")
+
+    def step():
+        y, mean, rstd = ops.group_norm(x, 8, w, b, act="silu", offsets=off, want_stats=True)
+        return (y,) + ops.group_norm_backward(dy, x, mean, rstd, 8, w, b, act="silu", offsets=off)
+    eager = [t.clone() for t in step()]
+    assert all(torch.equal(a, c) for a, c in zip(step(), eager))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(other, eager))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    keep = x.clone()
+    for k in range(4):
+        x.copy_(keep * (1 + k))
+        off.copy_(torch.tensor([0, 1000 + k, 3456 - 5 * k]))
+        graph.replay()
+        torch.cuda.synchronize()
+        again = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(held, again)), k
+
+
+@pytest.mark.gpu
+def test_more_than_two_to_the_31_elements():
+    from sis3d import ops
+    C, rows = 64, (1 << 31) // 64 + 1000
+    x = torch.empty(rows, C, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for i in range(0, rows, 1 << 22):
+        x[i:i + (1 << 22)].normal_(generator=g)
+    off = torch.tensor([0, rows - 700, rows], device="cuda")
+    y, mean, rstd = ops.group_norm(x, 8, offsets=off, want_stats=True)
+    tail = x[rows - 700:].clone()
+    want = reference(tail.double(), torch.zeros_like(tail).double(), [0, 700], 8, None, None, "none")
+    check_close(y[rows - 700:], want["y"], want["ty"] + half_of(torch.bfloat16) * want["y"].abs(), "tail")
+    # 2^31 standard normal values a sample: mean 0 and deviation 1 to a few parts in 10^4 (2^-14 is one deviation of the mean of 2^28)
+    assert float(mean[0].abs().max()) < 6 * 2.0 ** -14 and float((rstd[0] - 1).abs().max()) < 1e-3
+    first = x[:512].double().view(512, 8, 8)
+    z = (first - mean[0].double().view(8, 1)) * rstd[0].double().view(8, 1)
+    check_close(y[:512], z.view(512, 64), half_of(torch.bfloat16) * z.view(512, 64).abs() + 1e-6, "head")
+    dx, _, _ = ops.group_norm_backward(x, x, mean, rstd, 8, offsets=off)
+    want = reference(tail.double(), tail.double(), [0, 700], 8, None, None, "none")
+    check_close(dx[rows - 700:], want["dx"], want["tdx"] + half_of(torch.bfloat16) * want["dx"].abs(), "dx tail")
+
+
+@pytest.mark.gpu
+def test_autograd_module_and_differences():
+    """HipGroupNorm in a training step: autograd's gradients are the operator's, and they are the slope of the loss"""
+    from sis3d import ops
+    from sis3d.nets.backbones import HipGroupNorm
+    g = torch.Generator(device="cuda").manual_seed(5)
+    m = HipGroupNorm(4, 32, act="silu").cuda()
+    with torch.no_grad():
+        m.weight.normal_(1, 0.2, generator=g)
+        m.bias.normal_(0, 0.2, generator=g)
+    assert set(m.state_dict()) == {"weight", "bias"}
+    x = torch.randn(1, 5, 6, 7, 32, device="cuda", generator=g).permute(0, 4, 1, 2, 3).requires_grad_(True)
+    t = torch.randn(1, 32, 5, 6, 7, device="cuda", generator=g)              # planar: its gradient arrives planar
+    (m(x) * t).sum().backward()
+    y, mean, rstd = ops.group_norm(x.detach(), 4, m.weight.detach(), m.bias.detach(), m.eps, act="silu", want_stats=True)
+    dx, dw, db = ops.group_norm_backward(t.contiguous(memory_format=torch.channels_last_3d), x.detach(), mean, rstd, 4, m.weight.detach(),
+                                         m.bias.detach(), act="silu")
+    assert torch.equal(x.grad, dx) and torch.equal(m.weight.grad, dw) and torch.equal(m.bias.grad, db)
+    # central differences along random directions, step 2^-6: the rounding of y (u |y| a value, 6720 values, in quadrature) over the step is
+    # below 1e-3, the third derivative's share step^2 / 6 times one of order the gradient: both against |grad . v| of order 10..100
+    with torch.no_grad():
+        for leaf, grad in ((x, dx), (m.weight, dw), (m.bias, db)):
+            for k in range(3):
+                v = torch.randn(leaf.shape, device="cuda", generator=g)
+                keep, step = leaf.detach().clone(), 2.0 ** -6
+                f = []
+                for s in (step, -step):
+                    leaf.copy_(keep + s * v)
+                    f.append(float((m(x).double() * t.double()).sum()))
+                leaf.copy_(keep)
+                slope, want = (f[0] - f[1]) / (2 * step), float((grad.double() * v.double()).sum())
+                assert abs(slope - want) <= 1e-3 * float((grad.double() * v.double()).abs().sum()) + 2e-3, (slope, want)
+
+
+@pytest.mark.gpu
+def test_crops_of_the_mask_head():
+    """RaggedBatch.group_norm between the convolutions of packed crops: each crop as if it were alone"""
+    from sis3d import ops
+    windows = [(0, 0, 0, 9, 10, 11), (3, 2, 1, 4, 3, 2), (5, 5, 5, 17, 20, 14)]
+    rb = ops.RaggedBatch(windows, torch.device("cuda"))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    src = torch.randn(rb.voxels, 64, device="cuda", generator=g)
+    w, b = torch.rand(64, device="cuda", generator=g), torch.rand(64, device="cuda", generator=g)
+    got = rb.group_norm(src, 16, w, b, act="relu")
+    for crop, one in zip(rb.views(src), rb.views(got)):
+        alone = ops.group_norm(crop, 16, w, b, act="relu")
+        # the same formula with other tiles of rows: two results within the tolerance of the formula each
+        want = reference(rows_of(crop).double(), torch.zeros_like(rows_of(crop)).double(), [0, crop[0, 0].numel()], 16, w, b, "relu")
+        for t in (alone, one):
+            check_close(rows_of(t), want["y"], want["ty"] + half_of(torch.float32) * want["y"].abs(), "crop")
+
+
+@pytest.mark.gpu
+def test_refusals():
+    from sis3d import _lib, ops
+    x = torch.zeros(1, 4, 4, 4, 32, device="cuda").permute(0, 4, 1, 2, 3)
+    w = torch.ones(32, device="cuda")
+    bad = [lambda: ops.group_norm(x, 5), lambda: ops.group_norm(x, 0), lambda: ops.group_norm(x, 8, act="gelu"),
+           lambda: ops.group_norm(x.contiguous(), 8), lambda: ops.group_norm(x.double(), 8), lambda: ops.group_norm(x, 8, w[:16]),
+           lambda: ops.group_norm(x, 8, w.half()), lambda: ops.group_norm(x, 8, w.cpu()), lambda: ops.group_norm(x[:, 0, 0, 0, 0], 1),
+           lambda: ops.group_norm(x, 8, offsets=torch.tensor([0, 64], device="cuda")),
+           lambda: ops.group_norm(rows_of(x), 8, offsets=torch.tensor([0, 64], device="cuda", dtype=torch.int32)),
+           lambda: ops.group_norm(rows_of(x), 8, offsets=torch.tensor([0, 64])),
+           lambda: ops.group_norm(x, 8, out=torch.zeros(1, 32, 4, 4, 4, device="cuda")),
+           lambda: ops.group_norm(x, 8, out=torch.zeros_like(x).half()),
+           lambda: ops.group_norm(x.expand(2, -1, -1, -1, -1), 8, out=x.expand(2, -1, -1, -1, -1)),
+           lambda: ops.group_norm_backward(x.half(), x, torch.zeros(1, 8, device="cuda"), torch.zeros(1, 8, device="cuda"), 8),
+           lambda: ops.group_norm_backward(x, x, torch.zeros(1, 4, device="cuda"), torch.zeros(1, 8, device="cuda"), 8),
+           lambda: ops.group_norm(x.cpu(), 8), lambda: ops.group_norm(x, 8, eps=-1.0), lambda: ops.group_norm(x, 8, eps=float("nan"))]
+    for i, f in enumerate(bad):
+        with pytest.raises(_lib.Sis3dError):
+            f()
+            pytest.fail("refusal %d" % i)
+    with pytest.raises(ops.Sis3dUnsupported):
+        ops.group_norm(torch.zeros(1, 4099, 2, device="cuda").permute(0, 2, 1).contiguous().permute(0, 2, 1), 1)
+
+
+def test_abi_refuses_bad_arguments_without_a_gpu():
+    """every check of the C entry points comes before the first launch: codes, no device needed"""
+    from sis3d import _lib
+    l = _lib.lib()
+    p = ctypes.c_void_p(4096)                                                # never dereferenced
+    fwd = dict(x=p, dtype=0, S=1, rows=10, off=None, xn=0, xv=32, C=32, G=8, w=None, b=None, eps=1e-5, act=0, y=p, yn=0, yv=32, tail=0, mean=None,
+               rstd=None, ws=p, wsb=1 << 30, stream=None)
+
+    def forward(**k):
+        return l.sis3d_group_norm_forward(*dict(fwd, **k).values())
+    for k in (dict(dtype=3), dict(S=-1), dict(rows=-1), dict(C=0), dict(G=0), dict(G=5), dict(act=3), dict(act=-1), dict(x=None), dict(y=None),
+              dict(mean=p), dict(eps=-1.0), dict(eps=float("nan")), dict(ws=None), dict(ws=ctypes.c_void_p(4100))):
+        assert forward(**k) == -1, k
+    assert forward(wsb=0) == -3
+    assert forward(C=4099, G=1, xv=4099, yv=4099) == -4
+    assert forward(rows=0) == 0 and forward(S=0) == 0
+    bwd = dict(dy=p, dn=0, dv=32, x=p, dtype=0, S=1, rows=10, off=None, xn=0, xv=32, C=32, G=8, mean=p, rstd=p, w=None, b=None, act=0, dx=p, gn=0,
+               gv=32, dw=None, db=None, ws=p, wsb=1 << 30, stream=None)
+
+    def backward(**k):
+        return l.sis3d_group_norm_backward(*dict(bwd, **k).values())
+    for k in (dict(dtype=-1), dict(dy=None), dict(dx=None), dict(mean=None), dict(rstd=None), dict(G=3), dict(ws=None)):
+        assert backward(**k) == -1, k
+    assert backward(wsb=16) == -3 and backward(rows=0) == 0
+    assert l.sis3d_group_norm_workspace_bytes(0, 1, 10, 0, 32, 5, 0) == 0
+    assert l.sis3d_group_norm_workspace_bytes(0, 1, 10 ** 6, 0, 32, 8, 1) > 0
+
+
+def test_reference_gradients_are_slopes():
+    """the oracle of this file: its gradients are autograd's in 64 bits (CPU)"""
+    g = torch.Generator().manual_seed(0)
+    for act in ("none", "relu", "silu"):
+        x = torch.randn(23, 12, generator=g, dtype=torch.float64, requires_grad=True)
+        w, b = (torch.randn(12, generator=g, dtype=torch.float64, requires_grad=True) for _ in range(2))
+        dy = torch.randn(23, 12, generator=g, dtype=torch.float64)
+        parts = []
+        for lo, hi in ((0, 9), (9, 23)):
+            z = torch.nn.functional.group_norm(x[lo:hi].t()[None], 3, w, b, EPS)
+            parts.append({"none": z, "relu": z.relu(), "silu": z * z.sigmoid()}[act][0].t())
+        y = torch.cat(parts)
+        dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+        got = reference(x.detach(), dy, [0, 9, 23], 3, w.detach(), b.detach(), act)
+        for k, v in (("y", y.detach()), ("dx", dx), ("dw", dw), ("db", db)):
+            assert torch.allclose(got[k], v, rtol=1e-10, atol=1e-12), (act, k)
