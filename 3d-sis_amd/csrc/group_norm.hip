@@ -7,7 +7,8 @@
 //
 // Both directions are bound by memory: forward has to read x and write y, backward to read x and dy and write dx, and every group
 // needs all of its rows before the first result can be written.  Two launches each: the first reduces TILES of rows to partial sums
-// (a deterministic tree, no atomics), the second adds the partials of its own sample and applies.  A tile is processed by the same
+// (a deterministic tree, no atomics), the second adds the partials of its own sample and applies.  Samples of which a workgroup can
+// hold a column block's rows in cache take one launch for both.  A tile is processed by the same
 // workgroup number in both, i.e. on the same XCD, so that what fits its L2 is not fetched twice.
 //
 // Ragged batches: sample s owns rows [off[s], off[s + 1]) of one buffer, off on the device.  Tiles never cross samples: sample s uses the
@@ -20,7 +21,7 @@
 
 namespace {
 
-constexpr int NT = 512;
+constexpr int NT = 512, U = 4;    // threads of a workgroup; rows a thread has in flight
 
 struct GnArgs {
     const void *x, *dy;
@@ -30,7 +31,7 @@ struct GnArgs {
     const int64_t *off;           // S + 1 row offsets, or NULL: S samples of `rows` rows each
     int64_t rows;                 // per sample, or of the whole buffer (ragged)
     int64_t x_n, x_v, d_n, d_v, y_n, y_v;     // element strides between samples and rows of x, dy, y / dx
-    int S, C, G, cpg, gpb, T, tiles, act, zero_tail;
+    int S, C, G, cpg, gpb, T, t_log, tiles, zero_tail;     // T rows a tile; ragged: T = 1 << t_log
     float eps;
     double2 *part;                // forward: [workgroups][G] (sum, sum of squares)
     float2 *part_g, *part_c;      // backward: [workgroups][G] and [workgroups][C]
@@ -53,34 +54,41 @@ __device__ inline int64_t clamp_off(const GnArgs &a, int s)
     return o < 0 ? 0 : (o > a.rows ? a.rows : o);
 }
 
-// the tile of workgroup number `b`; uniform over the workgroup
+// the tile of workgroup number `b`; uniform over the workgroup, which calls it together
 __device__ inline Tile find_tile(const GnArgs &a, int b)
 {
     Tile r;
     int64_t begin;
     if (!a.off) {
-        const int tps = (int)((a.rows + a.T - 1) / a.T);
+        const int tps = a.tiles / a.S;
         r.s = b / tps;
         r.t = b - r.s * tps;
         r.first = r.s * tps;
         r.len = a.rows;
         begin = 0;
     } else {
-        // the last s with floor(off[s] / T) + s <= b
-        int lo = 0, hi = a.S + 1;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (clamp_off(a, mid) / a.T + mid <= b) lo = mid;
-            else hi = mid;
+        // the last s with floor(off[s] / T) + s <= b: one load a thread, or a search where there are more samples than threads
+        int lo;
+        if (a.S < NT) {
+            const int s = threadIdx.x;
+            lo = __syncthreads_count(s <= a.S && (clamp_off(a, s) >> a.t_log) + s <= b) - 1;
+        } else {
+            lo = 0;
+            int hi = a.S + 1;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if ((clamp_off(a, mid) >> a.t_log) + mid <= b) lo = mid;
+                else hi = mid;
+            }
         }
         r.s = lo;
         begin = clamp_off(a, lo);
         const int64_t end = lo < a.S ? clamp_off(a, lo + 1) : a.rows;
-        r.first = (int)(begin / a.T) + lo;
+        r.first = (int)(begin >> a.t_log) + lo;
         r.t = b - r.first;
         r.len = end > begin ? end - begin : 0;      // offsets that decrease give empty samples, never rows outside the buffer
     }
-    r.ntiles = (int)((r.len + a.T - 1) / a.T);
+    r.ntiles = a.off ? (int)((r.len + a.T - 1) >> a.t_log) : a.tiles / a.S;
     const int64_t left = r.len - (int64_t)r.t * a.T;
     r.n = r.t < 0 || left < 0 ? 0 : (left < a.T ? (int)left : a.T);
     r.row0 = begin + (int64_t)r.t * a.T;
@@ -109,47 +117,50 @@ template <int VEC> __device__ inline Cols columns(const GnArgs &a)
     return k;
 }
 
-// Adds, per group of the column block, pairs that the threads left in LDS: lds[row lane][channel of the block] -> out(group, pair).
-template <typename P, typename F> __device__ inline void reduce_groups(const P *lds, int rpb, int gl, int cpg, F out)
+// lanes (a power of two, at most a wave) that share the sums of one of `gl` groups
+__device__ inline int lanes_per_group(int gl)
 {
-    int lp = 1;
-    while (lp < 64 && lp * 2 * gl <= NT) lp *= 2;
-    const int per = rpb * cpg;
+    int lp = 64;
+    while (lp > 1 && lp * gl > NT) lp >>= 1;
+    return lp;
+}
+template <typename F> __device__ inline void finish_group(double s0, double s1, int lp, int l, int g, F out)
+{
+    for (int o = lp >> 1; o > 0; o >>= 1) {
+        s0 += __shfl_xor(s0, o);
+        s1 += __shfl_xor(s1, o);
+    }
+    if (l == 0) out(g, s0, s1);
+}
+
+// Adds, per group of the column block, pairs that the threads left in LDS: `epg` entries a group and row lane
+template <typename P, typename F> __device__ inline void reduce_groups(const P *lds, int rpb, int gl, int epg, F out)
+{
+    const int lp = lanes_per_group(gl), per = rpb * epg, l = threadIdx.x & (lp - 1);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
-        const int l = threadIdx.x % lp;
         double s0 = 0, s1 = 0;
         for (int i = l; i < per; i += lp) {
-            const int r = i / cpg;
-            const P v = lds[(size_t)r * gl * cpg + g * cpg + (i - r * cpg)];
+            const int r = i / epg;
+            const P v = lds[(r * gl + g) * epg + (i - r * epg)];
             s0 += v.x;
             s1 += v.y;
         }
-        for (int o = lp >> 1; o > 0; o >>= 1) {
-            s0 += __shfl_xor(s0, o);
-            s1 += __shfl_xor(s1, o);
-        }
-        if (l == 0) out(g, s0, s1);
+        finish_group(s0, s1, lp, l, g, out);
     }
 }
 
 // The same over the tiles of one sample: part[(first + p) * G + g]
 template <typename P, typename F> __device__ inline void reduce_tiles(const P *part, int first, int ntiles, int G, int g0, int gl, F out)
 {
-    int lp = 1;
-    while (lp < 64 && lp * 2 * gl <= NT) lp *= 2;
+    const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
-        const int l = threadIdx.x % lp;
         double s0 = 0, s1 = 0;
         for (int p = l; p < ntiles; p += lp) {
             const P v = part[(size_t)(first + p) * G + g0 + g];
             s0 += v.x;
             s1 += v.y;
         }
-        for (int o = lp >> 1; o > 0; o >>= 1) {
-            s0 += __shfl_xor(s0, o);
-            s1 += __shfl_xor(s1, o);
-        }
-        if (l == 0) out(g, s0, s1);
+        finish_group(s0, s1, lp, l, g, out);
     }
 }
 
@@ -170,71 +181,91 @@ template <int ACT> __device__ inline float act_slope(float z)
     } else return 1.f;
 }
 
-template <typename T, int VEC> __global__ __launch_bounds__(NT) void gn_stats(GnArgs a)
+// f(row) for this thread's rows of a tile, U of them at a time: loads first, so that U are in flight
+template <typename T, int VEC, typename F> __device__ inline void each_row(const T *x, int64_t stride, int ri, int rpb, int n, F f)
 {
-    extern __shared__ double2 lds[];
-    const Tile t = find_tile(a, blockIdx.x);
-    if (t.s < 0 || t.s >= a.S || t.n == 0) return;
-    const Cols k = columns<VEC>(a);
-    const T *x = (const T *)a.x + (a.off ? 0 : t.s * a.x_n) + t.row0 * a.x_v + k.c;
+    for (int r = ri; r < n; r += U * rpb) {
+        SisVec<T, VEC> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *(const SisVec<T, VEC> *)(x + min(r + u * rpb, n - 1) * stride);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u * rpb < n) f(r + u * rpb, v[u]);
+    }
+}
+template <typename T, int VEC, typename F>
+__device__ inline void each_row2(const T *x, int64_t xs, const T *d, int64_t ds, int ri, int rpb, int n, F f)
+{
+    for (int r = ri; r < n; r += U * rpb) {
+        SisVec<T, VEC> v[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = min(r + u * rpb, n - 1);
+            v[u] = *(const SisVec<T, VEC> *)(x + at * xs);
+            w[u] = *(const SisVec<T, VEC> *)(d + at * ds);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u * rpb < n) f(r + u * rpb, v[u], w[u]);
+    }
+}
+
+// Sums of one tile's rows, left per group in out(group, sum, sum of squares)
+template <typename T, int VEC, typename F> __device__ inline void tile_sums(const GnArgs &a, const Cols &k, const T *x, int n, double2 *lds, F out)
+{
+    const bool fold = a.cpg % VEC == 0;              // a vector's channels are of one group: one entry a thread
     if (k.live) {
-        float K[VEC], s1[VEC], s2[VEC], v[VEC];
-        int n = 0;
+        float K[VEC], s1[VEC], s2[VEC];
+        int m = 0;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) K[i] = s1[i] = s2[i] = 0.f;
-        if (k.ri < t.n) sis3d_load<T, VEC>(x + k.ri * a.x_v, K);
-        for (int r = k.ri; r < t.n; r += k.rpb, ++n) {
-            sis3d_load<T, VEC>(x + r * a.x_v, v);
+        if (k.ri < n) sis3d_load<T, VEC>(x + k.ri * a.x_v, K);
+        each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int, const SisVec<T, VEC> &v) {
+            ++m;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float d = v[i] - K[i];
+                const float d = sis3d_f32(v.v[i]) - K[i];
                 s1[i] += d;
                 s2[i] = fmaf(d, d, s2[i]);
             }
-        }
+        });
+        double f0 = 0, f1 = 0;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const double kk = K[i];
-            lds[(size_t)k.ri * k.nv * VEC + k.cv * VEC + i] = make_double2(n * kk + s1[i], s2[i] + kk * (2.0 * s1[i] + n * kk));
+            const double kk = K[i], t0 = m * kk + s1[i], t1 = s2[i] + kk * (2.0 * s1[i] + m * kk);
+            f0 += t0;
+            f1 += t1;
+            if (!fold) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2(t0, t1);
         }
+        if (fold) lds[k.ri * k.nv + k.cv] = make_double2(f0, f1);
     }
     __syncthreads();
-    reduce_groups(lds, k.rpb, k.gl, a.cpg, [&](int g, double s0, double s1) { a.part[(size_t)blockIdx.x * a.G + k.g0 + g] = make_double2(s0, s1); });
+    reduce_groups(lds, k.rpb, k.gl, fold ? a.cpg / VEC : a.cpg, out);
 }
 
-template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_apply(GnArgs a)
+// mean and r of a group from its sums
+__device__ inline void group_stats(const GnArgs &a, const Cols &k, const Tile &t, float *st, int g, double s0, double s1)
 {
-    extern __shared__ float st[];                    // [gl] mean, [gl] r
-    const Tile t = find_tile(a, blockIdx.x);
-    if (t.s < 0) return;
-    const Cols k = columns<VEC>(a);
-    T *y = (T *)a.y + (a.off ? 0 : t.s * a.y_n) + t.row0 * a.y_v + k.c;
-    if (t.s >= a.S) {                                // rows behind the last sample
-        if (a.zero_tail && k.live) {
-            const float z[VEC] = {};
-            for (int r = k.ri; r < t.n; r += k.rpb) sis3d_store<T, VEC>(y + r * a.y_v, z);
-        }
-        return;
-    }
     const double m = (double)t.len * a.cpg;
-    reduce_tiles(a.part, t.first, t.ntiles, a.G, k.g0, k.gl, [&](int g, double s0, double s1) {
-        double mu = 0, r = 0;
-        if (m > 0) {
-            mu = s0 / m;
-            const double var = s1 / m - mu * mu;
-            r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps);      // NaN passes
-        }
-        st[g] = (float)mu;
-        st[k.gl + g] = (float)r;
-        if (t.t == 0 && a.mean) {
-            a.mean[(size_t)t.s * a.G + k.g0 + g] = (float)mu;
-            a.rstd[(size_t)t.s * a.G + k.g0 + g] = (float)r;
-        }
-    });
-    __syncthreads();
+    double mu = 0, r = 0;
+    if (m > 0) {
+        mu = s0 / m;
+        const double var = s1 / m - mu * mu;
+        r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps);      // NaN passes
+    }
+    st[g] = (float)mu;
+    st[k.gl + g] = (float)r;
+    if (t.t == 0 && a.mean) {
+        a.mean[(size_t)t.s * a.G + k.g0 + g] = (float)mu;
+        a.rstd[(size_t)t.s * a.G + k.g0 + g] = (float)r;
+    }
+}
+
+template <typename T, int VEC, int ACT>
+__device__ inline void apply_rows(const GnArgs &a, const Cols &k, const float *st, const T *x, T *y, int n)
+{
     if (!k.live) return;
-    const T *x = (const T *)a.x + (a.off ? 0 : t.s * a.x_n) + t.row0 * a.x_v + k.c;
-    float mu[VEC], sc[VEC], sh[VEC], v[VEC];
+    float mu[VEC], sc[VEC], sh[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const int g = (k.cv * VEC + i) / a.cpg;
@@ -242,73 +273,177 @@ template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn
         sc[i] = st[k.gl + g] * (a.w ? a.w[k.c + i] : 1.f);
         sh[i] = a.b ? a.b[k.c + i] : 0.f;
     }
-    for (int r = k.ri; r < t.n; r += k.rpb) {
-        sis3d_load<T, VEC>(x + r * a.x_v, v);
+    each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int r, const SisVec<T, VEC> &v) {
+        float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = act<ACT>(fmaf(v[i] - mu[i], sc[i], sh[i]));
-        sis3d_store<T, VEC>(y + r * a.y_v, v);
+        for (int i = 0; i < VEC; ++i) o[i] = act<ACT>(fmaf(sis3d_f32(v.v[i]) - mu[i], sc[i], sh[i]));
+        sis3d_store<T, VEC>(y + r * a.y_v, o);
+    });
+}
+
+// rows behind the last sample
+template <typename T, int VEC> __device__ inline void zero_rows(const GnArgs &a, const Cols &k, T *y, int n)
+{
+    if (!a.zero_tail || !k.live) return;
+    const float z[VEC] = {};
+    for (int r = k.ri; r < n; r += k.rpb) sis3d_store<T, VEC>(y + r * a.y_v, z);
+}
+
+template <typename T> __device__ inline const T *rows_at(const void *p, const GnArgs &a, const Cols &k, const Tile &t, int64_t sn, int64_t sv)
+{
+    return (const T *)p + (a.off ? 0 : t.s * sn) + t.row0 * sv + k.c;
+}
+
+template <typename T, int VEC> __global__ __launch_bounds__(NT) void gn_stats(GnArgs a)
+{
+    extern __shared__ double2 lds[];
+    const Tile t = find_tile(a, blockIdx.x);
+    if (t.s < 0 || t.s >= a.S || t.n == 0) return;
+    const Cols k = columns<VEC>(a);
+    tile_sums<T, VEC>(a, k, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), t.n, lds,
+                      [&](int g, double s0, double s1) { a.part[(size_t)blockIdx.x * a.G + k.g0 + g] = make_double2(s0, s1); });
+}
+
+template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_apply(GnArgs a)
+{
+    extern __shared__ double2 ldsd[];
+    float *st = (float *)ldsd;                       // [gl] mean, [gl] r
+    const Tile t = find_tile(a, blockIdx.x);
+    if (t.s < 0) return;
+    const Cols k = columns<VEC>(a);
+    T *y = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
+    if (t.s >= a.S) { zero_rows<T, VEC>(a, k, y, t.n); return; }
+    reduce_tiles(a.part, t.first, t.ntiles, a.G, k.g0, k.gl, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
+    __syncthreads();
+    apply_rows<T, VEC, ACT>(a, k, st, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), y, t.n);
+}
+
+// both in one launch where a sample is one tile (T >= every sample): the second reading of the rows comes from cache
+template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_one(GnArgs a)
+{
+    extern __shared__ double2 lds[];
+    __shared__ float st[2 * NT];
+    const Tile t = find_tile(a, blockIdx.x);
+    if (t.s < 0) return;
+    const Cols k = columns<VEC>(a);
+    T *y = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
+    if (t.s >= a.S) { zero_rows<T, VEC>(a, k, y, t.n); return; }
+    const T *x = rows_at<T>(a.x, a, k, t, a.x_n, a.x_v);
+    tile_sums<T, VEC>(a, k, x, t.n, lds, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
+    __syncthreads();
+    apply_rows<T, VEC, ACT>(a, k, st, x, y, t.n);
+}
+
+// what a thread needs of its channels in the backward direction
+template <int VEC> struct Chan {
+    float mu[VEC], rs[VEC], w[VEC], b[VEC];
+    __device__ Chan(const GnArgs &a, const Cols &k, int s)
+    {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const size_t g = (size_t)s * a.G + (k.c + i) / a.cpg;
+            mu[i] = a.mean[g];
+            rs[i] = a.rstd[g];
+            w[i] = a.w ? a.w[k.c + i] : 1.f;
+            b[i] = a.b ? a.b[k.c + i] : 0.f;
+        }
     }
+};
+
+// Channel sums (d, d h) of a tile: to chan(channel, s0, s1), and their weighted sums per group to group(group, S1, S2)
+template <typename T, int VEC, int ACT, typename FC, typename FG>
+__device__ inline void tile_grad_sums(const GnArgs &a, const Cols &k, const Tile &t, const T *x, const T *dy, float2 *lds, FC chan, FG group)
+{
+    const int cl = k.gl * a.cpg;
+    if (k.live) {
+        const Chan<VEC> c(a, k, t.s);
+        float s0[VEC], s1[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s0[i] = s1[i] = 0.f;
+        each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float h = (sis3d_f32(v.v[i]) - c.mu[i]) * c.rs[i];
+                const float e = sis3d_f32(d.v[i]) * act_slope<ACT>(fmaf(h, c.w[i], c.b[i]));
+                s0[i] += e;
+                s1[i] = fmaf(e, h, s1[i]);
+            }
+        });
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) lds[k.ri * cl + k.cv * VEC + i] = make_float2(s0[i], s1[i]);
+    }
+    __syncthreads();
+    // over the row lanes: q threads a channel, thread (channel, part) adds the rows part, part + q, ... into row `part`, which it alone reads
+    const int q = cl < NT ? min(NT / cl, k.rpb) : 1;
+    for (int i = threadIdx.x; i < q * cl; i += NT) {
+        double s0 = 0, s1 = 0;
+        for (int j = i; j < k.rpb * cl; j += q * cl) {
+            const float2 v = lds[j];
+            s0 += v.x;
+            s1 += v.y;
+        }
+        lds[i] = make_float2((float)s0, (float)s1);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < cl; c += NT) {
+        double s0 = 0, s1 = 0;
+        for (int j = c; j < q * cl; j += cl) {
+            const float2 v = lds[j];
+            s0 += v.x;
+            s1 += v.y;
+        }
+        const int cg = k.g0 * a.cpg + c;
+        chan(cg, s0, s1);
+        const float w = a.w ? a.w[cg] : 1.f;
+        lds[c] = make_float2((float)(w * s0), (float)(w * s1));
+    }
+    __syncthreads();
+    reduce_groups(lds, 1, k.gl, a.cpg, group);
+}
+
+template <typename T, int VEC, int ACT>
+__device__ inline void apply_grad(const GnArgs &a, const Cols &k, const Tile &t, const float *st, const T *x, const T *dy, T *dx)
+{
+    if (!k.live) return;
+    const Chan<VEC> c(a, k, t.s);
+    float m1[VEC], m2[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        const int g = (k.cv * VEC + i) / a.cpg;
+        m1[i] = st[g];
+        m2[i] = st[k.gl + g];
+    }
+    each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int r, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float h = (sis3d_f32(v.v[i]) - c.mu[i]) * c.rs[i];
+            const float e = sis3d_f32(d.v[i]) * act_slope<ACT>(fmaf(h, c.w[i], c.b[i])) * c.w[i];
+            o[i] = c.rs[i] * (e - fmaf(h, m2[i], m1[i]));
+        }
+        sis3d_store<T, VEC>(dx + r * a.y_v, o);
+    });
 }
 
 template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_back_sums(GnArgs a)
 {
     extern __shared__ double2 ldsd[];
-    float2 *lds = (float2 *)ldsd;
     const Tile t = find_tile(a, blockIdx.x);
     const Cols k = columns<VEC>(a);
-    const int cl = k.gl * a.cpg;
     if (t.s < 0 || t.s >= a.S || t.n == 0) {         // no rows: its channel sums are read all the same
-        for (int c = threadIdx.x; c < cl; c += NT) a.part_c[(size_t)blockIdx.x * a.C + k.g0 * a.cpg + c] = make_float2(0.f, 0.f);
+        for (int c = threadIdx.x; c < k.gl * a.cpg; c += NT) a.part_c[(size_t)blockIdx.x * a.C + k.g0 * a.cpg + c] = make_float2(0.f, 0.f);
         return;
     }
-    if (k.live) {
-        const T *x = (const T *)a.x + (a.off ? 0 : t.s * a.x_n) + t.row0 * a.x_v + k.c;
-        const T *dy = (const T *)a.dy + (a.off ? 0 : t.s * a.d_n) + t.row0 * a.d_v + k.c;
-        float mu[VEC], rs[VEC], w[VEC], b[VEC], v[VEC], d[VEC], s0[VEC], s1[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const size_t g = (size_t)t.s * a.G + (k.c + i) / a.cpg;
-            mu[i] = a.mean[g];
-            rs[i] = a.rstd[g];
-            w[i] = a.w ? a.w[k.c + i] : 1.f;
-            b[i] = a.b ? a.b[k.c + i] : 0.f;
-            s0[i] = s1[i] = 0.f;
-        }
-        for (int r = k.ri; r < t.n; r += k.rpb) {
-            sis3d_load<T, VEC>(x + r * a.x_v, v);
-            sis3d_load<T, VEC>(dy + r * a.d_v, d);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float h = (v[i] - mu[i]) * rs[i];
-                const float e = d[i] * act_slope<ACT>(fmaf(h, w[i], b[i]));
-                s0[i] += e;
-                s1[i] = fmaf(e, h, s1[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) lds[(size_t)k.ri * cl + k.cv * VEC + i] = make_float2(s0[i], s1[i]);
-    }
-    __syncthreads();
-    // per channel over the row lanes, then per group with the weights
-    for (int c = threadIdx.x; c < cl; c += NT) {
-        double s0 = 0, s1 = 0;
-        for (int r = 0; r < k.rpb; ++r) {
-            const float2 v = lds[(size_t)r * cl + c];
-            s0 += v.x;
-            s1 += v.y;
-        }
-        const int cg = k.g0 * a.cpg + c;
-        a.part_c[(size_t)blockIdx.x * a.C + cg] = make_float2((float)s0, (float)s1);
-        const float w = a.w ? a.w[cg] : 1.f;
-        lds[c] = make_float2((float)(w * s0), (float)(w * s1));      // row lane 0's place of the same channel: read by this thread alone before
-    }
-    __syncthreads();
-    reduce_groups(lds, 1, k.gl, a.cpg, [&](int g, double s0, double s1) { a.part_g[(size_t)blockIdx.x * a.G + k.g0 + g] = make_float2((float)s0, (float)s1); });
+    tile_grad_sums<T, VEC, ACT>(
+        a, k, t, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), rows_at<T>(a.dy, a, k, t, a.d_n, a.d_v), (float2 *)ldsd,
+        [&](int c, double s0, double s1) { a.part_c[(size_t)blockIdx.x * a.C + c] = make_float2((float)s0, (float)s1); },
+        [&](int g, double s0, double s1) { a.part_g[(size_t)blockIdx.x * a.G + k.g0 + g] = make_float2((float)s0, (float)s1); });
 }
 
 template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_back_apply(GnArgs a)
 {
-    extern __shared__ float st[];                    // [gl] S1 / m, [gl] S2 / m
+    extern __shared__ double2 ldsd[];
+    float *st = (float *)ldsd;                       // [gl] S1 / m, [gl] S2 / m
     if ((int)blockIdx.x >= a.tiles) {                // the last workgroups add the channel sums of all tiles: dw, db
         if (blockIdx.y) return;
         __shared__ double acc[NT][2];
@@ -336,78 +471,80 @@ template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn
     const Tile t = find_tile(a, blockIdx.x);
     if (t.s < 0 || t.n == 0) return;
     const Cols k = columns<VEC>(a);
-    T *dx = (T *)a.y + (a.off ? 0 : t.s * a.y_n) + t.row0 * a.y_v + k.c;
-    if (t.s >= a.S) {
-        if (a.zero_tail && k.live) {
-            const float z[VEC] = {};
-            for (int r = k.ri; r < t.n; r += k.rpb) sis3d_store<T, VEC>(dx + r * a.y_v, z);
-        }
-        return;
-    }
+    T *dx = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
+    if (t.s >= a.S) { zero_rows<T, VEC>(a, k, dx, t.n); return; }
     const double m = (double)t.len * a.cpg;
     reduce_tiles(a.part_g, t.first, t.ntiles, a.G, k.g0, k.gl, [&](int g, double s0, double s1) {
         st[g] = (float)(s0 / m);
         st[k.gl + g] = (float)(s1 / m);
     });
     __syncthreads();
-    if (!k.live) return;
-    const T *x = (const T *)a.x + (a.off ? 0 : t.s * a.x_n) + t.row0 * a.x_v + k.c;
-    const T *dy = (const T *)a.dy + (a.off ? 0 : t.s * a.d_n) + t.row0 * a.d_v + k.c;
-    float mu[VEC], rs[VEC], w[VEC], b[VEC], m1[VEC], m2[VEC], v[VEC], d[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        const int gl = (k.cv * VEC + i) / a.cpg;
-        const size_t g = (size_t)t.s * a.G + k.g0 + gl;
-        mu[i] = a.mean[g];
-        rs[i] = a.rstd[g];
-        w[i] = a.w ? a.w[k.c + i] : 1.f;
-        b[i] = a.b ? a.b[k.c + i] : 0.f;
-        m1[i] = st[gl];
-        m2[i] = st[k.gl + gl];
-    }
-    for (int r = k.ri; r < t.n; r += k.rpb) {
-        sis3d_load<T, VEC>(x + r * a.x_v, v);
-        sis3d_load<T, VEC>(dy + r * a.d_v, d);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float h = (v[i] - mu[i]) * rs[i];
-            const float e = d[i] * act_slope<ACT>(fmaf(h, w[i], b[i])) * w[i];
-            v[i] = rs[i] * (e - fmaf(h, m2[i], m1[i]));
-        }
-        sis3d_store<T, VEC>(dx + r * a.y_v, v);
-    }
+    apply_grad<T, VEC, ACT>(a, k, t, st, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), rows_at<T>(a.dy, a, k, t, a.d_n, a.d_v), dx);
+}
+
+// both in one launch for one dense sample that is one tile: dw and db are its own channel sums
+template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_back_one(GnArgs a)
+{
+    extern __shared__ double2 ldsd[];
+    __shared__ float st[2 * NT];
+    const Tile t = find_tile(a, blockIdx.x);
+    const Cols k = columns<VEC>(a);
+    const double m = (double)t.len * a.cpg;
+    const T *x = rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), *dy = rows_at<T>(a.dy, a, k, t, a.d_n, a.d_v);
+    tile_grad_sums<T, VEC, ACT>(
+        a, k, t, x, dy, (float2 *)ldsd,
+        [&](int c, double s0, double s1) {
+            if (a.db) a.db[c] = (float)s0;
+            if (a.dw) a.dw[c] = (float)s1;
+        },
+        [&](int g, double s0, double s1) {
+            st[g] = (float)(s0 / m);
+            st[k.gl + g] = (float)(s1 / m);
+        });
+    __syncthreads();
+    apply_grad<T, VEC, ACT>(a, k, t, st, x, dy, (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v));
 }
 
 struct Plan {
-    int vec, gpb, ncol, T;
+    int vec, gpb, ncol, T, t_log, one, rc;
     int64_t tiles;
-    int rc;
 };
 
 int gcd_(int a, int b) { return b ? gcd_(b, a % b) : a; }
 
 // Tiles of rows and column blocks of whole groups.  `wide`: 16-byte accesses are possible (alignment of every pointer and stride).
-Plan make_plan(int dtype, int S, int64_t rows, int ragged, int C, int G, bool wide)
+Plan make_plan(int dtype, int S, int64_t rows, int ragged, int C, int G, bool wide, bool backward)
 {
     Plan p{};
     const int es = sis3d_elem_bytes(dtype), cpg = C / G;
     p.vec = wide && C % (16 / es) == 0 ? 16 / es : 1;
     const int gu = p.vec / gcd_(cpg, p.vec);               // groups whose channels are whole vectors
-    int most = (int)((int64_t)NT * p.vec / cpg) / gu * gu;
-    if (most > G) most = G;
-    if (most < gu || most < 1) { p.rc = SIS3D_EUNSUPPORTED; return p; }
-    if (most > 32) most = 32 / gu * gu > 0 ? 32 / gu * gu : gu;    // bounds what a workgroup of the second launch has to add up
-    p.gpb = most;
+    const int most = (int)((int64_t)NT * p.vec / cpg) / gu * gu;
+    if (most < 1) { p.rc = SIS3D_EUNSUPPORTED; return p; }
+    // a column block is one 128-byte line of a row, or one group if that is wider: the narrower it is, the fewer groups a workgroup of
+    // the second launch has to add the tiles' sums of
+    p.gpb = gu;
+    while (p.gpb < G && p.gpb * cpg * es < 128 && p.gpb + gu <= most) p.gpb += gu;
+    if (p.gpb > G) p.gpb = G;
     p.ncol = (G + p.gpb - 1) / p.gpb;
-    const int64_t total = ragged ? rows : rows * S;
-    int64_t T = (total * p.ncol + 511) / 512;              // about two workgroups per CU
-    const int rpb = NT * p.vec / (p.gpb * cpg);
-    if (T < rpb) T = rpb;
-    if (T < 1) T = 1;
+    const int64_t total = ragged ? rows : rows * S, seg = (int64_t)p.gpb * cpg * es;
+    int64_t T;
+    // one workgroup takes a whole sample where that is little: up to 128 KB of a column block it is sooner done than a second launch
+    p.one = rows * seg <= 128 * 1024 && !(backward && (S != 1 || ragged));
+    if (p.one) T = rows;
+    else {
+        T = (total * p.ncol + 511) / 512;                  // about two workgroups per CU
+        const int rpb = (int)(NT / (p.gpb * cpg / p.vec));
+        if (T < rpb) T = rpb;
+    }
+    if (T < 1) T = 1;                                      // no rows
     if (T > (1 << 24)) T = 1 << 24;
+    p.t_log = 0;
+    while (((int64_t)1 << p.t_log) < T) ++p.t_log;
+    if (ragged) T = (int64_t)1 << p.t_log;                 // a shift in place of divisions by T
     p.T = (int)T;
-    p.tiles = ragged ? rows / T + S + 1 : S * ((rows + T - 1) / T);
-    if (p.tiles > 0x7fffff00) p.rc = SIS3D_EUNSUPPORTED;
+    p.tiles = ragged ? (rows >> p.t_log) + S + 1 : S * ((rows + T - 1) / T);
+    if (p.tiles > 0x7fffff00 || p.ncol > 65535) p.rc = SIS3D_EUNSUPPORTED;
     return p;
 }
 
@@ -416,41 +553,44 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 size_t ws_bytes_of(const Plan &p, int C, int G, bool backward)
 {
     const size_t t = (size_t)p.tiles;
-    return backward ? t * ((size_t)C + G) * sizeof(float2) : t * G * sizeof(double2);
+    return p.one ? 0 : backward ? t * ((size_t)C + G) * sizeof(float2) : t * G * sizeof(double2);
 }
 
 #define GN_ACT(T, VEC, KERN)                                                                                       \
-    switch (a.act) {                                                                                               \
+    switch (act) {                                                                                                 \
     case ACT_RELU: hipLaunchKernelGGL((KERN<T, VEC, ACT_RELU>), grid, dim3(NT), lds, st, a); break;                \
     case ACT_SILU: hipLaunchKernelGGL((KERN<T, VEC, ACT_SILU>), grid, dim3(NT), lds, st, a); break;                \
     default: hipLaunchKernelGGL((KERN<T, VEC, ACT_NONE>), grid, dim3(NT), lds, st, a); break;                      \
     }
 
-template <typename T, int VEC> int launch(const GnArgs &a, const Plan &p, bool backward, hipStream_t st)
+template <typename T, int VEC> int launch(const GnArgs &a, const Plan &p, int act, bool backward, hipStream_t st)
 {
-    const int cl = p.gpb * a.cpg;
-    const int rpb = NT / (cl / VEC);
-    {
-        const dim3 grid((unsigned)p.tiles, p.ncol);
-        const size_t lds = (size_t)rpb * cl * (backward ? sizeof(float2) : sizeof(double2));
-        if (backward) { GN_ACT(T, VEC, gn_back_sums) }
-        else hipLaunchKernelGGL((gn_stats<T, VEC>), grid, dim3(NT), lds, st, a);
-        const int rc = sis3d_check_launch();
-        if (rc) return rc;
+    const int cl = p.gpb * a.cpg, rpb = NT / (cl / VEC);
+    dim3 grid((unsigned)p.tiles, p.ncol);
+    // forward: a pair of doubles a thread, or a channel where groups are not whole vectors; backward: a pair of floats a channel
+    size_t lds = backward ? (size_t)rpb * cl * sizeof(float2) : (size_t)rpb * (a.cpg % VEC ? cl : cl / VEC) * sizeof(double2);
+    if (p.one) {
+        if (backward) { GN_ACT(T, VEC, gn_back_one) }
+        else { GN_ACT(T, VEC, gn_one) }
+        return sis3d_check_launch();
     }
-    const dim3 grid((unsigned)p.tiles + (backward ? (a.C + 31) / 32 : 0), p.ncol);
-    const size_t lds = 2 * p.gpb * sizeof(float);
+    if (backward) { GN_ACT(T, VEC, gn_back_sums) }
+    else hipLaunchKernelGGL((gn_stats<T, VEC>), grid, dim3(NT), lds, st, a);
+    const int rc = sis3d_check_launch();
+    if (rc) return rc;
+    if (backward) grid.x += (a.C + 31) / 32;
+    lds = 2 * p.gpb * sizeof(float);
     if (backward) { GN_ACT(T, VEC, gn_back_apply) }
     else { GN_ACT(T, VEC, gn_apply) }
     return sis3d_check_launch();
 }
 
-int dispatch(const GnArgs &a, const Plan &p, int dtype, bool backward, hipStream_t st)
+int dispatch(const GnArgs &a, const Plan &p, int dtype, int act, bool backward, hipStream_t st)
 {
     switch (dtype) {
-    case SIS3D_F32: return p.vec > 1 ? launch<float, 4>(a, p, backward, st) : launch<float, 1>(a, p, backward, st);
-    case SIS3D_BF16: return p.vec > 1 ? launch<__bf16, 8>(a, p, backward, st) : launch<__bf16, 1>(a, p, backward, st);
-    default: return p.vec > 1 ? launch<_Float16, 8>(a, p, backward, st) : launch<_Float16, 1>(a, p, backward, st);
+    case SIS3D_F32: return p.vec > 1 ? launch<float, 4>(a, p, act, backward, st) : launch<float, 1>(a, p, act, backward, st);
+    case SIS3D_BF16: return p.vec > 1 ? launch<__bf16, 8>(a, p, act, backward, st) : launch<__bf16, 1>(a, p, act, backward, st);
+    default: return p.vec > 1 ? launch<_Float16, 8>(a, p, act, backward, st) : launch<_Float16, 1>(a, p, act, backward, st);
     }
 }
 
@@ -467,7 +607,7 @@ extern "C" size_t sis3d_group_norm_workspace_bytes(int dtype, int S, int64_t row
     if (check_args(dtype, S, rows, C, G, 0)) return 0;
     size_t most = 0;
     for (int wide = 0; wide < 2; ++wide) {                 // whichever access width the pointers will allow
-        const Plan p = make_plan(dtype, S, rows, ragged, C, G, wide);
+        const Plan p = make_plan(dtype, S, rows, ragged, C, G, wide, backward);
         const size_t b = p.rc ? 0 : ws_bytes_of(p, C, G, backward);
         if (b > most) most = b;
     }
@@ -491,16 +631,16 @@ extern "C" int sis3d_group_norm_forward(const void *x, int dtype, int S, int64_t
     if (!x || !y) return SIS3D_EINVAL;
     const int es = sis3d_elem_bytes(dtype);
     const int64_t strides = (offsets ? 0 : (x_sample | y_sample)) | x_row | y_row;
-    const Plan p = make_plan(dtype, S, rows, offsets != nullptr, C, G, aligned16(x) && aligned16(y) && strides * es % 16 == 0);
+    const Plan p = make_plan(dtype, S, rows, offsets != nullptr, C, G, aligned16(x) && aligned16(y) && strides * es % 16 == 0, false);
     if (p.rc) return p.rc;
     if (workspace_bytes < ws_bytes_of(p, C, G, false)) return SIS3D_EWORKSPACE;
-    if (!workspace || !aligned16(workspace)) return SIS3D_EINVAL;
+    if (!p.one && (!workspace || !aligned16(workspace))) return SIS3D_EINVAL;
     GnArgs a{};
     a.x = x; a.y = y; a.w = weight; a.b = bias; a.mean = mean; a.rstd = rstd; a.off = offsets; a.rows = rows;
     a.x_n = x_sample; a.x_v = x_row; a.y_n = y_sample; a.y_v = y_row;
-    a.S = S; a.C = C; a.G = G; a.cpg = C / G; a.gpb = p.gpb; a.T = p.T; a.tiles = (int)p.tiles; a.act = act; a.zero_tail = zero_tail; a.eps = eps;
+    a.S = S; a.C = C; a.G = G; a.cpg = C / G; a.gpb = p.gpb; a.T = p.T; a.t_log = p.t_log; a.tiles = (int)p.tiles; a.zero_tail = zero_tail; a.eps = eps;
     a.part = (double2 *)workspace;
-    return dispatch(a, p, dtype, false, st);
+    return dispatch(a, p, dtype, act, false, st);
 }
 
 extern "C" int sis3d_group_norm_backward(const void *dy, int64_t dy_sample, int64_t dy_row, const void *x, int dtype, int S, int64_t rows,
@@ -520,16 +660,16 @@ extern "C" int sis3d_group_norm_backward(const void *dy, int64_t dy_sample, int6
     if (!x || !dy || !dx || ((!mean || !rstd) && S)) return SIS3D_EINVAL;
     const int es = sis3d_elem_bytes(dtype);
     const int64_t strides = (offsets ? 0 : (x_sample | dy_sample | dx_sample)) | x_row | dy_row | dx_row;
-    const Plan p = make_plan(dtype, S, rows, offsets != nullptr, C, G, aligned16(x) && aligned16(dy) && aligned16(dx) && strides * es % 16 == 0);
+    const Plan p = make_plan(dtype, S, rows, offsets != nullptr, C, G, aligned16(x) && aligned16(dy) && aligned16(dx) && strides * es % 16 == 0, true);
     if (p.rc) return p.rc;
     if (workspace_bytes < ws_bytes_of(p, C, G, true)) return SIS3D_EWORKSPACE;
-    if (!workspace || !aligned16(workspace)) return SIS3D_EINVAL;
+    if (!p.one && (!workspace || !aligned16(workspace))) return SIS3D_EINVAL;
     GnArgs a{};
     a.x = x; a.dy = dy; a.y = dx; a.w = weight; a.b = bias; a.mean = (float *)mean; a.rstd = (float *)rstd; a.off = offsets; a.rows = rows;
     a.x_n = x_sample; a.x_v = x_row; a.d_n = dy_sample; a.d_v = dy_row; a.y_n = dx_sample; a.y_v = dx_row;
-    a.S = S; a.C = C; a.G = G; a.cpg = C / G; a.gpb = p.gpb; a.T = p.T; a.tiles = (int)p.tiles; a.act = act; a.zero_tail = 1;
+    a.S = S; a.C = C; a.G = G; a.cpg = C / G; a.gpb = p.gpb; a.T = p.T; a.t_log = p.t_log; a.tiles = (int)p.tiles; a.zero_tail = 1;
     a.part_c = (float2 *)workspace;
     a.part_g = a.part_c + (size_t)p.tiles * C;
     a.dw = dweight; a.db = dbias;
-    return dispatch(a, p, dtype, true, st);
+    return dispatch(a, p, dtype, act, true, st);
 }

@@ -1645,21 +1645,30 @@ def maxpool3(x, out=None, out_coff=0):
 
 
 # ------------------------------------------------- normalisation and class rows --
+import functools as _functools
+
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/sis3d.h SIS3D_F32 / SIS3D_BF16 / SIS3D_F16
 _ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2}
 
 
 def _on_device(fn):
     """run on the device of the first tensor argument (and on that device's current stream), whatever the current device is"""
-    import functools
-
-    @functools.wraps(fn)
+    @_functools.wraps(fn)
     def call(x, *args, **kwargs):
-        if isinstance(x, torch.Tensor) and x.is_cuda and x.device.index != torch.cuda.current_device():
+        if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() != torch.cuda.current_device():
             with torch.cuda.device(x.device):
                 return fn(x, *args, **kwargs)
         return fn(x, *args, **kwargs)
     return call
+
+
+def _raw_stream(t):
+    """hipStream_t of the current stream of t's device"""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _elem(t, name):
@@ -1677,9 +1686,13 @@ def _side(t, name, like, dtype, shape, optional=True):
         return None
     if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != dtype:
         raise _lib.Sis3dError("%s must be a %s tensor on %s" % (name, dtype, like.device))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise _lib.Sis3dError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 def _one_stride(sizes, strides):
@@ -1696,16 +1709,16 @@ def _one_stride(sizes, strides):
     return step
 
 
-def _channel_rows(t, name, offsets):
-    """(samples, rows, channels, sample stride, row stride) of (N,C,*spatial) in channels-last memory, or of (rows, C) with offsets"""
-    shape, stride = t.shape, t.stride()
-    if offsets is not None:
-        if t.dim() != 2:
+@_functools.lru_cache(maxsize=1024)
+def _channel_rows_of(shape, stride, samples, name):
+    """the answer of _channel_rows for tensors of this shape and these strides; samples: their number with offsets, or None"""
+    if samples is not None:
+        if len(shape) != 2:
             raise _lib.Sis3dError("%s must be (rows, C) with offsets" % name)
-        S, V, C = offsets.numel() - 1, shape[0], shape[1]
-        sn, sv, sc = 0, stride[0] if V > 1 else max(C, 1), stride[1]
+        S, V, C = samples, shape[0], shape[1]
+        sn, sv, sc = 0, stride[0], stride[1]
     else:
-        if t.dim() < 2:
+        if len(shape) < 2:
             raise _lib.Sis3dError("%s must be (N, C, ...)" % name)
         S, C, sc = shape[0], shape[1], stride[1]
         sn = stride[0] if S > 1 else 0
@@ -1713,19 +1726,36 @@ def _channel_rows(t, name, offsets):
         for n in shape[2:]:
             V *= n
         sv = _one_stride(shape[2:], stride[2:])
-    if V == 1:
+    if V <= 1:
         sv = C
-    if t.numel() and ((C > 1 and sc != 1) or sv is None or (V > 1 and sv < C)):
-        raise _lib.Sis3dError("%s must be channels-last in memory (or a channel range of such a tensor), got strides %s" % (name, tuple(stride)))
+    if S * V * C and ((C > 1 and sc != 1) or sv is None or sv < C):
+        raise _lib.Sis3dError("%s must be channels-last in memory (or a channel range of such a tensor), got strides %s" % (name, stride))
     return S, V, C, sn, sv if sv is not None else C
+
+
+def _channel_rows(t, name, offsets):
+    """(samples, rows, channels, sample stride, row stride) of (N,C,*spatial) in channels-last memory, or of (rows, C) with offsets"""
+    return _channel_rows_of(tuple(t.shape), t.stride(), None if offsets is None else offsets.numel() - 1, name)
 
 
 def _like_rows(x, offsets):
     """an uninitialised tensor of x's shape and type, dense channels-last"""
-    if offsets is not None or x.dim() == 2:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
     n = x.dim()
-    return torch.empty((x.shape[0],) + tuple(x.shape[2:]) + (x.shape[1],), dtype=x.dtype, device=x.device).permute(0, n - 1, *range(1, n - 1))
+    if offsets is not None or n == 2:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    shape = tuple(x.shape)
+    C = shape[1]
+    strides, step = [0] * n, C
+    for i in range(n - 1, 1, -1):
+        strides[i] = step
+        step *= shape[i]
+    strides[0], strides[1] = step, 1
+    return torch.empty_strided(shape, strides, dtype=x.dtype, device=x.device)
+
+
+@_functools.lru_cache(maxsize=1024)
+def _norm_workspace(code, S, V, ragged, C, groups, backward):
+    return lib().sis3d_group_norm_workspace_bytes(code, S, V, ragged, C, groups, backward)
 
 
 def _norm_args(x, groups, weight, bias, act, offsets):
@@ -1773,12 +1803,11 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act=None, offsets=No
     mean = rstd = None
     if want_stats:
         mean, rstd = torch.empty(S, groups, dtype=torch.float32, device=x.device), torch.empty(S, groups, dtype=torch.float32, device=x.device)
-    ragged = 0 if offsets is None else 1
-    wsb = lib().sis3d_group_norm_workspace_bytes(code, S, V, ragged, C, groups, 0)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
-    _norm_check(lib().sis3d_group_norm_forward(_ptr(x), code, S, V, _ptr(offsets), sn, sv, C, groups, _ptr(weight), _ptr(bias), float(eps),
-                                               _ACTS[act], _ptr(y), yn, yv, 1 if out is None else 0, _ptr(mean), _ptr(rstd), _ptr(ws), wsb,
-                                               _stream()), "sis3d_group_norm_forward", C, groups)
+    wsb = _norm_workspace(code, S, V, 0 if offsets is None else 1, C, groups, 0)
+    ws = _workspace(wsb, x)
+    _norm_check(lib().sis3d_group_norm_forward(_at(x), code, S, V, _at(offsets), sn, sv, C, groups, _at(weight), _at(bias), float(eps),
+                                               _ACTS[act], _at(y), yn, yv, 1 if out is None else 0, _at(mean), _at(rstd), _at(ws), wsb,
+                                               _raw_stream(x)), "sis3d_group_norm_forward", C, groups)
     return (y, mean, rstd) if want_stats else y
 
 
@@ -1795,24 +1824,22 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, act=N
     dx = _like_rows(x, offsets)
     dw = torch.empty(C, dtype=torch.float32, device=x.device) if weight is not None else None
     db = torch.empty(C, dtype=torch.float32, device=x.device) if bias is not None else None
-    wsb = lib().sis3d_group_norm_workspace_bytes(code, S, V, 0 if offsets is None else 1, C, groups, 1)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
-    _norm_check(lib().sis3d_group_norm_backward(_ptr(dy), dn, dv, _ptr(x), code, S, V, _ptr(offsets), sn, sv, C, groups, _ptr(mean), _ptr(rstd),
-                                                _ptr(weight), _ptr(bias), _ACTS[act], _ptr(dx), V * C, C, _ptr(dw), _ptr(db), _ptr(ws), wsb,
-                                                _stream()), "sis3d_group_norm_backward", C, groups)
+    wsb = _norm_workspace(code, S, V, 0 if offsets is None else 1, C, groups, 1)
+    ws = _workspace(wsb, x)
+    _norm_check(lib().sis3d_group_norm_backward(_at(dy), dn, dv, _at(x), code, S, V, _at(offsets), sn, sv, C, groups, _at(mean), _at(rstd),
+                                                _at(weight), _at(bias), _ACTS[act], _at(dx), V * C, C, _at(dw), _at(db), _at(ws), wsb,
+                                                _raw_stream(x)), "sis3d_group_norm_backward", C, groups)
     return dx, dw, db
 
 
-def _score_rows(score):
-    """(type, shape of the rows, outer count, rows, classes, three element strides) of (R,K) or (N,K,*spatial) class scores"""
-    code = _elem(score, "score")
-    if score.dim() < 2:
+@_functools.lru_cache(maxsize=1024)
+def _score_rows_of(shape, st):
+    if len(shape) < 2:
         raise _lib.Sis3dError("score must be (rows, classes) or (N, classes, ...)")
-    shape, st = tuple(score.shape), score.stride()
     K = shape[1]
     if K < 1:
         raise _lib.Sis3dError("score must have at least one class")
-    if score.dim() == 2:
+    if len(shape) == 2:
         N, V, sn, sv, rows = 1, shape[0], 0, st[0], shape[:1]
     else:
         N, sn, rows = shape[0], st[0], shape[:1] + shape[2:]
@@ -1821,11 +1848,21 @@ def _score_rows(score):
             V *= n
         sv = _one_stride(shape[2:], st[2:])
         if sv is None:
-            raise _lib.Sis3dError("score: the dimensions behind the classes must be dense among themselves, got strides %s" % (tuple(st),))
+            raise _lib.Sis3dError("score: the dimensions behind the classes must be dense among themselves, got strides %s" % (st,))
     sc = st[1] if K > 1 else 1
     if K > 1024 and sc != 1:
         raise Sis3dUnsupported("score: more than 1024 classes must be contiguous in memory (class stride %d)" % sc)
-    return code, rows, N, V, K, sn, sv, sc
+    return rows, N, V, K, sn, sv, sc
+
+
+def _score_rows(score):
+    """(type, shape of the rows, outer count, rows, classes, three element strides) of (R,K) or (N,K,*spatial) class scores"""
+    return (_elem(score, "score"),) + _score_rows_of(tuple(score.shape), score.stride())
+
+
+@_functools.lru_cache(maxsize=1024)
+def _class_workspace(rows, K, sc, top):
+    return lib().sis3d_class_rows_workspace_bytes(rows, K, sc, top)
 
 
 def _num_rows(num, like):
@@ -1865,10 +1902,10 @@ def class_logprobs(score, labels, top=0, num=None):
     dev = score.device
     logp, ent, norm, tl = (torch.empty(rows + tail, dtype=torch.float32, device=dev) for tail in ((), (), (2,), (top,)))
     tc = torch.empty(rows + (top,), dtype=torch.int64, device=dev)
-    wsb = lib().sis3d_class_rows_workspace_bytes(N * V, K, sc, top)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-    check(lib().sis3d_class_logprobs_forward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(labels), _ptr(num), top, _ptr(logp), _ptr(ent),
-                                             _ptr(norm), _ptr(tl), _ptr(tc), _ptr(ws), wsb, _stream()), "sis3d_class_logprobs_forward")
+    wsb = _class_workspace(N * V, K, sc, top)
+    ws = _workspace(wsb, score)
+    check(lib().sis3d_class_logprobs_forward(_at(score), code, N, V, K, sn, sv, sc, _at(labels), _at(num), top, _at(logp), _at(ent),
+                                             _at(norm), _at(tl), _at(tc), _at(ws), wsb, _raw_stream(score)), "sis3d_class_logprobs_forward")
     return logp, ent, norm, tl, tc
 
 
@@ -1885,8 +1922,8 @@ def class_logprobs_backward(score, labels, norm, entropy, grad_logp, grad_entrop
     num = _num_rows(num, score)
     d = _like_score(score, sc)
     _, _, _, _, _, dn, dv, dc = _score_rows(d)
-    check(lib().sis3d_class_logprobs_backward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(labels), _ptr(num), _ptr(norm), _ptr(entropy),
-                                              _ptr(grad_logp), _ptr(grad_entropy), _ptr(d), dn, dv, dc, _stream()),
+    check(lib().sis3d_class_logprobs_backward(_at(score), code, N, V, K, sn, sv, sc, _at(labels), _at(num), _at(norm), _at(entropy),
+                                              _at(grad_logp), _at(grad_entropy), _at(d), dn, dv, dc, _raw_stream(score)),
           "sis3d_class_logprobs_backward")
     return d
 
@@ -1914,10 +1951,10 @@ def distill_loss(score, kept, classes, temperature=1.0, num=None):
     kept, classes, temperature = _teacher(score, kept, classes, rows, temperature)
     num = _num_rows(num, score)
     loss, norm = (torch.empty(rows + tail, dtype=torch.float32, device=score.device) for tail in ((), (2,)))
-    wsb = lib().sis3d_class_rows_workspace_bytes(N * V, K, sc, 0)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=score.device) if wsb else None
-    check(lib().sis3d_distill_forward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(kept), _ptr(classes), kept.shape[-1], _ptr(num), temperature,
-                                      _ptr(loss), _ptr(norm), _ptr(ws), wsb, _stream()), "sis3d_distill_forward")
+    wsb = _class_workspace(N * V, K, sc, 0)
+    ws = _workspace(wsb, score)
+    check(lib().sis3d_distill_forward(_at(score), code, N, V, K, sn, sv, sc, _at(kept), _at(classes), kept.shape[-1], _at(num), temperature,
+                                      _at(loss), _at(norm), _at(ws), wsb, _raw_stream(score)), "sis3d_distill_forward")
     return loss, norm
 
 
@@ -1932,6 +1969,6 @@ def distill_loss_backward(score, kept, classes, norm, grad_loss, temperature=1.0
     num = _num_rows(num, score)
     d = _like_score(score, sc)
     _, _, _, _, _, dn, dv, dc = _score_rows(d)
-    check(lib().sis3d_distill_backward(_ptr(score), code, N, V, K, sn, sv, sc, _ptr(kept), _ptr(classes), kept.shape[-1], _ptr(num), temperature,
-                                       _ptr(norm), _ptr(grad_loss), _ptr(d), dn, dv, dc, _stream()), "sis3d_distill_backward")
+    check(lib().sis3d_distill_backward(_at(score), code, N, V, K, sn, sv, sc, _at(kept), _at(classes), kept.shape[-1], _at(num), temperature,
+                                       _at(norm), _at(grad_loss), _at(d), dn, dv, dc, _raw_stream(score)), "sis3d_distill_backward")
     return d

@@ -406,7 +406,7 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
     from sis3d import _lib
     l = _lib.lib()
     p = ctypes.c_void_p(4096)                                                # never dereferenced
-    fwd = dict(x=p, dtype=0, S=1, rows=10, off=None, xn=0, xv=32, C=32, G=8, w=None, b=None, eps=1e-5, act=0, y=p, yn=0, yv=32, tail=0, mean=None,
+    fwd = dict(x=p, dtype=0, S=1, rows=10 ** 6, off=None, xn=0, xv=32, C=32, G=8, w=None, b=None, eps=1e-5, act=0, y=p, yn=0, yv=32, tail=0, mean=None,
                rstd=None, ws=p, wsb=1 << 30, stream=None)
 
     def forward(**k):
@@ -417,7 +417,7 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
     assert forward(wsb=0) == -3
     assert forward(C=4099, G=1, xv=4099, yv=4099) == -4
     assert forward(rows=0) == 0 and forward(S=0) == 0
-    bwd = dict(dy=p, dn=0, dv=32, x=p, dtype=0, S=1, rows=10, off=None, xn=0, xv=32, C=32, G=8, mean=p, rstd=p, w=None, b=None, act=0, dx=p, gn=0,
+    bwd = dict(dy=p, dn=0, dv=32, x=p, dtype=0, S=1, rows=10 ** 6, off=None, xn=0, xv=32, C=32, G=8, mean=p, rstd=p, w=None, b=None, act=0, dx=p, gn=0,
                gv=32, dw=None, db=None, ws=p, wsb=1 << 30, stream=None)
 
     def backward(**k):
@@ -426,7 +426,13 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
         assert backward(**k) == -1, k
     assert backward(wsb=16) == -3 and backward(rows=0) == 0
     assert l.sis3d_group_norm_workspace_bytes(0, 1, 10, 0, 32, 5, 0) == 0
-    assert l.sis3d_group_norm_workspace_bytes(0, 1, 10 ** 6, 0, 32, 8, 1) > 0
+    for ragged in (0, 1):
+        for backward in (0, 1):
+            assert l.sis3d_group_norm_workspace_bytes(0, 0, 0, ragged, 32, 8, backward) >= 0        # no rows: an answer, not a division by them
+            assert l.sis3d_group_norm_workspace_bytes(2, 3, 0, ragged, 32, 8, backward) >= 0
+    # one launch, nothing to keep, where a sample is small; a sum over several samples' gradients takes two
+    size = l.sis3d_group_norm_workspace_bytes
+    assert size(0, 1, 10 ** 6, 0, 32, 8, 1) > 0 and size(0, 1, 10, 0, 32, 8, 1) == 0 and size(0, 2, 10, 0, 32, 8, 0) == 0 and size(0, 2, 10, 0, 32, 8, 1) > 0
 
 
 def test_reference_gradients_are_slopes():
