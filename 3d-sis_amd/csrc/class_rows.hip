@@ -10,8 +10,8 @@
 // All of it is bound by reading the scores once (and writing the gradient once).  Forward keeps a running maximum m and the sums
 // s = sum e^((l - m) / T) and t = sum (l - m) e^((l - m) / T) per lane, rescaled when m grows, so a row is read once whatever its length;
 // H = log s - t / s needs no second pass.  Everything is held in 32 bits.
-// A row's L is kept as the pair (m, log s): p = exp((l - m) / T - log s) then has no rounding of a large L in it, and rows of the
-// type's lowest value come out as what they are (all classes alike).
+// A row's L is kept as the pair (m, s): p = exp((l - m) / T) / s then has no rounding of a large L in it, and rows of the type's lowest
+// value come out as what they are (all classes alike).
 //
 // Three forms, by the number of classes:
 //   K <= 1024        a group of 1 .. 64 lanes holds a row in registers; class-strided (planar) scores give neighbouring rows to
@@ -40,7 +40,7 @@ struct RowArgs {
     const int64_t *labels;
     int top;
     float *logp, *entropy, *top_logp;
-    float2 *norm;                              // (m, log s) of each row
+    float2 *norm;                              // (m, s) of each row
     int64_t *top_class;
     const float *kept;                         // (R, nk)
     const int64_t *cls;
@@ -114,39 +114,76 @@ struct Soft {
         s += o.s;
         t += o.t;
     }
-    __device__ void join_xor(int o, float c2)
-    {
-        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o), t2 = __shfl_xor(t, o);
-        // the same order on both sides, so that every lane ends with the same bits
-        if (threadIdx.x & o) { Soft a{m2, s2, t2}; a.join(m, s, t, c2); *this = a; }
-        else join(m2, s2, t2, c2);
-    }
-    __device__ float2 norm() const { return make_float2(m, s == 0.f ? -INFINITY : logf(s)); }      // s = 0: a row of nothing but -inf
+    __device__ void join_wave(float c2);
+    __device__ float log_s() const { return s == 0.f ? -INFINITY : logf(s); }      // s = 0: a row of nothing but -inf
     __device__ float entropy() const { return s == 0.f ? 0.f : logf(s) - LN2 * (t / s); }
 };
 
+// (m, log s) of a row, for the few log probabilities that it reports
+struct Norm { float m, ls; };
+
 // l / T - L, -inf where L is
-__device__ inline float log_p(float l, float2 norm, float inv, float inv_lo)
+__device__ inline float log_p(float l, Norm n, float inv, float inv_lo)
 {
-    const float d = l - norm.x;
-    return norm.y == -INFINITY ? -INFINITY : fmaf(d, inv, fmaf(fmaxf(d, LOWEST), inv_lo, -norm.y));
+    const float d = l - n.m;
+    return n.ls == -INFINITY ? -INFINITY : fmaf(d, inv, fmaf(fmaxf(d, LOWEST), inv_lo, -n.ls));
 }
 
-__device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, float2 norm)
+__device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, Norm n)
 {
     const int64_t y = a.labels[r];
-    return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, norm, 1.f, 0.f));
+    return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, n, 1.f, 0.f));
 }
 
-__device__ inline float lp_grad(float l, float2 norm, float h, float ga, float ge)
-{
-    const float lp = log_p(l, norm, 1.f, 0.f), p = exp2_(lp * LOG2E);
-    return -p * (ga + ge * (fmaxf(lp, -200.f) + h));
-}
-__device__ inline float kd_p(const RowArgs &a, float l, float2 norm) { return exp2_(log_p(l, norm, a.inv, a.inv_lo) * LOG2E); }
+// a row in the backward direction
+struct Back {
+    float m, is, ls, h, ga, ge;                // 1 / s (0 for a row of nothing but -inf), log s, entropy, gradients (ga: times T for the loss)
+    __device__ Back(float2 norm) : m(norm.x), is(norm.y == 0.f ? 0.f : 1.f / norm.y), ls(0.f), h(0.f), ga(0.f), ge(0.f) {}
+    __device__ void set_log_s(float s) { ls = s == 0.f ? 0.f : logf(s); }
+    __device__ float p(float l, float c2) const { return exp2_((l - m) * c2) * is; }
+    __device__ float lp_grad(float l) const
+    {
+        const float d = l - m;
+        return -(exp2_(d * LOG2E) * is) * fmaf(ge, fmaxf(d, -200.f) - ls + h, ga);      // p is 0 from there on, and 0 * inf is not wanted
+    }
+};
 
 // a teacher's entry: 0 = absent, 1 = present, 2 = no such class
 __device__ inline int entry(const RowArgs &a, int64_t c) { return c < 0 ? 0 : (c >= a.K ? 2 : 1); }
+
+// sum / maximum over a wave in the vector pipe (row shifts by 1, 2, 4, 8, then the rows' last lanes broadcast): every lane gets it
+template <int CTRL, int ROWS> __device__ inline float dpp(float old, float v)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ inline float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ inline float wave_sum(float v)
+{
+    v += dpp<0x111, 0xf>(0.f, v);
+    v += dpp<0x112, 0xf>(0.f, v);
+    v += dpp<0x114, 0xf>(0.f, v);
+    v += dpp<0x118, 0xf>(0.f, v);
+    v += dpp<0x142, 0xa>(0.f, v);
+    v += dpp<0x143, 0xc>(0.f, v);
+    return last_lane(v);
+}
+__device__ inline float wave_max(float v)
+{
+    v = fmaxf(v, dpp<0x111, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x112, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x114, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x118, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp<0x143, 0xc>(v, v));
+    return last_lane(v);
+}
+
+__device__ inline void Soft::join_wave(float c2)
+{
+    raise(wave_max(m), c2);
+    s = wave_sum(s);
+    t = wave_sum(t);
+}
 
 // ---------------------------------------------------------------- K <= 1024: a row in the registers of 1 .. 64 lanes --
 struct Group {
@@ -210,7 +247,7 @@ __device__ inline Teacher group_teacher(const RowArgs &a, const Group &g)
     return t;
 }
 // the part of the loss that one lane's entries of a row give; q log q is 0 at q = 0
-template <typename T> __device__ inline float teacher_loss(const RowArgs &a, const Group &g, const Teacher &t, const T *row, float2 norm)
+template <typename T> __device__ inline float teacher_loss(const RowArgs &a, const Group &g, const Teacher &t, const T *row, Norm norm)
 {
     float loss = 0.f;
     if (!t.any) return loss;
@@ -243,13 +280,13 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     for (int e = 0; e < E; ++e) so.add(v[e], a.c2);
     so.s = group_sum(so.s, g);
     so.t = group_sum(so.t, g);
-    const float2 norm = so.norm();
+    const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
         const Teacher t = group_teacher(a, g);
         const float loss = a.tau * a.tau * group_sum(g.live ? teacher_loss(a, g, t, p, norm) : 0.f, g);
         if (g.sub == 0 && g.in) {
             a.loss[g.r] = !g.live ? 0.f : (t.bad ? NAN : loss);
-            a.norm[g.r] = g.live ? norm : make_float2(0.f, 0.f);
+            a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
         }
         return;
     }
@@ -257,7 +294,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
         const int64_t y = a.labels[g.at];
         a.logp[g.r] = g.live ? label_logp(a, g.r, y >= 0 && y < a.K ? sis3d_f32(p[y * a.s_c]) : 0.f, norm) : 0.f;
         a.entropy[g.r] = g.live ? so.entropy() : 0.f;
-        a.norm[g.r] = g.live ? norm : make_float2(0.f, 0.f);
+        a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
     }
     uint32_t taken = 0;
     for (int i = 0; i < a.top; ++i) {
@@ -287,19 +324,19 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     float q[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) q[e] = 0.f;
-    float ga = 0.f, ge = 0.f, h = 0.f;
-    float2 norm = a.norm_in[g.at];
+    Back k(a.norm_in[g.at]);
     if constexpr (MODE == LP) {
         const int64_t y = a.labels[g.at];
-        h = a.entropy_in[g.at];
-        ga = y < 0 ? 0.f : (y >= a.K ? NAN : a.g1[g.at]);
-        ge = a.g2 ? a.g2[g.at] : 0.f;
+        k.set_log_s(a.norm_in[g.at].y);
+        k.h = a.entropy_in[g.at];
+        k.ga = y < 0 ? 0.f : (y >= a.K ? NAN : a.g1[g.at]);
+        k.ge = a.g2 ? a.g2[g.at] : 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (g.sub + e * g.lpr == y) q[e] = ga;
+            if (g.sub + e * g.lpr == y) q[e] = k.ga;
     } else {
         const Teacher t = group_teacher(a, g);
-        ga = t.bad ? NAN : (t.any ? a.g1[g.at] * a.tau : 0.f);
+        k.ga = t.bad ? NAN : (t.any ? a.g1[g.at] * a.tau : 0.f);
         if (t.any)
             for (int i = 0; i < a.nk; ++i) {
                 const int64_t c = a.cls[g.at * a.nk + i];
@@ -315,8 +352,8 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
         if (c >= a.K || !g.in) continue;
         const float l = sis3d_f32(p[c * a.s_c]);
         float o;
-        if constexpr (MODE == LP) o = lp_grad(l, norm, h, ga, ge) + q[e];
-        else o = ga * (kd_p(a, l, norm) - q[e]);
+        if constexpr (MODE == LP) o = k.lp_grad(l) + q[e];
+        else o = k.ga * (k.p(l, a.c2) - q[e]);
         d[c * a.d_c] = sis3d_from_f32<T>(g.live ? o : 0.f);
     }
 }
@@ -351,6 +388,22 @@ template <typename T> struct Span {
     __device__ int edges() const { return head + tail; }
 };
 
+// batch<N>(v): a lane's N vectors v, v + NL, ..., all there but perhaps the last.  Whole batches of UL, then one of what is left: without
+// a condition between the loads of a batch, so that they are in flight together.
+constexpr int UL = 4;
+template <int N> struct Count {};
+template <int NL, typename F> __device__ inline void each_batch(int nvec, int lane, F batch)
+{
+    int v = lane;
+    for (int left = nvec / (UL * NL); left > 0; --left, v += UL * NL) batch(Count<UL>(), v);
+    switch ((nvec - nvec / (UL * NL) * (UL * NL) + NL - 1) / NL) {
+    case 1: batch(Count<1>(), v); break;
+    case 2: batch(Count<2>(), v); break;
+    case 3: batch(Count<3>(), v); break;
+    case 4: batch(Count<4>(), v); break;
+    }
+}
+
 template <typename T, int W, int MODE> struct Long {
     static constexpr int NL = 64 * W, CAP = W == 1 ? 512 : 1024, VEC = 16 / sizeof(T);
     struct Shared {
@@ -367,26 +420,35 @@ template <typename T, int W, int MODE> struct Long {
         so.init();
         float best = -INFINITY;
         int at = lane();
-        for (int v = lane(); v < sp.nvec; v += NL) {
-            float x[VEC];
-            sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
-            float mx = x[0];
+        const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
+        each_batch<NL>(sp.nvec, lane(), [&]<int N>(Count<N>, int v) {
+            SisVec<T, VEC> raw[N];
 #pragma unroll
-            for (int i = 1; i < VEC; ++i) mx = fmaxf(mx, x[i]);
-            if constexpr (MODE == LP) at = mx > best ? v : at;
-            best = fmaxf(best, mx);
-            so.raise(fmaxf(so.m, mx), a.c2);
+            for (int u = 0; u < N; ++u) raw[u] = *(const SisVec<T, VEC> *)(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
+            const bool last = v + (N - 1) * NL < sp.nvec;       // no vector: -inf adds nothing
+            float x[N][VEC], top = so.m;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) so.add(x[i], a.c2);
-        }
-        // the key of a vector: its first class stands for the place of its maximum, vectors being disjoint ranges of classes
+            for (int u = 0; u < N; ++u) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[u][i] = u < N - 1 || last ? sis3d_f32(raw[u].v[i]) : -INFINITY;
+                float mx = x[u][0];
+#pragma unroll
+                for (int i = 1; i < VEC; ++i) mx = fmaxf(mx, x[u][i]);
+                if constexpr (MODE == LP) at = mx > best ? v + u * NL : at;
+                best = fmaxf(best, mx);
+                top = fmaxf(top, mx);
+            }
+            so.raise(top, a.c2);
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) so.add(x[u][i], a.c2);
+        });
+        // the key of a vector: its last class stands for the place of its maximum, vectors being disjoint ranges of classes
         best_key = lane() < sp.nvec ? key_of(best, sp.first_class(at) + VEC - 1) : 0;
-        if (lane() < sp.edges()) {
-            const float l = sis3d_f32(sp.row[sp.edge_class(lane())]);
-            so.raise(fmaxf(so.m, l), a.c2);
-            so.add(l, a.c2);
-        }
-        for (int o = 32; o > 0; o >>= 1) so.join_xor(o, a.c2);
+        so.raise(fmaxf(so.m, edge), a.c2);
+        if (lane() < sp.edges()) so.add(edge, a.c2);
+        so.join_wave(a.c2);
         if constexpr (W > 1) {
             if ((threadIdx.x & 63) == 0) {
                 sh.red[threadIdx.x >> 6][0] = so.m;
@@ -489,23 +551,24 @@ __device__ inline Group wave_group(int64_t r)
     return g;
 }
 
-template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t r, const T *row, float2 norm)
+template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t r, const T *row, const Soft &so)
 {
+    const Norm norm{so.m, so.log_s()};
     const Group g = wave_group(r);
     const Teacher t = group_teacher(a, g);
     const float loss = a.tau * a.tau * group_sum(teacher_loss(a, g, t, row, norm), g);
     if (g.sub == 0) {
         a.loss[r] = t.bad ? NAN : loss;
-        a.norm[r] = norm;
+        a.norm[r] = make_float2(so.m, so.s);
     }
 }
 
-template <typename T> __device__ inline void row_outputs(const RowArgs &a, int64_t r, const T *row, const Soft &so, float2 norm)
+template <typename T> __device__ inline void row_outputs(const RowArgs &a, int64_t r, const T *row, const Soft &so, Norm norm)
 {
     const int64_t y = a.labels[r];
     a.logp[r] = label_logp(a, r, y >= 0 && y < a.K ? sis3d_f32(row[y]) : 0.f, norm);
     a.entropy[r] = so.entropy();
-    a.norm[r] = norm;
+    a.norm[r] = make_float2(so.m, so.s);
 }
 
 // outputs of a row past the live count, by a team of `n` lanes
@@ -535,9 +598,9 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     const Span<T> sp(row, 0, a.K);
     uint64_t best;
     const Soft so = L::pass(a, sp, sh, best);
-    const float2 norm = so.norm();
+    const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
-        if (W == 1 || threadIdx.x < 64) wave_loss(a, r, row, norm);
+        if (W == 1 || threadIdx.x < 64) wave_loss(a, r, row, so);
     } else {
         if (L::lane() == 0) row_outputs(a, r, row, so, norm);
         if (a.top)
@@ -581,10 +644,10 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join
         const float4 v = *(const float4 *)(a.part + ((size_t)r * a.parts + lane) * 4);
         so = Soft{v.x, v.y, v.z};
     }
-    for (int o = 32; o > 0; o >>= 1) so.join_xor(o, a.c2);
-    const float2 norm = so.norm();
+    so.join_wave(a.c2);
+    const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
-        wave_loss(a, r, row, norm);
+        wave_loss(a, r, row, so);
     } else {
         if (lane == 0) row_outputs(a, r, row, so, norm);
         if (!a.top) return;
@@ -626,14 +689,14 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
         for (int c = k0 + lane; c < k1; c += NL) out[c] = sis3d_from_f32<T>(0.f);
         return;
     }
-    const float2 norm = a.norm_in[r];
-    float ga, ge = 0.f, h = 0.f;
+    Back k(a.norm_in[r]);
     int y = -1;
     if constexpr (MODE == LP) {
         const int64_t label = a.labels[r];
-        h = a.entropy_in[r];
-        ga = label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[r]);
-        ge = a.g2 ? a.g2[r] : 0.f;
+        k.set_log_s(a.norm_in[r].y);
+        k.h = a.entropy_in[r];
+        k.ga = label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[r]);
+        k.ge = a.g2 ? a.g2[r] : 0.f;
         y = label >= 0 && label < a.K ? (int)label : -1;
     } else {
         const Teacher t = group_teacher(a, wave_group(r));
@@ -644,26 +707,33 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
                 c_s[team][i] = on ? (int)c : -1;
                 q_s[team][i] = on ? exp2_((a.kept[r * a.nk + i] - t.m) * a.c2) / t.s : 0.f;
             }
-        ga = t.bad ? NAN : (t.any ? a.g1[r] * a.tau : 0.f);
+        k.ga = t.bad ? NAN : (t.any ? a.g1[r] * a.tau : 0.f);
     }
     const Span<T> sp(row, k0, k1);
+    const float gs = k.ga * k.is;
     auto grad = [&](float l, int c) {
-        if constexpr (MODE == LP) return lp_grad(l, norm, h, ga, ge) + (c == y ? ga : 0.f);
-        else return ga * kd_p(a, l, norm);
+        if constexpr (MODE == LP) return k.lp_grad(l) + (c == y ? k.ga : 0.f);
+        else return gs * exp2_((l - k.m) * a.c2);
     };
     const bool wide = ((uintptr_t)(out + k0 + sp.head) & 15) == 0;
-    for (int v = lane; v < sp.nvec; v += NL) {
-        float x[VEC];
-        sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
-        const int c = sp.first_class(v);
+    each_batch<NL>(sp.nvec, lane, [&]<int N>(Count<N>, int v) {
+        SisVec<T, VEC> raw[N];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[i] = grad(x[i], c + i);
-        if (wide) sis3d_store<T, VEC>(out + c, x);
-        else {
+        for (int u = 0; u < N; ++u) raw[u] = *(const SisVec<T, VEC> *)(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) out[c + i] = sis3d_from_f32<T>(x[i]);
+        for (int u = 0; u < N; ++u) {
+            const int c = sp.first_class(v + u * NL);
+            float x[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[i] = grad(sis3d_f32(raw[u].v[i]), c + i);
+            if (u == N - 1 && v + u * NL >= sp.nvec) continue;
+            if (wide) sis3d_store<T, VEC>(out + c, x);
+            else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) out[c + i] = sis3d_from_f32<T>(x[i]);
+            }
         }
-    }
+    });
     if (lane < sp.edges()) {
         const int c = sp.edge_class(lane);
         out[c] = sis3d_from_f32<T>(grad(sis3d_f32(row[c]), c));
@@ -682,7 +752,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
                     q += q_s[team][j];
                     first = first && j >= i;
                 }
-            if (first) out[c] = sis3d_from_f32<T>(ga * (kd_p(a, sis3d_f32(row[c]), norm) - q));
+            if (first) out[c] = sis3d_from_f32<T>(k.ga * (k.p(sis3d_f32(row[c]), a.c2) - q));
         }
     }
 }

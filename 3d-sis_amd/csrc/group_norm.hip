@@ -33,8 +33,8 @@ struct GnArgs {
     int64_t x_n, x_v, d_n, d_v, y_n, y_v;     // element strides between samples and rows of x, dy, y / dx
     int S, C, G, cpg, gpb, T, t_log, tiles, zero_tail;     // T rows a tile; ragged: T = 1 << t_log
     float eps;
-    double2 *part;                // forward: [workgroups][G] (sum, sum of squares)
-    float2 *part_g, *part_c;      // backward: [workgroups][G] and [workgroups][C]
+    double2 *part;                // forward: [G][workgroups] (sum, sum of squares)
+    float2 *part_g, *part_c;      // backward: [G][workgroups] and [workgroups][C]
     float *dw, *db;
 };
 
@@ -149,14 +149,14 @@ template <typename P, typename F> __device__ inline void reduce_groups(const P *
     }
 }
 
-// The same over the tiles of one sample: part[(first + p) * G + g]
-template <typename P, typename F> __device__ inline void reduce_tiles(const P *part, int first, int ntiles, int G, int g0, int gl, F out)
+// The same over the tiles of one sample: part[g * tiles + first + p], so that a wave reads neighbouring tiles
+template <typename P, typename F> __device__ inline void reduce_tiles(const P *part, int tiles, int first, int ntiles, int g0, int gl, F out)
 {
     const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
         double s0 = 0, s1 = 0;
         for (int p = l; p < ntiles; p += lp) {
-            const P v = part[(size_t)(first + p) * G + g0 + g];
+            const P v = part[(size_t)(g0 + g) * tiles + first + p];
             s0 += v.x;
             s1 += v.y;
         }
@@ -181,22 +181,41 @@ template <int ACT> __device__ inline float act_slope(float z)
     } else return 1.f;
 }
 
-// f(row) for this thread's rows of a tile, U of them at a time: loads first, so that U are in flight
+// f(row, there, vectors) for this thread's rows of a tile, U rows at a time, loads first so that they are in flight together.  In the last
+// batch rows that are not there repeat the tile's last one (there = false): no condition stands between the loads.
 template <typename T, int VEC, typename F> __device__ inline void each_row(const T *x, int64_t stride, int ri, int rpb, int n, F f)
 {
-    for (int r = ri; r < n; r += U * rpb) {
+    int r = ri;
+    for (int left = n / (U * rpb); left > 0; --left, r += U * rpb) {
+        SisVec<T, VEC> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *(const SisVec<T, VEC> *)(x + (r + u * rpb) * stride);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(r + u * rpb, true, v[u]);
+    }
+    if (r < n) {
         SisVec<T, VEC> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = *(const SisVec<T, VEC> *)(x + min(r + u * rpb, n - 1) * stride);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (r + u * rpb < n) f(r + u * rpb, v[u]);
+        for (int u = 0; u < U; ++u) f(r + u * rpb, r + u * rpb < n, v[u]);
     }
 }
 template <typename T, int VEC, typename F>
 __device__ inline void each_row2(const T *x, int64_t xs, const T *d, int64_t ds, int ri, int rpb, int n, F f)
 {
-    for (int r = ri; r < n; r += U * rpb) {
+    int r = ri;
+    for (int left = n / (U * rpb); left > 0; --left, r += U * rpb) {
+        SisVec<T, VEC> v[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] = *(const SisVec<T, VEC> *)(x + (r + u * rpb) * xs);
+            w[u] = *(const SisVec<T, VEC> *)(d + (r + u * rpb) * ds);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(r + u * rpb, true, v[u], w[u]);
+    }
+    if (r < n) {
         SisVec<T, VEC> v[U], w[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -205,8 +224,7 @@ __device__ inline void each_row2(const T *x, int64_t xs, const T *d, int64_t ds,
             w[u] = *(const SisVec<T, VEC> *)(d + at * ds);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (r + u * rpb < n) f(r + u * rpb, v[u], w[u]);
+        for (int u = 0; u < U; ++u) f(r + u * rpb, r + u * rpb < n, v[u], w[u]);
     }
 }
 
@@ -220,11 +238,11 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
 #pragma unroll
         for (int i = 0; i < VEC; ++i) K[i] = s1[i] = s2[i] = 0.f;
         if (k.ri < n) sis3d_load<T, VEC>(x + k.ri * a.x_v, K);
-        each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int, const SisVec<T, VEC> &v) {
-            ++m;
+        each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int, bool there, const SisVec<T, VEC> &v) {
+            m += there;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float d = sis3d_f32(v.v[i]) - K[i];
+                const float d = there ? sis3d_f32(v.v[i]) - K[i] : 0.f;
                 s1[i] += d;
                 s2[i] = fmaf(d, d, s2[i]);
             }
@@ -273,11 +291,11 @@ __device__ inline void apply_rows(const GnArgs &a, const Cols &k, const float *s
         sc[i] = st[k.gl + g] * (a.w ? a.w[k.c + i] : 1.f);
         sh[i] = a.b ? a.b[k.c + i] : 0.f;
     }
-    each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int r, const SisVec<T, VEC> &v) {
+    each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int r, bool there, const SisVec<T, VEC> &v) {
         float o[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = act<ACT>(fmaf(sis3d_f32(v.v[i]) - mu[i], sc[i], sh[i]));
-        sis3d_store<T, VEC>(y + r * a.y_v, o);
+        if (there) sis3d_store<T, VEC>(y + r * a.y_v, o);
     });
 }
 
@@ -301,7 +319,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(NT) void gn_stats(Gn
     if (t.s < 0 || t.s >= a.S || t.n == 0) return;
     const Cols k = columns<VEC>(a);
     tile_sums<T, VEC>(a, k, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), t.n, lds,
-                      [&](int g, double s0, double s1) { a.part[(size_t)blockIdx.x * a.G + k.g0 + g] = make_double2(s0, s1); });
+                      [&](int g, double s0, double s1) { a.part[(size_t)(k.g0 + g) * a.tiles + blockIdx.x] = make_double2(s0, s1); });
 }
 
 template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_apply(GnArgs a)
@@ -313,7 +331,7 @@ template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn
     const Cols k = columns<VEC>(a);
     T *y = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
     if (t.s >= a.S) { zero_rows<T, VEC>(a, k, y, t.n); return; }
-    reduce_tiles(a.part, t.first, t.ntiles, a.G, k.g0, k.gl, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
+    reduce_tiles(a.part, a.tiles, t.first, t.ntiles, k.g0, k.gl, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
     __syncthreads();
     apply_rows<T, VEC, ACT>(a, k, st, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), y, t.n);
 }
@@ -360,13 +378,13 @@ __device__ inline void tile_grad_sums(const GnArgs &a, const Cols &k, const Tile
         float s0[VEC], s1[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s0[i] = s1[i] = 0.f;
-        each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
+        each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int, bool there, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float h = (sis3d_f32(v.v[i]) - c.mu[i]) * c.rs[i];
                 const float e = sis3d_f32(d.v[i]) * act_slope<ACT>(fmaf(h, c.w[i], c.b[i]));
-                s0[i] += e;
-                s1[i] = fmaf(e, h, s1[i]);
+                s0[i] += there ? e : 0.f;
+                s1[i] += there ? e * h : 0.f;
             }
         });
 #pragma unroll
@@ -413,7 +431,7 @@ __device__ inline void apply_grad(const GnArgs &a, const Cols &k, const Tile &t,
         m1[i] = st[g];
         m2[i] = st[k.gl + g];
     }
-    each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int r, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
+    each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int r, bool there, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
         float o[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -421,7 +439,7 @@ __device__ inline void apply_grad(const GnArgs &a, const Cols &k, const Tile &t,
             const float e = sis3d_f32(d.v[i]) * act_slope<ACT>(fmaf(h, c.w[i], c.b[i])) * c.w[i];
             o[i] = c.rs[i] * (e - fmaf(h, m2[i], m1[i]));
         }
-        sis3d_store<T, VEC>(dx + r * a.y_v, o);
+        if (there) sis3d_store<T, VEC>(dx + r * a.y_v, o);
     });
 }
 
@@ -437,7 +455,7 @@ template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn
     tile_grad_sums<T, VEC, ACT>(
         a, k, t, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), rows_at<T>(a.dy, a, k, t, a.d_n, a.d_v), (float2 *)ldsd,
         [&](int c, double s0, double s1) { a.part_c[(size_t)blockIdx.x * a.C + c] = make_float2((float)s0, (float)s1); },
-        [&](int g, double s0, double s1) { a.part_g[(size_t)blockIdx.x * a.G + k.g0 + g] = make_float2((float)s0, (float)s1); });
+        [&](int g, double s0, double s1) { a.part_g[(size_t)(k.g0 + g) * a.tiles + blockIdx.x] = make_float2((float)s0, (float)s1); });
 }
 
 template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn_back_apply(GnArgs a)
@@ -474,7 +492,7 @@ template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn
     T *dx = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
     if (t.s >= a.S) { zero_rows<T, VEC>(a, k, dx, t.n); return; }
     const double m = (double)t.len * a.cpg;
-    reduce_tiles(a.part_g, t.first, t.ntiles, a.G, k.g0, k.gl, [&](int g, double s0, double s1) {
+    reduce_tiles(a.part_g, a.tiles, t.first, t.ntiles, k.g0, k.gl, [&](int g, double s0, double s1) {
         st[g] = (float)(s0 / m);
         st[k.gl + g] = (float)(s1 / m);
     });
@@ -524,13 +542,14 @@ Plan make_plan(int dtype, int S, int64_t rows, int ragged, int C, int G, bool wi
     // a column block is one 128-byte line of a row, or one group if that is wider: the narrower it is, the fewer groups a workgroup of
     // the second launch has to add the tiles' sums of
     p.gpb = gu;
-    while (p.gpb < G && p.gpb * cpg * es < 128 && p.gpb + gu <= most) p.gpb += gu;
+    const int64_t total = ragged ? rows : rows * S;
+    // one workgroup takes a whole sample where that is little: up to 128 KB of a line it is sooner done than a second launch.  Its column
+    // blocks are narrower than a line while there are fewer than 512 of them: the rows come from cache, and more CUs take part
+    p.one = rows * (cpg * gu * es > 128 ? cpg * gu * es : 128) <= 128 * 1024 && !(backward && (S != 1 || ragged));
+    while (p.gpb < G && p.gpb * cpg * es < 128 && p.gpb + gu <= most && !(p.one && (int64_t)S * G / p.gpb <= 512)) p.gpb += gu;
     if (p.gpb > G) p.gpb = G;
     p.ncol = (G + p.gpb - 1) / p.gpb;
-    const int64_t total = ragged ? rows : rows * S, seg = (int64_t)p.gpb * cpg * es;
     int64_t T;
-    // one workgroup takes a whole sample where that is little: up to 128 KB of a column block it is sooner done than a second launch
-    p.one = rows * seg <= 128 * 1024 && !(backward && (S != 1 || ragged));
     if (p.one) T = rows;
     else {
         T = (total * p.ncol + 511) / 512;                  // about two workgroups per CU

@@ -1891,7 +1891,7 @@ def class_logprobs(score, labels, top=0, num=None):
     score (R,K), or (N,K,*spatial) planar or channels-last, fp32 / bf16 / fp16; labels int64 (R,) or (N,*spatial): a negative label is
     none (log probability 0).  num: int32 tensor with the number of live rows (detection passes pad theirs): outputs behind are 0.
     -> (logp, entropy, norm, top_logp, top_class): logp / entropy fp32 like labels; norm (...,2) for the backward pass (a row's
-    largest score and the log of its sum relative to it: they add up to the row's log-sum-exp); top_logp fp32 / top_class int64
+    largest score m and the sum s of exp(score - m): m + log s is the row's log-sum-exp); top_logp fp32 / top_class int64
     (...,top), best first, the lowest class first among equal scores; top <= min(32, K)."""
     code, rows, N, V, K, sn, sv, sc = _score_rows(score)
     top = int(top)

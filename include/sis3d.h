@@ -590,7 +590,7 @@ int sis3d_group_norm_backward(const void *dy, int64_t dy_sample, int64_t dy_row,
  * score: `dtype` elements; N * V rows, row r = n * V + v at n * s_n + v * s_v, class c of it c * s_c further (element strides): rows
  * (1, R, s_v = K, s_c = 1), channels-last and planar maps ((N,K,...) with s_c = V) alike.  K > 1024 needs s_c = 1 (else EUNSUPPORTED).
  * num_rows: device int32, live rows (NULL: all); the rows behind are not read and their outputs are zero.
- * norm [R][2]: the row's largest score m and log sum exp((l - m) / T); their sum (m / T + ...) is the row's log-sum-exp.
+ * norm [R][2]: the row's largest score m and s = sum exp((l - m) / T): m / T + log s is the row's log-sum-exp.
  *   sis3d_class_logprobs_forward   logp [R] = log p(labels[r]) (0 where the label is negative, NaN where it is >= K), entropy [R] (nat),
  *                                  top_logp / top_class [R][top] the largest scores in descending order, the lowest class first among equal
  *                                  ones, NaN ranked with -inf.  top <= min(32, K), 0: none.  -inf scores have p = 0; a row of nothing but
