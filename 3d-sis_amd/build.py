@@ -31,7 +31,7 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     os.makedirs(OBJ, exist_ok=True)
     base = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
-    hdrs = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "mfma16.h"), os.path.join(CSRC, "elem.h"), os.path.join(ROOT, "include", "sis3d.h")]
+    hdrs = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "mfma16.h"), os.path.join(ROOT, "include", "sis3d.h")]
     objs, jobs = [], []
     # slowest translation units first so the pool drains evenly
     for name in FAST + EXACT:
@@ -39,7 +39,7 @@ def build(force=False, verbose=True):
         if not os.path.exists(src):
             continue
         obj = os.path.join(OBJ, name.replace(".hip", ".o"))
-        if force or _newer(src, obj) or any(_newer(h, obj) for h in hdrs):
+        if force or _newer(src, obj) or any(_newer(h, obj) for h in hdrs + ([os.path.join(CSRC, "elem.h")] if name in NO_PACKED else [])):
             jobs.append(base + (["-ffp-contract=off"] if name in EXACT else []) + (["-fno-slp-vectorize"] if name == "conv3d_wino.hip" else [])
                         + (["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if name in NO_PACKED else []) + ["-c", src, "-o", obj])
         objs.append(obj)

@@ -88,69 +88,6 @@ __device__ inline uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__sh
 __device__ inline uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ inline uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-// running sums of a softmax: m in score units (never below LOWEST), s = sum 2^x, t = sum x 2^x, x = (l - m) c2
-struct Soft {
-    float m, s, t;
-    __device__ void init() { m = LOWEST; s = t = 0.f; }
-    __device__ void raise(float to, float c2)
-    {
-        const float x = (m - to) * c2, f = exp2_(x);
-        t = f * fmaf(fmaxf(x, -200.f), s, t);          // -200: 2^x is 0 from there on, and 0 * inf is not wanted
-        s *= f;
-        m = to;
-    }
-    __device__ void add(float l, float c2)             // l <= m
-    {
-        const float x = (l - m) * c2, e = exp2_(x);
-        s += e;
-        t = fmaf(fmaxf(x, -200.f), e, t);
-    }
-    __device__ void join(float m2, float s2, float t2, float c2)
-    {
-        Soft o{m2, s2, t2};
-        const float to = fmaxf(m, m2);
-        raise(to, c2);
-        o.raise(to, c2);
-        s += o.s;
-        t += o.t;
-    }
-    __device__ void join_wave(float c2);
-    __device__ float log_s() const { return s == 0.f ? -INFINITY : logf(s); }      // s = 0: a row of nothing but -inf
-    __device__ float entropy() const { return s == 0.f ? 0.f : logf(s) - LN2 * (t / s); }
-};
-
-// (m, log s) of a row, for the few log probabilities that it reports
-struct Norm { float m, ls; };
-
-// l / T - L, -inf where L is
-__device__ inline float log_p(float l, Norm n, float inv, float inv_lo)
-{
-    const float d = l - n.m;
-    return n.ls == -INFINITY ? -INFINITY : fmaf(d, inv, fmaf(fmaxf(d, LOWEST), inv_lo, -n.ls));
-}
-
-__device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, Norm n)
-{
-    const int64_t y = a.labels[r];
-    return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, n, 1.f, 0.f));
-}
-
-// a row in the backward direction
-struct Back {
-    float m, is, ls, h, ga, ge;                // 1 / s (0 for a row of nothing but -inf), log s, entropy, gradients (ga: times T for the loss)
-    __device__ Back(float2 norm) : m(norm.x), is(norm.y == 0.f ? 0.f : 1.f / norm.y), ls(0.f), h(0.f), ga(0.f), ge(0.f) {}
-    __device__ void set_log_s(float s) { ls = s == 0.f ? 0.f : logf(s); }
-    __device__ float p(float l, float c2) const { return exp2_((l - m) * c2) * is; }
-    __device__ float lp_grad(float l) const
-    {
-        const float d = l - m;
-        return -(exp2_(d * LOG2E) * is) * fmaf(ge, fmaxf(d, -200.f) - ls + h, ga);      // p is 0 from there on, and 0 * inf is not wanted
-    }
-};
-
-// a teacher's entry: 0 = absent, 1 = present, 2 = no such class
-__device__ inline int entry(const RowArgs &a, int64_t c) { return c < 0 ? 0 : (c >= a.K ? 2 : 1); }
-
 // sum / maximum over a wave in the vector pipe (row shifts by 1, 2, 4, 8, then the rows' last lanes broadcast): every lane gets it
 template <int CTRL, int ROWS> __device__ inline float dpp(float old, float v)
 {
@@ -178,12 +115,92 @@ __device__ inline float wave_max(float v)
     return last_lane(v);
 }
 
-__device__ inline void Soft::join_wave(float c2)
+// running sums of a softmax: m in score units (never below LOWEST), s = sum 2^x and, where an entropy is wanted, t = sum x 2^x,
+// x = (l - m) c2
+template <bool ENT> struct Soft {
+    float m, s, t;
+    __device__ void init() { m = LOWEST; s = t = 0.f; }
+    __device__ void raise(float to, float c2)
+    {
+        const float x = (m - to) * c2, f = exp2_(x);
+        if constexpr (ENT) t = f * fmaf(fmaxf(x, -200.f), s, t);          // -200: 2^x is 0 from there on, and 0 * inf is not wanted
+        s *= f;
+        m = to;
+    }
+    __device__ void add(float l, float c2)             // l <= m
+    {
+        const float x = (l - m) * c2, e = exp2_(x);
+        s += e;
+        if constexpr (ENT) t = fmaf(fmaxf(x, -200.f), e, t);
+    }
+    __device__ void join(float m2, float s2, float t2, float c2)
+    {
+        Soft o{m2, s2, t2};
+        const float to = fmaxf(m, m2);
+        raise(to, c2);
+        o.raise(to, c2);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ void join_wave(float c2)
+    {
+        raise(wave_max(m), c2);
+        s = wave_sum(s);
+        if constexpr (ENT) t = wave_sum(t);
+    }
+    __device__ float log_s() const { return s == 0.f ? -INFINITY : logf(s); }      // s = 0: a row of nothing but -inf
+    __device__ float entropy() const { return s == 0.f ? 0.f : logf(s) - LN2 * (t / s); }
+};
+
+// (m, log s) of a row, for the few log probabilities that it reports
+struct Norm { float m, ls; };
+
+// l / T - L, -inf where L is
+__device__ inline float log_p(float l, Norm n, float inv, float inv_lo)
 {
-    raise(wave_max(m), c2);
-    s = wave_sum(s);
-    t = wave_sum(t);
+    const float d = l - n.m;
+    return n.ls == -INFINITY ? -INFINITY : fmaf(d, inv, fmaf(fmaxf(d, LOWEST), inv_lo, -n.ls));
 }
+
+__device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, Norm n)
+{
+    const int64_t y = a.labels[r];
+    return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, n, 1.f, 0.f));
+}
+
+// A row in the backward direction, prepared so that a class costs one exponential and two or three operations:
+//     log probabilities   -p (ga + ge (log p + H)) = 2^x (k1 max(d, -200) + k0),  d = l - m, x = d log2(e)
+//     distillation        ga p = 2^x k0,  x = d log2(e) / T
+// (p is 0 from d = -200 on, and 0 * inf is not wanted; a row of nothing but -inf has 1 / s = 0).
+template <int MODE> struct Back {
+    float m, is, ga, k0, k1, c2;
+    __device__ void scores(float2 norm, float h, float ga_, float ge)
+    {
+        m = norm.x;
+        is = norm.y == 0.f ? 0.f : 1.f / norm.y;
+        ga = ga_;
+        k1 = -is * ge;
+        k0 = -is * (ga + ge * (h - (norm.y == 0.f ? 0.f : logf(norm.y))));
+        c2 = LOG2E;
+    }
+    __device__ void loss(float2 norm, float ga_, float c2_)
+    {
+        m = norm.x;
+        is = norm.y == 0.f ? 0.f : 1.f / norm.y;
+        ga = ga_;
+        k0 = ga * is;
+        c2 = c2_;
+    }
+    __device__ float operator()(float l) const         // without the label's or the teacher's share
+    {
+        const float d = l - m, e = exp2_(d * c2);
+        if constexpr (MODE == LP) return e * fmaf(k1, fmaxf(d, -200.f), k0);
+        else return e * k0;
+    }
+};
+
+// a teacher's entry: 0 = absent, 1 = present, 2 = no such class
+__device__ inline int entry(const RowArgs &a, int64_t c) { return c < 0 ? 0 : (c >= a.K ? 2 : 1); }
 
 // ---------------------------------------------------------------- K <= 1024: a row in the registers of 1 .. 64 lanes --
 struct Group {
@@ -224,8 +241,8 @@ __device__ inline float group_max(float v, const Group &g)
     return v;
 }
 
-// largest kept logit, sum of exponentials of a row's kept logits, and whether an entry names no class; lanes share the entries
-struct Teacher { float m, s; bool any, bad; };
+// A row's kept entries, shared by the lanes of a group: entry i is lane i % lpr's
+struct Teacher { float m, s; bool any, bad; };     // largest kept logit, sum of exponentials; an entry that counts, one that cannot
 __device__ inline Teacher group_teacher(const RowArgs &a, const Group &g)
 {
     Teacher t{-INFINITY, 0.f, false, false};
@@ -246,19 +263,11 @@ __device__ inline Teacher group_teacher(const RowArgs &a, const Group &g)
     t.s = group_sum(t.s, g);
     return t;
 }
-// the part of the loss that one lane's entries of a row give; q log q is 0 at q = 0
-template <typename T> __device__ inline float teacher_loss(const RowArgs &a, const Group &g, const Teacher &t, const T *row, Norm norm)
+// an entry's share of the loss; q log q is 0 at q = 0
+__device__ inline float entry_loss(const RowArgs &a, const Teacher &t, float ls, float kept, float l, Norm norm)
 {
-    float loss = 0.f;
-    if (!t.any) return loss;
-    const float ls = logf(t.s);
-    for (int i = g.sub; i < a.nk; i += g.lpr) {
-        const int64_t c = a.cls[g.at * a.nk + i];
-        if (entry(a, c) != 1) continue;
-        const float x = (a.kept[g.at * a.nk + i] - t.m) * a.c2, q = exp2_(x) / t.s;
-        if (q != 0.f) loss += q * (x * LN2 - ls - log_p(sis3d_f32(row[c * a.s_c]), norm, a.inv, a.inv_lo));
-    }
-    return loss;
+    const float x = (kept - t.m) * a.c2, q = exp2_(x) / t.s;
+    return q != 0.f ? q * (x * LN2 - ls - log_p(l, norm, a.inv, a.inv_lo)) : 0.f;
 }
 
 template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void small_forward(RowArgs a)
@@ -266,7 +275,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     const Group g = group_of(a);
     const T *p = (const T *)a.score + row_at(a, g.at, a.s_n, a.s_v);
     float v[E];
-    Soft so;
+    Soft<MODE == LP> so;
     so.init();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -283,7 +292,15 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
         const Teacher t = group_teacher(a, g);
-        const float loss = a.tau * a.tau * group_sum(g.live ? teacher_loss(a, g, t, p, norm) : 0.f, g);
+        float loss = 0.f;
+        if (t.any && g.live) {
+            const float ls = logf(t.s);
+            for (int i = g.sub; i < a.nk; i += g.lpr) {
+                const int64_t c = a.cls[g.at * a.nk + i];
+                if (entry(a, c) == 1) loss += entry_loss(a, t, ls, a.kept[g.at * a.nk + i], sis3d_f32(p[c * a.s_c]), norm);
+            }
+        }
+        loss = a.tau * a.tau * group_sum(loss, g);
         if (g.sub == 0 && g.in) {
             a.loss[g.r] = !g.live ? 0.f : (t.bad ? NAN : loss);
             a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
@@ -324,37 +341,30 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     float q[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) q[e] = 0.f;
-    Back k(a.norm_in[g.at]);
+    Back<MODE> k;
     if constexpr (MODE == LP) {
         const int64_t y = a.labels[g.at];
-        k.set_log_s(a.norm_in[g.at].y);
-        k.h = a.entropy_in[g.at];
-        k.ga = y < 0 ? 0.f : (y >= a.K ? NAN : a.g1[g.at]);
-        k.ge = a.g2 ? a.g2[g.at] : 0.f;
+        k.scores(a.norm_in[g.at], a.entropy_in[g.at], y < 0 ? 0.f : (y >= a.K ? NAN : a.g1[g.at]), a.g2 ? a.g2[g.at] : 0.f);
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (g.sub + e * g.lpr == y) q[e] = k.ga;
     } else {
         const Teacher t = group_teacher(a, g);
-        k.ga = t.bad ? NAN : (t.any ? a.g1[g.at] * a.tau : 0.f);
+        k.loss(a.norm_in[g.at], t.bad ? NAN : (t.any ? a.g1[g.at] * a.tau : 0.f), a.c2);
         if (t.any)
             for (int i = 0; i < a.nk; ++i) {
                 const int64_t c = a.cls[g.at * a.nk + i];
                 const float w = entry(a, c) == 1 ? exp2_((a.kept[g.at * a.nk + i] - t.m) * a.c2) / t.s : 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    if (g.sub + e * g.lpr == c) q[e] += w;
+                    if (g.sub + e * g.lpr == c) q[e] -= w * k.ga;
             }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int c = g.sub + e * g.lpr;
         if (c >= a.K || !g.in) continue;
-        const float l = sis3d_f32(p[c * a.s_c]);
-        float o;
-        if constexpr (MODE == LP) o = k.lp_grad(l) + q[e];
-        else o = k.ga * (k.p(l, a.c2) - q[e]);
-        d[c * a.d_c] = sis3d_from_f32<T>(g.live ? o : 0.f);
+        d[c * a.d_c] = sis3d_from_f32<T>(g.live ? k(sis3d_f32(p[c * a.s_c])) + q[e] : 0.f);
     }
 }
 
@@ -388,21 +398,40 @@ template <typename T> struct Span {
     __device__ int edges() const { return head + tail; }
 };
 
-// batch<N>(v): a lane's N vectors v, v + NL, ..., all there but perhaps the last.  Whole batches of UL, then one of what is left: without
-// a condition between the loads of a batch, so that they are in flight together.
+// A lane's vectors lane, lane + NL, ... of a span, UL at a time and the next UL on their way while these are worked on; the first are
+// asked for when the object is made, so that a row's other loads travel with them.  f(count, v, vectors): `count` of them from v on, all
+// there but perhaps the last one of the last batch.
 constexpr int UL = 4;
-template <int N> struct Count {};
-template <int NL, typename F> __device__ inline void each_batch(int nvec, int lane, F batch)
-{
-    int v = lane;
-    for (int left = nvec / (UL * NL); left > 0; --left, v += UL * NL) batch(Count<UL>(), v);
-    switch ((nvec - nvec / (UL * NL) * (UL * NL) + NL - 1) / NL) {
-    case 1: batch(Count<1>(), v); break;
-    case 2: batch(Count<2>(), v); break;
-    case 3: batch(Count<3>(), v); break;
-    case 4: batch(Count<4>(), v); break;
+template <int N> struct Count { static constexpr int value = N; };
+template <typename T, int NL> struct Stream {
+    static constexpr int VEC = 16 / sizeof(T);
+    const Span<T> &sp;
+    const int lane;
+    SisVec<T, VEC> raw[UL];
+    __device__ Stream(const Span<T> &s, int l) : sp(s), lane(l) { load(raw, l); }
+    __device__ void load(SisVec<T, VEC> (&r)[UL], int v) const
+    {
+#pragma unroll
+        for (int u = 0; u < UL; ++u) r[u] = sis3d_load_once<T, VEC>(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
     }
-}
+    template <typename F> __device__ void each(F f)
+    {
+        int v = lane, left = (sp.nvec + NL - 1) / NL;          // steps of NL vectors
+        for (; left > UL; left -= UL, v += UL * NL) {
+            SisVec<T, VEC> next[UL];
+            load(next, v + UL * NL);
+            f(Count<UL>(), v, raw);
+#pragma unroll
+            for (int u = 0; u < UL; ++u) raw[u] = next[u];
+        }
+        switch (left) {
+        case 1: f(Count<1>(), v, raw); break;
+        case 2: f(Count<2>(), v, raw); break;
+        case 3: f(Count<3>(), v, raw); break;
+        case 4: f(Count<4>(), v, raw); break;
+        }
+    }
+};
 
 template <typename T, int W, int MODE> struct Long {
     static constexpr int NL = 64 * W, CAP = W == 1 ? 512 : 1024, VEC = 16 / sizeof(T);
@@ -414,17 +443,15 @@ template <typename T, int W, int MODE> struct Long {
     static __device__ int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
 
     // one pass over the span: the team's sums in every lane, and this lane's largest (score, class) among its vectors
-    static __device__ Soft pass(const RowArgs &a, const Span<T> &sp, Shared &sh, uint64_t &best_key)
+    static __device__ Soft<MODE == LP> pass(const RowArgs &a, const Span<T> &sp, Stream<T, NL> &st, Shared &sh, uint64_t &best_key)
     {
-        Soft so;
+        Soft<MODE == LP> so;
         so.init();
         float best = -INFINITY;
         int at = lane();
         const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
-        each_batch<NL>(sp.nvec, lane(), [&]<int N>(Count<N>, int v) {
-            SisVec<T, VEC> raw[N];
-#pragma unroll
-            for (int u = 0; u < N; ++u) raw[u] = *(const SisVec<T, VEC> *)(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
+        st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
+            constexpr int N = decltype(count)::value;
             const bool last = v + (N - 1) * NL < sp.nvec;       // no vector: -inf adds nothing
             float x[N][VEC], top = so.m;
 #pragma unroll
@@ -456,7 +483,7 @@ template <typename T, int W, int MODE> struct Long {
                 sh.red[threadIdx.x >> 6][2] = so.t;
             }
             __syncthreads();
-            so = Soft{sh.red[0][0], sh.red[0][1], sh.red[0][2]};
+            so = Soft<MODE == LP>{sh.red[0][0], sh.red[0][1], sh.red[0][2]};
 #pragma unroll
             for (int w = 1; w < W; ++w) so.join(sh.red[w][0], sh.red[w][1], sh.red[w][2], a.c2);
         }
@@ -539,31 +566,62 @@ template <typename T, int W, int MODE> struct Long {
     }
 };
 
-// a wave as the lanes of one row
-__device__ inline Group wave_group(int64_t r)
-{
-    Group g;
-    g.r = g.at = r;
-    g.sub = threadIdx.x & 63;
-    g.lpr = 64;
-    g.step = 1;
-    g.in = g.live = true;
-    return g;
-}
+// A row's kept entries in the lanes of a wave, at most two a lane: asked for before the row is read, used behind it
+struct Kept {
+    float x[2], l[2];                          // teacher's logit, student's score; -inf: no such entry
+    int c[2];                                  // class, -1: none
+    bool bad;
+    template <typename T> __device__ Kept(const RowArgs &a, int64_t r, const T *row, bool on = true) : bad(false)
+    {
+        const int nk = on ? a.nk : 0;
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = lane + 64 * j;
+            x[j] = -INFINITY;
+            l[j] = 0.f;
+            c[j] = -1;
+            if (j * 64 >= nk) break;
+            if (i >= nk) continue;
+            const int64_t k = a.cls[r * a.nk + i];
+            const float v = a.kept[r * a.nk + i];
+            if (k < 0) continue;
+            x[j] = v;
+            if (k >= a.K || v != v) { bad = true; continue; }
+            c[j] = (int)k;
+            l[j] = sis3d_f32(row[k]);
+        }
+    }
+    __device__ Teacher teacher(const RowArgs &a) const
+    {
+        Teacher t;
+        t.m = wave_max(fmaxf(x[0], x[1]));
+        t.bad = __any(bad);
+        t.any = t.m > -INFINITY;
+        t.s = t.any ? wave_sum(exp2_((x[0] - t.m) * a.c2) + exp2_((x[1] - t.m) * a.c2)) : 0.f;
+        return t;
+    }
+};
 
-template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t r, const T *row, const Soft &so)
+template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t r, const Kept &kept, const Soft<false> &so)
 {
     const Norm norm{so.m, so.log_s()};
-    const Group g = wave_group(r);
-    const Teacher t = group_teacher(a, g);
-    const float loss = a.tau * a.tau * group_sum(teacher_loss(a, g, t, row, norm), g);
-    if (g.sub == 0) {
+    const Teacher t = kept.teacher(a);
+    float loss = 0.f;
+    if (t.any) {
+        const float ls = logf(t.s);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (kept.c[j] >= 0) loss += entry_loss(a, t, ls, kept.x[j], kept.l[j], norm);
+    }
+    loss = a.tau * a.tau * wave_sum(loss);
+    if ((threadIdx.x & 63) == 0) {
         a.loss[r] = t.bad ? NAN : loss;
         a.norm[r] = make_float2(so.m, so.s);
     }
 }
 
-template <typename T> __device__ inline void row_outputs(const RowArgs &a, int64_t r, const T *row, const Soft &so, Norm norm)
+template <typename T> __device__ inline void row_outputs(const RowArgs &a, int64_t r, const T *row, const Soft<true> &so, Norm norm)
 {
     const int64_t y = a.labels[r];
     a.logp[r] = label_logp(a, r, y >= 0 && y < a.K ? sis3d_f32(row[y]) : 0.f, norm);
@@ -596,12 +654,16 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     if (r >= live_rows(a)) { zero_row<MODE>(a, r, L::lane(), L::NL); return; }
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     const Span<T> sp(row, 0, a.K);
+    Stream<T, L::NL> st(sp, L::lane());
     uint64_t best;
-    const Soft so = L::pass(a, sp, sh, best);
-    const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
-        if (W == 1 || threadIdx.x < 64) wave_loss(a, r, row, so);
+        const bool first = W == 1 || threadIdx.x < 64;
+        const Kept kept(a, r, row, first);
+        const auto so = L::pass(a, sp, st, sh, best);
+        if (first) wave_loss<T>(a, r, kept, so);
     } else {
+        const auto so = L::pass(a, sp, st, sh, best);
+        const Norm norm{so.m, so.log_s()};
         if (L::lane() == 0) row_outputs(a, r, row, so, norm);
         if (a.top)
             L::alternatives(a, sp, sh, best, [&](int rank, uint64_t k) {
@@ -622,8 +684,9 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void split_for
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
     const Span<T> sp(row, k0, k1);
+    Stream<T, L::NL> st(sp, L::lane());
     uint64_t best;
-    const Soft so = L::pass(a, sp, sh, best);
+    const auto so = L::pass(a, sp, st, sh, best);
     if (threadIdx.x == 0) *(float4 *)(a.part + (size_t)blockIdx.x * 4) = make_float4(so.m, so.s, so.t, 0.f);
     if constexpr (MODE == LP)
         if (a.top) L::alternatives(a, sp, sh, best, [&](int rank, uint64_t k) { a.part_keys[(size_t)blockIdx.x * a.top + rank] = k; });
@@ -638,16 +701,16 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join
     const int lane = threadIdx.x;
     if (r >= live_rows(a)) { zero_row<MODE>(a, r, lane, 64); return; }
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
-    Soft so;
+    Soft<MODE == LP> so;
     so.init();
     if (lane < a.parts) {
         const float4 v = *(const float4 *)(a.part + ((size_t)r * a.parts + lane) * 4);
-        so = Soft{v.x, v.y, v.z};
+        so = Soft<MODE == LP>{v.x, v.y, v.z};
     }
     so.join_wave(a.c2);
     const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
-        wave_loss(a, r, row, so);
+        wave_loss<T>(a, r, Kept(a, r, row), so);
     } else {
         if (lane == 0) row_outputs(a, r, row, so, norm);
         if (!a.top) return;
@@ -679,7 +742,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     __shared__ float q_s[4 / W][KEPT_MAX];
     __shared__ int c_s[4 / W][KEPT_MAX];
     const int team = W == 1 ? threadIdx.x >> 6 : 0, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int64_t item = W == 1 ? (int64_t)blockIdx.x * 4 + team : blockIdx.x, r = item / a.parts;
+    const int64_t item = W == 1 ? (int64_t)blockIdx.x * 4 + team : blockIdx.x, r = a.parts == 1 ? item : item / a.parts;
     if (r >= a.R) return;
     const int part = (int)(item - r * a.parts);
     const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
@@ -689,43 +752,35 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
         for (int c = k0 + lane; c < k1; c += NL) out[c] = sis3d_from_f32<T>(0.f);
         return;
     }
-    Back k(a.norm_in[r]);
+    const Span<T> sp(row, k0, k1);
+    Stream<T, NL> st(sp, lane);
+    const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : 0.f;
+    Back<MODE> k;
     int y = -1;
     if constexpr (MODE == LP) {
         const int64_t label = a.labels[r];
-        k.set_log_s(a.norm_in[r].y);
-        k.h = a.entropy_in[r];
-        k.ga = label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[r]);
-        k.ge = a.g2 ? a.g2[r] : 0.f;
-        y = label >= 0 && label < a.K ? (int)label : -1;
+        k.scores(a.norm_in[r], a.entropy_in[r], label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[r]), a.g2 ? a.g2[r] : 0.f);
+        y = label >= k0 && label < k1 ? (int)label : -1;
     } else {
-        const Teacher t = group_teacher(a, wave_group(r));
+        const Kept kept(a, r, row);
+        const Teacher t = kept.teacher(a);
+        k.loss(a.norm_in[r], t.bad ? NAN : (t.any ? a.g1[r] * a.tau : 0.f), a.c2);
         if (W == 1 || threadIdx.x < 64)
-            for (int i = lane; i < a.nk; i += 64) {
-                const int64_t c = a.cls[r * a.nk + i];
-                const bool on = t.any && entry(a, c) == 1;
-                c_s[team][i] = on ? (int)c : -1;
-                q_s[team][i] = on ? exp2_((a.kept[r * a.nk + i] - t.m) * a.c2) / t.s : 0.f;
-            }
-        k.ga = t.bad ? NAN : (t.any ? a.g1[r] * a.tau : 0.f);
-    }
-    const Span<T> sp(row, k0, k1);
-    const float gs = k.ga * k.is;
-    auto grad = [&](float l, int c) {
-        if constexpr (MODE == LP) return k.lp_grad(l) + (c == y ? k.ga : 0.f);
-        else return gs * exp2_((l - k.m) * a.c2);
-    };
-    const bool wide = ((uintptr_t)(out + k0 + sp.head) & 15) == 0;
-    each_batch<NL>(sp.nvec, lane, [&]<int N>(Count<N>, int v) {
-        SisVec<T, VEC> raw[N];
 #pragma unroll
-        for (int u = 0; u < N; ++u) raw[u] = *(const SisVec<T, VEC> *)(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
+            for (int j = 0; j < 2; ++j) {
+                c_s[team][lane + 64 * j] = kept.c[j];
+                q_s[team][lane + 64 * j] = t.any ? exp2_((kept.x[j] - t.m) * a.c2) / t.s : 0.f;
+            }
+    }
+    const bool wide = ((uintptr_t)(out + k0 + sp.head) & 15) == 0;
+    st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
+        constexpr int N = decltype(count)::value;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int c = sp.first_class(v + u * NL);
             float x[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[i] = grad(sis3d_f32(raw[u].v[i]), c + i);
+            for (int i = 0; i < VEC; ++i) x[i] = k(sis3d_f32(raw[u].v[i]));
             if (u == N - 1 && v + u * NL >= sp.nvec) continue;
             if (wide) sis3d_store<T, VEC>(out + c, x);
             else {
@@ -734,14 +789,13 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
             }
         }
     });
-    if (lane < sp.edges()) {
-        const int c = sp.edge_class(lane);
-        out[c] = sis3d_from_f32<T>(grad(sis3d_f32(row[c]), c));
-    }
-    if constexpr (MODE == KD) {
-        // the kept classes of this part again, with the teacher's share: written behind the team's own stores.  A class that is kept
-        // twice is written by its first entry with the sum of both.
-        team_sync<W>();
+    if (lane < sp.edges()) out[sp.edge_class(lane)] = sis3d_from_f32<T>(k(edge));
+    // The label's class, or the kept classes of this part, again with their share: written behind the team's own stores.  A class that
+    // is kept twice is written by its first entry with the sum of both.
+    team_sync<W>();
+    if constexpr (MODE == LP) {
+        if (lane == 0 && y >= 0) out[y] = sis3d_from_f32<T>(k(sis3d_f32(row[y])) + k.ga);
+    } else {
         for (int i = lane; i < a.nk; i += NL) {
             const int c = c_s[team][i];
             if (c < k0 || c >= k1) continue;
@@ -752,7 +806,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
                     q += q_s[team][j];
                     first = first && j >= i;
                 }
-            if (first) out[c] = sis3d_from_f32<T>(k.ga * (k.p(sis3d_f32(row[c]), a.c2) - q));
+            if (first) out[c] = sis3d_from_f32<T>(k(sis3d_f32(row[c])) - k.ga * q);
         }
     }
 }

