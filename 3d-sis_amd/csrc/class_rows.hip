@@ -19,9 +19,9 @@
 //   longer rows      a wave (K <= 4096) or a workgroup streams a row with 16-byte loads from its first aligned element on
 //   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
 //
-// Alternatives of a long row without sorting it: every lane knows the largest (score, class) of its own vectors.  The lanes are put
-// into >= k groups; the smallest of the group maxima is a bound that at least k elements reach, so only lanes whose maximum
-// reaches it are read again (from cache) and their elements at or above it -- k log k of them or so -- are ranked by counting.
+// Alternatives of a long row without sorting it: every lane knows the largest score of its own vectors.  The lanes are put into >= k
+// groups; the smallest of the group maxima is a bound that at least k elements reach, so only lanes whose maximum reaches it are read
+// again (from cache) and their elements at or above it -- k log k of them or so -- are ranked by counting, by (score, class).
 #include "elem.h"
 
 namespace {
@@ -113,6 +113,17 @@ __device__ inline float wave_max(float v)
     v = fmaxf(v, dpp<0x142, 0xa>(v, v));
     v = fmaxf(v, dpp<0x143, 0xc>(v, v));
     return last_lane(v);
+}
+
+__device__ inline float wave_min(float v) { return -wave_max(-v); }
+// the largest of the 2, 4, 8 or 16 neighbouring lanes that v's lane is one of: quads by permutation, then mirrored halves and rows
+__device__ inline float lanes_max(float v, int lanes)
+{
+    v = fmaxf(v, dpp<0xb1, 0xf>(v, v));
+    if (lanes >= 4) v = fmaxf(v, dpp<0x4e, 0xf>(v, v));
+    if (lanes >= 8) v = fmaxf(v, dpp<0x141, 0xf>(v, v));
+    if (lanes >= 16) v = fmaxf(v, dpp<0x140, 0xf>(v, v));
+    return v;
 }
 
 // running sums of a softmax: m in score units (never below LOWEST), s = sum 2^x and, where an entropy is wanted, t = sum x 2^x,
@@ -370,6 +381,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
 
 // ---------------------------------------------------------------------------- long rows, classes contiguous --
 // A team of W waves (1: four teams to a workgroup; 4: the workgroup) has a row or a part of one.
+template <int W> __device__ inline int team_of() { return W == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0; }
 template <int W> __device__ inline void team_sync()
 {
     if constexpr (W == 1) {
@@ -443,12 +455,12 @@ template <typename T, int W, int MODE> struct Long {
     static __device__ int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
 
     // one pass over the span: the team's sums in every lane, and this lane's largest (score, class) among its vectors
-    static __device__ Soft<MODE == LP> pass(const RowArgs &a, const Span<T> &sp, Stream<T, NL> &st, Shared &sh, uint64_t &best_key)
+    static __device__ Soft<MODE == LP> pass(const RowArgs &a, const Span<T> &sp, Stream<T, NL> &st, Shared &sh, float &best, int &at)
     {
         Soft<MODE == LP> so;
         so.init();
-        float best = -INFINITY;
-        int at = lane();
+        best = -INFINITY;
+        at = lane();
         const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
         st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
             constexpr int N = decltype(count)::value;
@@ -471,8 +483,6 @@ template <typename T, int W, int MODE> struct Long {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) so.add(x[u][i], a.c2);
         });
-        // the key of a vector: its last class stands for the place of its maximum, vectors being disjoint ranges of classes
-        best_key = lane() < sp.nvec ? key_of(best, sp.first_class(at) + VEC - 1) : 0;
         so.raise(fmaxf(so.m, edge), a.c2);
         if (lane() < sp.edges()) so.add(edge, a.c2);
         so.join_wave(a.c2);
@@ -490,33 +500,20 @@ template <typename T, int W, int MODE> struct Long {
         return so;
     }
 
-    // the `top` largest keys of the span, out(rank, key) once for each rank that exists
-    template <typename F> static __device__ void alternatives(const RowArgs &a, const Span<T> &sp, Shared &sh, uint64_t best_key, F out)
+    // Elements of the span that pass `keep(score, class)`, from the lanes whose `again` says that they have one and from the edges: into
+    // sh.cand, at most CAP of them, and their number as the answer
+    template <typename F> static __device__ int collect(const Span<T> &sp, Shared &sh, bool again, F keep)
     {
-        const int n = sp.nvec * VEC + sp.edges(), want = a.top < n ? a.top : n;
-        int groups = 1;
-        while (groups < want) groups *= 2;
-        // a bound that at least `want` elements of this wave's vectors reach; 0 where a group has no vector
-        uint64_t b = best_key;
-        for (int o = 32; o >= groups; o >>= 1) b = max64(b, shfl_xor64(b, o));
-        for (int o = groups >> 1; o > 0; o >>= 1) b = min64(b, shfl_xor64(b, o));
-        if (lane() == 0) sh.count = 0;
-        if constexpr (W > 1) {
-            if ((threadIdx.x & 63) == 0) sh.bound[threadIdx.x >> 6] = b;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < W; ++w) b = max64(b, sh.bound[w]);
-        } else team_sync<W>();
-        // lanes of this wave that have to be read again
         const int w = W == 1 ? 0 : threadIdx.x >> 6, ln = threadIdx.x & 63;
-        const bool again = best_key != 0 && best_key >= b;
+        team_sync<W>();
+        if (lane() == 0) sh.count = 0;
         const uint64_t mask = __ballot(again);
         if (again) sh.lanes[w][__popcll(mask & ((1ull << ln) - 1))] = ln;
         team_sync<W>();
-        auto offer = [&](uint64_t k) {
-            if (k >= b) {
+        auto offer = [&](float v, int c) {
+            if (keep(v, c)) {
                 const int i = atomicAdd(&sh.count, 1);
-                if (i < CAP) sh.cand[i] = k;
+                if (i < CAP) sh.cand[i] = key_of(v, c);
             }
         };
         const int per = (sp.nvec + NL - 1) / NL, items = __popcll(mask) * per;
@@ -526,14 +523,58 @@ template <typename T, int W, int MODE> struct Long {
             float x[VEC];
             sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) offer(key_of(x[e], sp.first_class(v) + e));
+            for (int e = 0; e < VEC; ++e) offer(x[e], sp.first_class(v) + e);
         }
         if (lane() < sp.edges()) {
             const int c = sp.edge_class(lane());
-            offer(key_of(sis3d_f32(sp.row[c]), c));
+            offer(sis3d_f32(sp.row[c]), c);
         }
         team_sync<W>();
-        const int m = sh.count;
+        return sh.count;
+    }
+
+    // The `top` largest keys of the span, out(rank, key) once for each rank.  best, at: this lane's largest score among its vectors, and
+    // the first vector that has it.
+    template <typename F> static __device__ void alternatives(const RowArgs &a, const Span<T> &sp, Shared &sh, float best, int at, F out)
+    {
+        const int want = a.top, w = W == 1 ? 0 : threadIdx.x >> 6, ln = threadIdx.x & 63;       // a span has far more classes
+        // the smallest of the maxima of >= want groups of lanes: at least want elements of this wave reach it
+        float b = wave_min(lanes_max(best, want > 16 ? 2 : want > 8 ? 4 : want > 4 ? 8 : 16));
+        if constexpr (W > 1) {
+            if (ln == 0) sh.red[w][0] = b;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < W; ++i) b = fmaxf(b, sh.red[i][0]);
+        }
+        int m = collect(sp, sh, best >= b && best > -INFINITY, [&](float v, int) { return v >= b && v > -INFINITY; });
+        if (m < want) {                                    // -inf (and NaN, which counts as that) from the lowest class on: 64 hold enough
+            const int c = sp.k0 + ln;
+            const float v = sis3d_f32(sp.row[c]);
+            const bool none = !(v > -INFINITY);
+            const uint64_t mask = __ballot(none);
+            const int i = m + __popcll(mask & ((1ull << ln) - 1));
+            team_sync<W>();
+            if (none && i < want && w == 0) sh.cand[i] = key_of(v, c);
+            team_sync<W>();
+            m = want;
+        }
+        if (m > CAP) {
+            // Many equal scores at the bound: a bound on (score, class).  A vector's last class stands for the place of its maximum,
+            // vectors being disjoint ranges of classes.
+            int groups = 1;
+            while (groups < want) groups *= 2;
+            const uint64_t mine = lane() < sp.nvec ? key_of(best, sp.first_class(at) + VEC - 1) : 0;
+            uint64_t k = mine;
+            for (int o = 32; o >= groups; o >>= 1) k = max64(k, shfl_xor64(k, o));
+            for (int o = groups >> 1; o > 0; o >>= 1) k = min64(k, shfl_xor64(k, o));
+            if constexpr (W > 1) {
+                if (ln == 0) sh.bound[w] = k;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < W; ++i) k = max64(k, sh.bound[i]);
+            }
+            m = collect(sp, sh, mine != 0 && mine >= k, [&](float v, int c) { return key_of(v, c) >= k; });
+        }
         if (m <= CAP) {
             for (int i = lane(); i < m; i += NL) {
                 const uint64_t k = sh.cand[i];
@@ -541,10 +582,10 @@ template <typename T, int W, int MODE> struct Long {
                 for (int j = 0; j < m; ++j) rank += sh.cand[j] > k;
                 if (rank < want) out(rank, k);
             }
-            team_sync<W>();
             return;
         }
-        // more elements at the bound than there is room for (rows made for it): the largest below the last one, `want` times
+        // rows made to have more elements at the bound than there is room for: the largest below the last one, `want` times
+        const int n = sp.nvec * VEC + sp.edges();
         uint64_t last = ~0ull;
         for (int r = 0; r < want; ++r) {
             uint64_t k = 0;
@@ -562,7 +603,6 @@ template <typename T, int W, int MODE> struct Long {
             if (lane() == 0) out(r, k);
             last = k;
         }
-        team_sync<W>();
     }
 };
 
@@ -648,25 +688,26 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
 {
     using L = Long<T, W, MODE>;
     __shared__ typename L::Shared shared[4 / W];
-    auto &sh = shared[W == 1 ? threadIdx.x >> 6 : 0];
-    const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    auto &sh = shared[team_of<W>()];
+    const int64_t r = (int64_t)blockIdx.x * (4 / W) + team_of<W>();
     if (r >= a.R) return;                                  // the whole team
     if (r >= live_rows(a)) { zero_row<MODE>(a, r, L::lane(), L::NL); return; }
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     const Span<T> sp(row, 0, a.K);
     Stream<T, L::NL> st(sp, L::lane());
-    uint64_t best;
+    float best;
+    int at;
     if constexpr (MODE == KD) {
         const bool first = W == 1 || threadIdx.x < 64;
         const Kept kept(a, r, row, first);
-        const auto so = L::pass(a, sp, st, sh, best);
+        const auto so = L::pass(a, sp, st, sh, best, at);
         if (first) wave_loss<T>(a, r, kept, so);
     } else {
-        const auto so = L::pass(a, sp, st, sh, best);
+        const auto so = L::pass(a, sp, st, sh, best, at);
         const Norm norm{so.m, so.log_s()};
         if (L::lane() == 0) row_outputs(a, r, row, so, norm);
         if (a.top)
-            L::alternatives(a, sp, sh, best, [&](int rank, uint64_t k) {
+            L::alternatives(a, sp, sh, best, at, [&](int rank, uint64_t k) {
                 a.top_class[r * a.top + rank] = key_class(k);
                 a.top_logp[r * a.top + rank] = log_p(key_score(k), norm, 1.f, 0.f);
             });
@@ -685,11 +726,12 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void split_for
     const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
     const Span<T> sp(row, k0, k1);
     Stream<T, L::NL> st(sp, L::lane());
-    uint64_t best;
-    const auto so = L::pass(a, sp, st, sh, best);
+    float best;
+    int at;
+    const auto so = L::pass(a, sp, st, sh, best, at);
     if (threadIdx.x == 0) *(float4 *)(a.part + (size_t)blockIdx.x * 4) = make_float4(so.m, so.s, so.t, 0.f);
     if constexpr (MODE == LP)
-        if (a.top) L::alternatives(a, sp, sh, best, [&](int rank, uint64_t k) { a.part_keys[(size_t)blockIdx.x * a.top + rank] = k; });
+        if (a.top) L::alternatives(a, sp, sh, best, at, [&](int rank, uint64_t k) { a.part_keys[(size_t)blockIdx.x * a.top + rank] = k; });
 }
 
 // joins the parts of a row: one wave
@@ -741,11 +783,15 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     constexpr int NL = 64 * W, VEC = 16 / sizeof(T);
     __shared__ float q_s[4 / W][KEPT_MAX];
     __shared__ int c_s[4 / W][KEPT_MAX];
-    const int team = W == 1 ? threadIdx.x >> 6 : 0, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int64_t item = W == 1 ? (int64_t)blockIdx.x * 4 + team : blockIdx.x, r = a.parts == 1 ? item : item / a.parts;
+    const int team = team_of<W>(), lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t item = (int64_t)blockIdx.x * (4 / W) + team, r = a.parts == 1 ? item : item / a.parts;
     if (r >= a.R) return;
-    const int part = (int)(item - r * a.parts);
-    const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
+    int k0 = 0, k1 = a.K;
+    if (a.parts > 1) {
+        const int part = (int)(item - r * a.parts);
+        k0 = (int)((int64_t)a.K * part / a.parts);
+        k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
+    }
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     T *out = (T *)a.dscore + row_at(a, r, a.d_n, a.d_v);
     if (r >= live_rows(a)) {
