@@ -69,6 +69,14 @@ __device__ inline int64_t row_at(const RowArgs &a, int64_t r, int64_t sn, int64_
 }
 
 __device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float log_(float x) { return LN2 * __builtin_amdgcn_logf(x); }        // of sums: normal numbers
+// a product that is rounded by itself and not fused with what is done with it
+__device__ inline float mul_rounded(float a, float b)
+{
+#pragma clang fp contract(off)
+    return a * b;
+}
+__device__ inline float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // (score, class) as one number: larger score first, then the lower class; -0 counts as 0, NaN as -inf
 __device__ inline uint64_t key_of(float v, int c)
@@ -88,7 +96,23 @@ __device__ inline uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__sh
 __device__ inline uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ inline uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-// sum / maximum over a wave in the vector pipe (row shifts by 1, 2, 4, 8, then the rows' last lanes broadcast): every lane gets it
+// maximum of three in one instruction.  Written out because the compiler puts a canonicalising instruction in front of every operand that
+// it has only seen as bits; what that guards against (a signalling NaN) would at worst cost a NaN row the order of its alternatives.
+__device__ inline float max3_(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+template <int N> __device__ inline float max_of(const float (&x)[N])
+{
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2) m = max3_(m, x[i], x[i + 1]);
+    return N % 2 ? m : fmaxf(m, x[N - 1]);
+}
+
+// sum over a wave in the vector pipe (row shifts by 1, 2, 4, 8, then the rows' last lanes broadcast): every lane gets it
 template <int CTRL, int ROWS> __device__ inline float dpp(float old, float v)
 {
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
@@ -104,17 +128,20 @@ __device__ inline float wave_sum(float v)
     v += dpp<0x143, 0xc>(0.f, v);
     return last_lane(v);
 }
+// one step of a maximum over the 16 lanes of a row, rotated by N: every lane takes part, so one instruction does it (written out for the
+// reason given at max3_; the waits are those between a vector result and its use across lanes)
+template <int N> __device__ inline float max_ror(float v)
+{
+    float r;
+    asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:%2 row_mask:0xf bank_mask:0xf\n\ts_nop 1" : "=v"(r) : "v"(v), "n"(N));
+    return r;
+}
+__device__ inline float lane_at(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
 __device__ inline float wave_max(float v)
 {
-    v = fmaxf(v, dpp<0x111, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x112, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x114, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x118, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x142, 0xa>(v, v));
-    v = fmaxf(v, dpp<0x143, 0xc>(v, v));
-    return last_lane(v);
+    v = max_ror<8>(max_ror<4>(max_ror<2>(max_ror<1>(v))));
+    return max3_(lane_at(v, 0), lane_at(v, 16), fmaxf(lane_at(v, 32), lane_at(v, 48)));
 }
-
 __device__ inline float wave_min(float v) { return -wave_max(-v); }
 // the largest of the 2, 4, 8 or 16 neighbouring lanes that v's lane is one of: quads by permutation, then mirrored halves and rows
 __device__ inline float lanes_max(float v, int lanes)
@@ -159,8 +186,44 @@ template <bool ENT> struct Soft {
         s = wave_sum(s);
         if constexpr (ENT) t = wave_sum(t);
     }
-    __device__ float log_s() const { return s == 0.f ? -INFINITY : logf(s); }      // s = 0: a row of nothing but -inf
-    __device__ float entropy() const { return s == 0.f ? 0.f : logf(s) - LN2 * (t / s); }
+    __device__ float log_s() const { return s == 0.f ? -INFINITY : log_(s); }      // s = 0: a row of nothing but -inf
+    __device__ float entropy() const { return s == 0.f ? 0.f : log_(s) - LN2 * (t / s); }
+};
+
+// The same sums for one lane of a long row, x = l c2 - M in one fused operation (its rounding is that of x; one of M would be common to all
+// classes and cancels).  M, in units of x, need only be near the largest: it follows it when it is exceeded by more than 2.  Scores
+// whose product with c2 leaves the range of a float end in sums of 0, inf or NaN: such rows are taken again by exact_row.
+template <bool ENT> struct Lane {
+    float M, s, t;
+    __device__ void init() { M = -3e38f; s = t = 0.f; }
+    __device__ void raise(float to)
+    {
+        const float x = M - to, f = exp2_(x);
+        if constexpr (ENT) t = f * fmaf(fmaxf(x, -200.f), s, t);
+        s *= f;
+        M = to;
+    }
+    __device__ void follow(float top, float c2)
+    {
+        const float to = mul_rounded(top, c2);
+        if (to > M + 2.f) raise(to);
+    }
+    __device__ void add(float l, float c2)
+    {
+        const float x = fmaf(l, c2, -M), e = exp2_(x);
+        s += e;
+        if constexpr (ENT) t = fmaf(fmaxf(x, -200.f), e, t);
+    }
+    // all lanes of a wave, relative to its largest score m: divided by m's own term, so that a row of one class has s = 1 exactly
+    __device__ Soft<ENT> join_wave(float largest, float c2)
+    {
+        const float m = fmaxf(wave_max(largest), LOWEST);
+        raise(mul_rounded(m, c2));
+        s = wave_sum(s);
+        if constexpr (ENT) t = wave_sum(t);
+        const float x = fmaf(m, c2, -M), e = exp2_(x);
+        return Soft<ENT>{m, s / e, ENT ? fmaf(-x, s, t) / e : 0.f};
+    }
 };
 
 // (m, log s) of a row, for the few log probabilities that it reports
@@ -179,34 +242,52 @@ __device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, Norm n
     return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, n, 1.f, 0.f));
 }
 
-// A row in the backward direction, prepared so that a class costs one exponential and two or three operations:
-//     log probabilities   -p (ga + ge (log p + H)) = 2^x (k1 max(d, -200) + k0),  d = l - m, x = d log2(e)
-//     distillation        ga p = 2^x k0,  x = d log2(e) / T
-// (p is 0 from d = -200 on, and 0 * inf is not wanted; a row of nothing but -inf has 1 / s = 0).
+// A row in the backward direction, prepared so that a class costs one exponential and a few operations:
+//     log probabilities   -p (ga + ge (log p + H)) = 2^x (k1 max(x, -288) + k0),  x = (l - m) log2(e)
+//     distillation        ga p = 2^x k0,  x = (l - m) log2(e) / T
+// (p is 0 from x = -288 on, and 0 * inf is not wanted; a row of nothing but -inf has 1 / s = 0).  `near` takes x from one fused operation
+// with M = m c2 rounded, whose rounding is taken out of k0 and k1 beforehand; `exact` serves rows whose m c2 leaves the range.
 template <int MODE> struct Back {
-    float m, is, ga, k0, k1, c2;
+    float m, ga, k0, k1, c2, M, n0, n1;
+    bool in_range;
+    __device__ void finish()
+    {
+        M = mul_rounded(m, c2);
+        in_range = fabsf(M) < 1e37f;
+        const float off = fmaf(m, c2, -M), f = exp2_(-off);        // l c2 - M = x + off
+        n1 = MODE == LP ? k1 * f : 0.f;
+        n0 = MODE == LP ? f * fmaf(-k1, off, k0) : f * k0;
+    }
     __device__ void scores(float2 norm, float h, float ga_, float ge)
     {
+        const float is = norm.y == 0.f ? 0.f : 1.f / norm.y;
         m = norm.x;
-        is = norm.y == 0.f ? 0.f : 1.f / norm.y;
         ga = ga_;
-        k1 = -is * ge;
-        k0 = -is * (ga + ge * (h - (norm.y == 0.f ? 0.f : logf(norm.y))));
+        k1 = -is * ge * LN2;
+        k0 = -is * (ga + ge * (h - (norm.y == 0.f ? 0.f : log_(norm.y))));
         c2 = LOG2E;
+        finish();
     }
     __device__ void loss(float2 norm, float ga_, float c2_)
     {
         m = norm.x;
-        is = norm.y == 0.f ? 0.f : 1.f / norm.y;
         ga = ga_;
-        k0 = ga * is;
+        k0 = norm.y == 0.f ? 0.f : ga / norm.y;
         c2 = c2_;
+        finish();
     }
-    __device__ float operator()(float l) const         // without the label's or the teacher's share
+    // without the label's or the teacher's share
+    __device__ float exact(float l) const
     {
-        const float d = l - m, e = exp2_(d * c2);
-        if constexpr (MODE == LP) return e * fmaf(k1, fmaxf(d, -200.f), k0);
+        const float x = (l - m) * c2, e = exp2_(x);
+        if constexpr (MODE == LP) return e * fmaf(k1, fmaxf(x, -288.f), k0);
         else return e * k0;
+    }
+    __device__ float near(float l) const
+    {
+        const float x = fmaf(l, c2, -M), e = exp2_(x);
+        if constexpr (MODE == LP) return e * fmaf(n1, fmaxf(x, -288.f), n0);
+        else return e * n0;
     }
 };
 
@@ -277,7 +358,7 @@ __device__ inline Teacher group_teacher(const RowArgs &a, const Group &g)
 // an entry's share of the loss; q log q is 0 at q = 0
 __device__ inline float entry_loss(const RowArgs &a, const Teacher &t, float ls, float kept, float l, Norm norm)
 {
-    const float x = (kept - t.m) * a.c2, q = exp2_(x) / t.s;
+    const float x = (kept - t.m) * a.c2, q = exp2_(x) * rcp_(t.s);
     return q != 0.f ? q * (x * LN2 - ls - log_p(l, norm, a.inv, a.inv_lo)) : 0.f;
 }
 
@@ -305,7 +386,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
         const Teacher t = group_teacher(a, g);
         float loss = 0.f;
         if (t.any && g.live) {
-            const float ls = logf(t.s);
+            const float ls = log_(t.s);
             for (int i = g.sub; i < a.nk; i += g.lpr) {
                 const int64_t c = a.cls[g.at * a.nk + i];
                 if (entry(a, c) == 1) loss += entry_loss(a, t, ls, a.kept[g.at * a.nk + i], sis3d_f32(p[c * a.s_c]), norm);
@@ -365,7 +446,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
         if (t.any)
             for (int i = 0; i < a.nk; ++i) {
                 const int64_t c = a.cls[g.at * a.nk + i];
-                const float w = entry(a, c) == 1 ? exp2_((a.kept[g.at * a.nk + i] - t.m) * a.c2) / t.s : 0.f;
+                const float w = entry(a, c) == 1 ? exp2_((a.kept[g.at * a.nk + i] - t.m) * a.c2) * rcp_(t.s) : 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     if (g.sub + e * g.lpr == c) q[e] -= w * k.ga;
@@ -375,7 +456,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     for (int e = 0; e < E; ++e) {
         const int c = g.sub + e * g.lpr;
         if (c >= a.K || !g.in) continue;
-        d[c * a.d_c] = sis3d_from_f32<T>(g.live ? k(sis3d_f32(p[c * a.s_c])) + q[e] : 0.f);
+        d[c * a.d_c] = sis3d_from_f32<T>(g.live ? k.exact(sis3d_f32(p[c * a.s_c])) + q[e] : 0.f);
     }
 }
 
@@ -429,18 +510,25 @@ template <typename T, int NL> struct Stream {
     template <typename F> __device__ void each(F f)
     {
         int v = lane, left = (sp.nvec + NL - 1) / NL;          // steps of NL vectors
-        for (; left > UL; left -= UL, v += UL * NL) {
-            SisVec<T, VEC> next[UL];
+        SisVec<T, VEC> next[UL];
+        while (left > UL) {
             load(next, v + UL * NL);
             f(Count<UL>(), v, raw);
-#pragma unroll
-            for (int u = 0; u < UL; ++u) raw[u] = next[u];
+            left -= UL, v += UL * NL;
+            if (left <= UL) { last(left, v, next, f); return; }
+            load(raw, v + UL * NL);
+            f(Count<UL>(), v, next);
+            left -= UL, v += UL * NL;
         }
+        last(left, v, raw, f);
+    }
+    template <typename F> __device__ void last(int left, int v, const SisVec<T, VEC> (&r)[UL], F f)
+    {
         switch (left) {
-        case 1: f(Count<1>(), v, raw); break;
-        case 2: f(Count<2>(), v, raw); break;
-        case 3: f(Count<3>(), v, raw); break;
-        case 4: f(Count<4>(), v, raw); break;
+        case 1: f(Count<1>(), v, r); break;
+        case 2: f(Count<2>(), v, r); break;
+        case 3: f(Count<3>(), v, r); break;
+        case 4: f(Count<4>(), v, r); break;
         }
     }
 };
@@ -454,38 +542,79 @@ template <typename T, int W, int MODE> struct Long {
     };
     static __device__ int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
 
+    static __device__ float team_max(float v, Shared &sh)
+    {
+        v = wave_max(v);
+        if constexpr (W > 1) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6][0] = v;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < W; ++w) v = fmaxf(v, sh.red[w][0]);
+        }
+        return v;
+    }
+    static __device__ float team_sum(float v, Shared &sh)
+    {
+        v = wave_sum(v);
+        if constexpr (W > 1) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6][0] = v;
+            __syncthreads();
+            v = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v += sh.red[w][0];
+        }
+        return v;
+    }
+    // The sums of a row that is masked throughout, holds the lowest or nearly the largest numbers, or is not finite: class by class, the
+    // largest score first
+    static __device__ Soft<MODE == LP> exact_row(const RowArgs &a, const Span<T> &sp, Shared &sh)
+    {
+        const int k1 = sp.k0 + sp.nvec * VEC + sp.edges();
+        Soft<MODE == LP> so;
+        so.init();
+        float m = LOWEST;
+        for (int c = sp.k0 + lane(); c < k1; c += NL) m = fmaxf(m, sis3d_f32(sp.row[c]));
+        so.m = team_max(m, sh);
+        for (int c = sp.k0 + lane(); c < k1; c += NL) so.add(sis3d_f32(sp.row[c]), a.c2);
+        so.s = team_sum(so.s, sh);
+        if constexpr (MODE == LP) so.t = team_sum(so.t, sh);
+        return so;
+    }
+
     // one pass over the span: the team's sums in every lane, and this lane's largest (score, class) among its vectors
     static __device__ Soft<MODE == LP> pass(const RowArgs &a, const Span<T> &sp, Stream<T, NL> &st, Shared &sh, float &best, int &at)
     {
-        Soft<MODE == LP> so;
-        so.init();
+        Lane<MODE == LP> ln;
+        ln.init();
         best = -INFINITY;
         at = lane();
         const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
         st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
             constexpr int N = decltype(count)::value;
             const bool last = v + (N - 1) * NL < sp.nvec;       // no vector: -inf adds nothing
-            float x[N][VEC], top = so.m;
+            float x[N][VEC], top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < N; ++u) {
+                sis3d_unpack<T, VEC>(raw[u], x[u]);
+                if (u == N - 1)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) x[u][i] = u < N - 1 || last ? sis3d_f32(raw[u].v[i]) : -INFINITY;
-                float mx = x[u][0];
-#pragma unroll
-                for (int i = 1; i < VEC; ++i) mx = fmaxf(mx, x[u][i]);
+                    for (int i = 0; i < VEC; ++i) x[u][i] = last ? x[u][i] : -INFINITY;
+                const float mx = max_of(x[u]);
                 if constexpr (MODE == LP) at = mx > best ? v + u * NL : at;
                 best = fmaxf(best, mx);
                 top = fmaxf(top, mx);
             }
-            so.raise(top, a.c2);
+            ln.follow(top, a.c2);
 #pragma unroll
             for (int u = 0; u < N; ++u)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) so.add(x[u][i], a.c2);
+                for (int i = 0; i < VEC; ++i) ln.add(x[u][i], a.c2);
         });
-        so.raise(fmaxf(so.m, edge), a.c2);
-        if (lane() < sp.edges()) so.add(edge, a.c2);
-        so.join_wave(a.c2);
+        ln.follow(edge, a.c2);
+        if (lane() < sp.edges()) ln.add(edge, a.c2);
+        auto so = ln.join_wave(fmaxf(best, edge), a.c2);
         if constexpr (W > 1) {
             if ((threadIdx.x & 63) == 0) {
                 sh.red[threadIdx.x >> 6][0] = so.m;
@@ -497,6 +626,7 @@ template <typename T, int W, int MODE> struct Long {
 #pragma unroll
             for (int w = 1; w < W; ++w) so.join(sh.red[w][0], sh.red[w][1], sh.red[w][2], a.c2);
         }
+        if (!(so.s > 0.f && so.s < INFINITY)) so = exact_row(a, sp, sh);        // the same for all lanes of the team
         return so;
     }
 
@@ -649,7 +779,7 @@ template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t
     const Teacher t = kept.teacher(a);
     float loss = 0.f;
     if (t.any) {
-        const float ls = logf(t.s);
+        const float ls = log_(t.s);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
             if (kept.c[j] >= 0) loss += entry_loss(a, t, ls, kept.x[j], kept.l[j], norm);
@@ -815,18 +945,21 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 c_s[team][lane + 64 * j] = kept.c[j];
-                q_s[team][lane + 64 * j] = t.any ? exp2_((kept.x[j] - t.m) * a.c2) / t.s : 0.f;
+                q_s[team][lane + 64 * j] = t.any ? exp2_((kept.x[j] - t.m) * a.c2) * rcp_(t.s) : 0.f;
             }
     }
     const bool wide = ((uintptr_t)(out + k0 + sp.head) & 15) == 0;
-    st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
+    if (!k.in_range) {
+        for (int c = k0 + lane; c < k1; c += NL) out[c] = sis3d_from_f32<T>(k.exact(sis3d_f32(row[c])));
+    } else st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
         constexpr int N = decltype(count)::value;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int c = sp.first_class(v + u * NL);
             float x[VEC];
+            sis3d_unpack<T, VEC>(raw[u], x);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[i] = k(sis3d_f32(raw[u].v[i]));
+            for (int i = 0; i < VEC; ++i) x[i] = k.near(x[i]);
             if (u == N - 1 && v + u * NL >= sp.nvec) continue;
             if (wide) sis3d_store<T, VEC>(out + c, x);
             else {
@@ -835,12 +968,12 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
             }
         }
     });
-    if (lane < sp.edges()) out[sp.edge_class(lane)] = sis3d_from_f32<T>(k(edge));
+    if (lane < sp.edges() && k.in_range) out[sp.edge_class(lane)] = sis3d_from_f32<T>(k.exact(edge));
     // The label's class, or the kept classes of this part, again with their share: written behind the team's own stores.  A class that
     // is kept twice is written by its first entry with the sum of both.
     team_sync<W>();
     if constexpr (MODE == LP) {
-        if (lane == 0 && y >= 0) out[y] = sis3d_from_f32<T>(k(sis3d_f32(row[y])) + k.ga);
+        if (lane == 0 && y >= 0) out[y] = sis3d_from_f32<T>(k.exact(sis3d_f32(row[y])) + k.ga);
     } else {
         for (int i = lane; i < a.nk; i += NL) {
             const int c = c_s[team][i];
@@ -852,7 +985,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
                     q += q_s[team][j];
                     first = first && j >= i;
                 }
-            if (first) out[c] = sis3d_from_f32<T>(k(sis3d_f32(row[c])) - k.ga * q);
+            if (first) out[c] = sis3d_from_f32<T>(k.exact(sis3d_f32(row[c])) - k.ga * q);
         }
     }
 }

@@ -189,14 +189,14 @@ template <typename T, int VEC, typename F> __device__ inline void each_row(const
     for (int left = n / (U * rpb); left > 0; --left, r += U * rpb) {
         SisVec<T, VEC> v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = *(const SisVec<T, VEC> *)(x + (r + u * rpb) * stride);
+        for (int u = 0; u < U; ++u) v[u] = sis3d_raw<T, VEC>(x + (r + u * rpb) * stride);
 #pragma unroll
         for (int u = 0; u < U; ++u) f(r + u * rpb, true, v[u]);
     }
     if (r < n) {
         SisVec<T, VEC> v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = *(const SisVec<T, VEC> *)(x + min(r + u * rpb, n - 1) * stride);
+        for (int u = 0; u < U; ++u) v[u] = sis3d_raw<T, VEC>(x + min(r + u * rpb, n - 1) * stride);
 #pragma unroll
         for (int u = 0; u < U; ++u) f(r + u * rpb, r + u * rpb < n, v[u]);
     }
@@ -209,8 +209,8 @@ __device__ inline void each_row2(const T *x, int64_t xs, const T *d, int64_t ds,
         SisVec<T, VEC> v[U], w[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            v[u] = *(const SisVec<T, VEC> *)(x + (r + u * rpb) * xs);
-            w[u] = *(const SisVec<T, VEC> *)(d + (r + u * rpb) * ds);
+            v[u] = sis3d_raw<T, VEC>(x + (r + u * rpb) * xs);
+            w[u] = sis3d_raw<T, VEC>(d + (r + u * rpb) * ds);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) f(r + u * rpb, true, v[u], w[u]);
@@ -220,8 +220,8 @@ __device__ inline void each_row2(const T *x, int64_t xs, const T *d, int64_t ds,
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int at = min(r + u * rpb, n - 1);
-            v[u] = *(const SisVec<T, VEC> *)(x + at * xs);
-            w[u] = *(const SisVec<T, VEC> *)(d + at * ds);
+            v[u] = sis3d_raw<T, VEC>(x + at * xs);
+            w[u] = sis3d_raw<T, VEC>(d + at * ds);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) f(r + u * rpb, r + u * rpb < n, v[u], w[u]);
@@ -240,9 +240,11 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
         if (k.ri < n) sis3d_load<T, VEC>(x + k.ri * a.x_v, K);
         each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int, bool there, const SisVec<T, VEC> &v) {
             m += there;
+            float f[VEC];
+            sis3d_unpack<T, VEC>(v, f);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float d = there ? sis3d_f32(v.v[i]) - K[i] : 0.f;
+                const float d = there ? f[i] - K[i] : 0.f;
                 s1[i] += d;
                 s2[i] = fmaf(d, d, s2[i]);
             }
@@ -293,8 +295,9 @@ __device__ inline void apply_rows(const GnArgs &a, const Cols &k, const float *s
     }
     each_row<T, VEC>(x, a.x_v, k.ri, k.rpb, n, [&](int r, bool there, const SisVec<T, VEC> &v) {
         float o[VEC];
+        sis3d_unpack<T, VEC>(v, o);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = act<ACT>(fmaf(sis3d_f32(v.v[i]) - mu[i], sc[i], sh[i]));
+        for (int i = 0; i < VEC; ++i) o[i] = act<ACT>(fmaf(o[i] - mu[i], sc[i], sh[i]));
         if (there) sis3d_store<T, VEC>(y + r * a.y_v, o);
     });
 }
@@ -379,10 +382,13 @@ __device__ inline void tile_grad_sums(const GnArgs &a, const Cols &k, const Tile
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s0[i] = s1[i] = 0.f;
         each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int, bool there, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
+            float xf[VEC], df[VEC];
+            sis3d_unpack<T, VEC>(v, xf);
+            sis3d_unpack<T, VEC>(d, df);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float h = (sis3d_f32(v.v[i]) - c.mu[i]) * c.rs[i];
-                const float e = sis3d_f32(d.v[i]) * act_slope<ACT>(fmaf(h, c.w[i], c.b[i]));
+                const float h = (xf[i] - c.mu[i]) * c.rs[i];
+                const float e = df[i] * act_slope<ACT>(fmaf(h, c.w[i], c.b[i]));
                 s0[i] += there ? e : 0.f;
                 s1[i] += there ? e * h : 0.f;
             }
@@ -432,11 +438,13 @@ __device__ inline void apply_grad(const GnArgs &a, const Cols &k, const Tile &t,
         m2[i] = st[k.gl + g];
     }
     each_row2<T, VEC>(x, a.x_v, dy, a.d_v, k.ri, k.rpb, t.n, [&](int r, bool there, const SisVec<T, VEC> &v, const SisVec<T, VEC> &d) {
-        float o[VEC];
+        float o[VEC], df[VEC];
+        sis3d_unpack<T, VEC>(v, o);
+        sis3d_unpack<T, VEC>(d, df);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float h = (sis3d_f32(v.v[i]) - c.mu[i]) * c.rs[i];
-            const float e = sis3d_f32(d.v[i]) * act_slope<ACT>(fmaf(h, c.w[i], c.b[i])) * c.w[i];
+            const float h = (o[i] - c.mu[i]) * c.rs[i];
+            const float e = df[i] * act_slope<ACT>(fmaf(h, c.w[i], c.b[i])) * c.w[i];
             o[i] = c.rs[i] * (e - fmaf(h, m2[i], m1[i]));
         }
         if (there) sis3d_store<T, VEC>(dx + r * a.y_v, o);
