@@ -19,9 +19,10 @@
 //   longer rows      a wave (K <= 4096) or a workgroup streams a row with 16-byte loads from its first aligned element on
 //   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
 //
-// Alternatives of a long row without sorting it: every lane knows the largest score of its own vectors.  The lanes are put into >= k
-// groups; the smallest of the group maxima is a bound that at least k elements reach, so only lanes whose maximum reaches it are read
-// again (from cache) and their elements at or above it -- k log k of them or so -- are ranked by counting, by (score, class).
+// Alternatives of a long row without sorting it or reading it twice: every lane knows the largest score it has seen.  The lanes of a wave
+// are put into >= k groups; the smallest of the group maxima is a bound that at least k elements reach.  It is taken after 1, 2, 4, ...
+// batches of loads, and vectors with an element that reaches it are noted while they pass -- k log k of them or so a time.  Those that still
+// reach the last bound, one or two a lane, are read again and their elements at or above it ranked by counting, by (score, class).
 #include "elem.h"
 
 namespace {
@@ -494,9 +495,12 @@ template <typename T> struct Span {
 // A lane's vectors lane, lane + NL, ... of a span, UL at a time and the next UL on their way while these are worked on; the first are
 // asked for when the object is made, so that a row's other loads travel with them.  f(count, v, vectors): `count` of them from v on, all
 // there but perhaps the last one of the last batch.
-constexpr int UL = 4;
+#ifndef UL_
+#define UL_ 4
+#endif
+constexpr int UL = UL_;
 template <int N> struct Count { static constexpr int value = N; };
-template <typename T, int NL> struct Stream {
+template <typename T, int NL, bool ONCE> struct Stream {
     static constexpr int VEC = 16 / sizeof(T);
     const Span<T> &sp;
     const int lane;
@@ -505,7 +509,7 @@ template <typename T, int NL> struct Stream {
     __device__ void load(SisVec<T, VEC> (&r)[UL], int v) const
     {
 #pragma unroll
-        for (int u = 0; u < UL; ++u) r[u] = sis3d_load_once<T, VEC>(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
+        for (int u = 0; u < UL; ++u) r[u] = sis3d_raw<T, VEC, ONCE>(sp.body + (int64_t)min(v + u * NL, sp.nvec - 1) * VEC);
     }
     template <typename F> __device__ void each(F f)
     {
@@ -522,6 +526,24 @@ template <typename T, int NL> struct Stream {
         }
         last(left, v, raw, f);
     }
+    // the same with less code (one batch and one vector of it), for work that takes more instructions than a cache of them holds ten times
+    template <typename F> __device__ void each_compact(F f)
+    {
+        int v = lane, left = (sp.nvec + NL - 1) / NL;
+        for (; left > UL; left -= UL, v += UL * NL) {
+            SisVec<T, VEC> next[UL];
+            load(next, v + UL * NL);
+            f(Count<UL>(), v, raw);
+#pragma unroll
+            for (int u = 0; u < UL; ++u) raw[u] = next[u];
+        }
+#pragma unroll 1
+        for (; left > 0; --left, v += NL) {
+            f(Count<1>(), v, raw);
+#pragma unroll
+            for (int u = 0; u + 1 < UL; ++u) raw[u] = raw[u + 1];
+        }
+    }
     template <typename F> __device__ void last(int left, int v, const SisVec<T, VEC> (&r)[UL], F f)
     {
         switch (left) {
@@ -533,14 +555,45 @@ template <typename T, int NL> struct Stream {
     }
 };
 
-template <typename T, int W, int MODE> struct Long {
-    static constexpr int NL = 64 * W, CAP = W == 1 ? 512 : 1024, VEC = 16 / sizeof(T);
+template <typename T, int W, int MODE, bool TOP> struct Long {
+    static constexpr int NL = 64 * W, ROOM = 256, VEC = 16 / sizeof(T);
+    struct Vec { float m; int v; };            // a vector and its largest score
     struct Shared {
-        uint64_t cand[CAP], bound[W];
-        float red[W][3];
-        int lanes[W][64], count;
+        uint64_t cand[W][ROOM], bound[W];      // a wave's elements
+        Vec vecs[TOP ? W : 1][TOP ? ROOM : 1]; // and the vectors they are in
+        float red[W][5];
+        int lanes[W][64], count[W], total;
     };
     static __device__ int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
+    static __device__ int wave() { return W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+    // What a wave notes while it reads; all but `best` and `at` is the same in all lanes
+    struct Noted {
+        float best, b;                         // this lane's largest score; the bound
+        int at;                                // the first vector that has `best`
+        int lanes, count, batch, next;
+        bool over;                             // there was no room
+        __device__ void init(int want, int lane)
+        {
+            best = b = -INFINITY;
+            at = lane;
+            lanes = want > 16 ? 2 : want > 8 ? 4 : want > 4 ? 8 : 16;
+            count = batch = 0;
+            next = 1;
+            over = false;
+        }
+        __device__ void tighten() { b = fmaxf(b, wave_min(lanes_max(best, lanes))); }
+        // puts entries of the lanes that have one behind the list's others
+        template <typename E> __device__ void note(E *list, bool there, E entry)
+        {
+            const uint64_t mask = __ballot(there);
+            if (!mask) return;
+            const int n = __popcll(mask);
+            if (count + n > ROOM) { over = true; return; }
+            if (there) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = entry;
+            count += n;
+        }
+    };
 
     static __device__ float team_max(float v, Shared &sh)
     {
@@ -584,44 +637,68 @@ template <typename T, int W, int MODE> struct Long {
     }
 
     // one pass over the span: the team's sums in every lane, and this lane's largest (score, class) among its vectors
-    static __device__ Soft<MODE == LP> pass(const RowArgs &a, const Span<T> &sp, Stream<T, NL> &st, Shared &sh, float &best, int &at)
+    static __device__ Soft<MODE == LP> pass(const RowArgs &a, const Span<T> &sp, Stream<T, NL, !TOP> &st, Shared &sh, Noted &nt)
     {
         Lane<MODE == LP> ln;
         ln.init();
-        best = -INFINITY;
-        at = lane();
+        nt.init(a.top, lane());
         const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
-        st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
+        auto batch = [&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
             constexpr int N = decltype(count)::value;
             const bool last = v + (N - 1) * NL < sp.nvec;       // no vector: -inf adds nothing
-            float x[N][VEC], top = -INFINITY;
+            float x[N][VEC], mx[N], top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 sis3d_unpack<T, VEC>(raw[u], x[u]);
                 if (u == N - 1)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) x[u][i] = last ? x[u][i] : -INFINITY;
-                const float mx = max_of(x[u]);
-                if constexpr (MODE == LP) at = mx > best ? v + u * NL : at;
-                best = fmaxf(best, mx);
-                top = fmaxf(top, mx);
+                mx[u] = max_of(x[u]);
+                if constexpr (TOP) nt.at = mx[u] > nt.best ? v + u * NL : nt.at;
+                nt.best = fmaxf(nt.best, mx[u]);
+                top = fmaxf(top, mx[u]);
             }
             ln.follow(top, a.c2);
+            if constexpr (TOP) {
+                if (++nt.batch == nt.next || nt.b == -INFINITY) {
+                    nt.tighten();
+                    nt.next = 2 * nt.batch;
+                }
+#pragma unroll
+                for (int u = 0; u < N; ++u) nt.note(sh.vecs[wave()], mx[u] >= nt.b && mx[u] > -INFINITY, Vec{mx[u], v + u * NL});
+            }
 #pragma unroll
             for (int u = 0; u < N; ++u)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) ln.add(x[u][i], a.c2);
-        });
+        };
+        if constexpr (MODE == LP) st.each_compact(batch);      // with and without alternatives: the same sums, bit for bit
+        else st.each(batch);
         ln.follow(edge, a.c2);
         if (lane() < sp.edges()) ln.add(edge, a.c2);
-        auto so = ln.join_wave(fmaxf(best, edge), a.c2);
+        float block = INFINITY;                 // a bound from all waves' groups together, a quarter as many of each
+        if constexpr (TOP) {
+            nt.tighten();
+            if (W > 1) block = wave_min(lanes_max(nt.best, a.top > 16 ? 8 : 16));
+        }
+        auto so = ln.join_wave(fmaxf(nt.best, edge), a.c2);
         if constexpr (W > 1) {
             if ((threadIdx.x & 63) == 0) {
                 sh.red[threadIdx.x >> 6][0] = so.m;
                 sh.red[threadIdx.x >> 6][1] = so.s;
                 sh.red[threadIdx.x >> 6][2] = so.t;
+                sh.red[threadIdx.x >> 6][3] = nt.b;
+                sh.red[threadIdx.x >> 6][4] = block;
             }
             __syncthreads();
+            if constexpr (TOP) {
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    nt.b = fmaxf(nt.b, sh.red[w][3]);
+                    block = fminf(block, sh.red[w][4]);
+                }
+                nt.b = fmaxf(nt.b, block);
+            }
             so = Soft<MODE == LP>{sh.red[0][0], sh.red[0][1], sh.red[0][2]};
 #pragma unroll
             for (int w = 1; w < W; ++w) so.join(sh.red[w][0], sh.red[w][1], sh.red[w][2], a.c2);
@@ -630,20 +707,21 @@ template <typename T, int W, int MODE> struct Long {
         return so;
     }
 
-    // Elements of the span that pass `keep(score, class)`, from the lanes whose `again` says that they have one and from the edges: into
-    // sh.cand, at most CAP of them, and their number as the answer
+    // Elements of the span that pass `keep(score, class)`, from the lanes whose `again` says that they have one and from the edges: read
+    // again into sh.cand as one list, and their number as the answer, which may be more than there is room for
     template <typename F> static __device__ int collect(const Span<T> &sp, Shared &sh, bool again, F keep)
     {
-        const int w = W == 1 ? 0 : threadIdx.x >> 6, ln = threadIdx.x & 63;
+        const int w = wave(), ln = threadIdx.x & 63;
+        uint64_t *cand = sh.cand[0];
         team_sync<W>();
-        if (lane() == 0) sh.count = 0;
+        if (lane() == 0) sh.total = 0;
         const uint64_t mask = __ballot(again);
         if (again) sh.lanes[w][__popcll(mask & ((1ull << ln) - 1))] = ln;
         team_sync<W>();
         auto offer = [&](float v, int c) {
             if (keep(v, c)) {
-                const int i = atomicAdd(&sh.count, 1);
-                if (i < CAP) sh.cand[i] = key_of(v, c);
+                const int i = atomicAdd(&sh.total, 1);
+                if (i < W * ROOM) cand[i] = key_of(v, c);
             }
         };
         const int per = (sp.nvec + NL - 1) / NL, items = __popcll(mask) * per;
@@ -660,40 +738,79 @@ template <typename T, int W, int MODE> struct Long {
             offer(sis3d_f32(sp.row[c]), c);
         }
         team_sync<W>();
-        return sh.count;
+        return sh.total;
     }
 
-    // The `top` largest keys of the span, out(rank, key) once for each rank.  best, at: this lane's largest score among its vectors, and
-    // the first vector that has it.
-    template <typename F> static __device__ void alternatives(const RowArgs &a, const Span<T> &sp, Shared &sh, float best, int at, F out)
+    // The `top` largest keys of the span, out(rank, key) once for each rank, from what the waves have noted
+    template <typename F> static __device__ void alternatives(const RowArgs &a, const Span<T> &sp, Shared &sh, Noted &nt, F out)
     {
-        const int want = a.top, w = W == 1 ? 0 : threadIdx.x >> 6, ln = threadIdx.x & 63;       // a span has far more classes
-        // the smallest of the maxima of >= want groups of lanes: at least want elements of this wave reach it
-        float b = wave_min(lanes_max(best, want > 16 ? 2 : want > 8 ? 4 : want > 4 ? 8 : 16));
-        if constexpr (W > 1) {
-            if (ln == 0) sh.red[w][0] = b;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < W; ++i) b = fmaxf(b, sh.red[i][0]);
+        const int want = a.top, w = wave(), ln = threadIdx.x & 63;       // a span has far more classes
+        // of the vectors noted, those that reach the last bound are read again and their elements that do are noted
+        const int vecs = nt.over ? 0 : nt.count;
+        int kept = 0;
+        for (int i = 0; i < vecs; i += 64) {
+            const Vec e = sh.vecs[w][min(i + ln, vecs - 1)];
+            const uint64_t mask = __ballot(i + ln < vecs && e.m >= nt.b);
+            if (mask >> ln & 1) sh.vecs[w][kept + __popcll(mask & ((1ull << ln) - 1))] = e;         // not behind its own place
+            kept += __popcll(mask);
+            team_sync<1>();
         }
-        int m = collect(sp, sh, best >= b && best > -INFINITY, [&](float v, int) { return v >= b && v > -INFINITY; });
-        if (m < want) {                                    // -inf (and NaN, which counts as that) from the lowest class on: 64 hold enough
+        nt.count = 0;
+        for (int i = 0; i < kept; i += 64) {
+            const int v = sh.vecs[w][min(i + ln, kept - 1)].v, c = sp.first_class(v);
+            float x[VEC];
+            sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) nt.note(sh.cand[w], i + ln < kept && x[e] >= nt.b && x[e] > -INFINITY, key_of(x[e], c + e));
+        }
+        const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
+        nt.note(sh.cand[w], edge >= nt.b && edge > -INFINITY, key_of(edge, sp.edge_class(lane())));
+        bool over = nt.over;
+        int m = nt.count;
+        if constexpr (W > 1) {
+            if (ln == 0) sh.count[w] = over ? -1 : m;
+            __syncthreads();
+            m = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int n = sh.count[i];
+                over = over || n < 0;
+                m += n;
+            }
+        } else team_sync<1>();
+        if (!over && m >= want) {
+            for (int i = ln; i < nt.count; i += 64) {
+                const uint64_t k = sh.cand[w][i];
+                int rank = 0;
+#pragma unroll
+                for (int q = 0; q < W; ++q) {
+                    const int n = W == 1 ? nt.count : sh.count[q];
+#pragma unroll 4
+                    for (int j = 0; j < n; ++j) rank += sh.cand[q][j] > k;
+                }
+                if (rank < want) out(rank, k);
+            }
+            return;
+        }
+        const int room = W * ROOM;
+        uint64_t *cand = sh.cand[0];
+        if (!over) {
+            // fewer numbers than that: -inf (and NaN, which counts as that) from the lowest class on; the first 64 classes hold enough
+            m = collect(sp, sh, nt.best > -INFINITY, [](float v, int) { return v > -INFINITY; });
             const int c = sp.k0 + ln;
             const float v = sis3d_f32(sp.row[c]);
             const bool none = !(v > -INFINITY);
             const uint64_t mask = __ballot(none);
             const int i = m + __popcll(mask & ((1ull << ln) - 1));
-            team_sync<W>();
-            if (none && i < want && w == 0) sh.cand[i] = key_of(v, c);
+            if (none && i < want && w == 0) cand[i] = key_of(v, c);
             team_sync<W>();
             m = want;
-        }
-        if (m > CAP) {
+        } else {
             // Many equal scores at the bound: a bound on (score, class).  A vector's last class stands for the place of its maximum,
             // vectors being disjoint ranges of classes.
             int groups = 1;
             while (groups < want) groups *= 2;
-            const uint64_t mine = lane() < sp.nvec ? key_of(best, sp.first_class(at) + VEC - 1) : 0;
+            const uint64_t mine = lane() < sp.nvec ? key_of(nt.best, sp.first_class(nt.at) + VEC - 1) : 0;
             uint64_t k = mine;
             for (int o = 32; o >= groups; o >>= 1) k = max64(k, shfl_xor64(k, o));
             for (int o = groups >> 1; o > 0; o >>= 1) k = min64(k, shfl_xor64(k, o));
@@ -705,11 +822,11 @@ template <typename T, int W, int MODE> struct Long {
             }
             m = collect(sp, sh, mine != 0 && mine >= k, [&](float v, int c) { return key_of(v, c) >= k; });
         }
-        if (m <= CAP) {
+        if (m <= room) {
             for (int i = lane(); i < m; i += NL) {
-                const uint64_t k = sh.cand[i];
+                const uint64_t k = cand[i];
                 int rank = 0;
-                for (int j = 0; j < m; ++j) rank += sh.cand[j] > k;
+                for (int j = 0; j < m; ++j) rank += cand[j] > k;
                 if (rank < want) out(rank, k);
             }
             return;
@@ -814,9 +931,9 @@ template <int MODE> __device__ inline void zero_row(const RowArgs &a, int64_t r,
         }
 }
 
-template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void long_forward(RowArgs a)
+template <typename T, int W, int MODE, bool TOP> __global__ __launch_bounds__(256) void long_forward(RowArgs a)
 {
-    using L = Long<T, W, MODE>;
+    using L = Long<T, W, MODE, TOP>;
     __shared__ typename L::Shared shared[4 / W];
     auto &sh = shared[team_of<W>()];
     const int64_t r = (int64_t)blockIdx.x * (4 / W) + team_of<W>();
@@ -824,20 +941,19 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     if (r >= live_rows(a)) { zero_row<MODE>(a, r, L::lane(), L::NL); return; }
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     const Span<T> sp(row, 0, a.K);
-    Stream<T, L::NL> st(sp, L::lane());
-    float best;
-    int at;
+    Stream<T, L::NL, !TOP> st(sp, L::lane());
+    typename L::Noted nt;
     if constexpr (MODE == KD) {
         const bool first = W == 1 || threadIdx.x < 64;
         const Kept kept(a, r, row, first);
-        const auto so = L::pass(a, sp, st, sh, best, at);
+        const auto so = L::pass(a, sp, st, sh, nt);
         if (first) wave_loss<T>(a, r, kept, so);
     } else {
-        const auto so = L::pass(a, sp, st, sh, best, at);
+        const auto so = L::pass(a, sp, st, sh, nt);
         const Norm norm{so.m, so.log_s()};
         if (L::lane() == 0) row_outputs(a, r, row, so, norm);
-        if (a.top)
-            L::alternatives(a, sp, sh, best, at, [&](int rank, uint64_t k) {
+        if constexpr (TOP)
+            L::alternatives(a, sp, sh, nt, [&](int rank, uint64_t k) {
                 a.top_class[r * a.top + rank] = key_class(k);
                 a.top_logp[r * a.top + rank] = log_p(key_score(k), norm, 1.f, 0.f);
             });
@@ -845,9 +961,9 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
 }
 
 // one part of a row to a workgroup
-template <typename T, int MODE> __global__ __launch_bounds__(256) void split_forward(RowArgs a)
+template <typename T, int MODE, bool TOP> __global__ __launch_bounds__(256) void split_forward(RowArgs a)
 {
-    using L = Long<T, 4, MODE>;
+    using L = Long<T, 4, MODE, TOP>;
     __shared__ typename L::Shared sh;
     const int64_t r = blockIdx.x / a.parts;
     const int part = blockIdx.x - (int)(r * a.parts);
@@ -855,13 +971,11 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void split_for
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     const int k0 = (int)((int64_t)a.K * part / a.parts), k1 = (int)((int64_t)a.K * (part + 1) / a.parts);
     const Span<T> sp(row, k0, k1);
-    Stream<T, L::NL> st(sp, L::lane());
-    float best;
-    int at;
-    const auto so = L::pass(a, sp, st, sh, best, at);
+    Stream<T, L::NL, !TOP> st(sp, L::lane());
+    typename L::Noted nt;
+    const auto so = L::pass(a, sp, st, sh, nt);
     if (threadIdx.x == 0) *(float4 *)(a.part + (size_t)blockIdx.x * 4) = make_float4(so.m, so.s, so.t, 0.f);
-    if constexpr (MODE == LP)
-        if (a.top) L::alternatives(a, sp, sh, best, at, [&](int rank, uint64_t k) { a.part_keys[(size_t)blockIdx.x * a.top + rank] = k; });
+    if constexpr (TOP) L::alternatives(a, sp, sh, nt, [&](int rank, uint64_t k) { a.part_keys[(size_t)blockIdx.x * a.top + rank] = k; });
 }
 
 // joins the parts of a row: one wave
@@ -929,7 +1043,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
         return;
     }
     const Span<T> sp(row, k0, k1);
-    Stream<T, NL> st(sp, lane);
+    Stream<T, NL, true> st(sp, lane);
     const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : 0.f;
     Back<MODE> k;
     int y = -1;
@@ -1012,13 +1126,18 @@ template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
         else hipLaunchKernelGGL((small_forward<T, 16, MODE>), grid, dim3(256), 0, st, a);
         return sis3d_check_launch();
     }
-    if (a.parts > 1) {
-        hipLaunchKernelGGL((split_forward<T, MODE>), dim3((unsigned)(a.R * a.parts)), dim3(256), 0, st, a);
-        const int rc = sis3d_check_launch();
-        if (rc) return rc;
-        hipLaunchKernelGGL((split_join<T, MODE>), dim3((unsigned)a.R), dim3(64), 0, st, a);
-    } else if (a.K <= K_WAVE) hipLaunchKernelGGL((long_forward<T, 1, MODE>), dim3((unsigned)((a.R + 3) / 4)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((long_forward<T, 4, MODE>), dim3((unsigned)a.R), dim3(256), 0, st, a);
+    const dim3 block(256), each(a.parts > 1 ? (unsigned)(a.R * a.parts) : a.K <= K_WAVE ? (unsigned)((a.R + 3) / 4) : (unsigned)a.R);
+    auto launch = [&](auto top) {
+        constexpr bool TOP = decltype(top)::value && MODE == LP;
+        if (a.parts > 1) hipLaunchKernelGGL((split_forward<T, MODE, TOP>), each, block, 0, st, a);
+        else if (a.K <= K_WAVE) hipLaunchKernelGGL((long_forward<T, 1, MODE, TOP>), each, block, 0, st, a);
+        else hipLaunchKernelGGL((long_forward<T, 4, MODE, TOP>), each, block, 0, st, a);
+    };
+    if (a.top) launch(Count<1>());
+    else launch(Count<0>());
+    const int rc = sis3d_check_launch();
+    if (rc || a.parts == 1) return rc;
+    hipLaunchKernelGGL((split_join<T, MODE>), dim3((unsigned)a.R), dim3(64), 0, st, a);
     return sis3d_check_launch();
 }
 
