@@ -495,13 +495,11 @@ template <typename T> struct Span {
 // A lane's vectors lane, lane + NL, ... of a span, UL at a time and the next UL on their way while these are worked on; the first are
 // asked for when the object is made, so that a row's other loads travel with them.  f(count, v, vectors): `count` of them from v on, all
 // there but perhaps the last one of the last batch.
-#ifndef UL_
-#define UL_ 4
-#endif
-constexpr int UL = UL_;
+// UL: 4 where a workgroup has a row, 2 where a wave has a short one (40000 x 1203 fp16, distillation forward: 39.4 us with 4, 36.5 with 2)
+constexpr int loads_of(int NL) { return NL > 64 ? 4 : 2; }
 template <int N> struct Count { static constexpr int value = N; };
 template <typename T, int NL, bool ONCE> struct Stream {
-    static constexpr int VEC = 16 / sizeof(T);
+    static constexpr int VEC = 16 / sizeof(T), UL = loads_of(NL);
     const Span<T> &sp;
     const int lane;
     SisVec<T, VEC> raw[UL];
@@ -546,17 +544,17 @@ template <typename T, int NL, bool ONCE> struct Stream {
     }
     template <typename F> __device__ void last(int left, int v, const SisVec<T, VEC> (&r)[UL], F f)
     {
-        switch (left) {
-        case 1: f(Count<1>(), v, r); break;
-        case 2: f(Count<2>(), v, r); break;
-        case 3: f(Count<3>(), v, r); break;
-        case 4: f(Count<4>(), v, r); break;
+        if (left == 1) f(Count<1>(), v, r);
+        else if (left == 2) f(Count<2>(), v, r);
+        if constexpr (UL > 2) {
+            if (left == 3) f(Count<3>(), v, r);
+            else if (left == 4) f(Count<4>(), v, r);
         }
     }
 };
 
 template <typename T, int W, int MODE, bool TOP> struct Long {
-    static constexpr int NL = 64 * W, ROOM = 256, VEC = 16 / sizeof(T);
+    static constexpr int NL = 64 * W, ROOM = 256, VEC = 16 / sizeof(T), UL = loads_of(NL);
     struct Vec { float m; int v; };            // a vector and its largest score
     struct Shared {
         uint64_t cand[W][ROOM], bound[W];      // a wave's elements
@@ -567,16 +565,14 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     static __device__ int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
     static __device__ int wave() { return W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-    // What a wave notes while it reads; all but `best` and `at` is the same in all lanes
+    // What a wave notes while it reads; all but `best` is the same in all lanes
     struct Noted {
         float best, b;                         // this lane's largest score; the bound
-        int at;                                // the first vector that has `best`
         int lanes, count, batch, next;
         bool over;                             // there was no room
-        __device__ void init(int want, int lane)
+        __device__ void init(int want)
         {
             best = b = -INFINITY;
-            at = lane;
             lanes = want > 16 ? 2 : want > 8 ? 4 : want > 4 ? 8 : 16;
             count = batch = 0;
             next = 1;
@@ -641,7 +637,7 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     {
         Lane<MODE == LP> ln;
         ln.init();
-        nt.init(a.top, lane());
+        nt.init(a.top);
         const float edge = lane() < sp.edges() ? sis3d_f32(sp.row[sp.edge_class(lane())]) : -INFINITY;
         auto batch = [&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
             constexpr int N = decltype(count)::value;
@@ -654,7 +650,6 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) x[u][i] = last ? x[u][i] : -INFINITY;
                 mx[u] = max_of(x[u]);
-                if constexpr (TOP) nt.at = mx[u] > nt.best ? v + u * NL : nt.at;
                 nt.best = fmaxf(nt.best, mx[u]);
                 top = fmaxf(top, mx[u]);
             }
@@ -810,7 +805,13 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
             // vectors being disjoint ranges of classes.
             int groups = 1;
             while (groups < want) groups *= 2;
-            const uint64_t mine = lane() < sp.nvec ? key_of(nt.best, sp.first_class(nt.at) + VEC - 1) : 0;
+            int at = lane();
+            for (int v = lane(); v < sp.nvec; v += NL) {
+                float x[VEC];
+                sis3d_load<T, VEC>(sp.body + (int64_t)v * VEC, x);
+                if (max_of(x) == nt.best) { at = v; break; }
+            }
+            const uint64_t mine = lane() < sp.nvec ? key_of(nt.best, sp.first_class(at) + VEC - 1) : 0;
             uint64_t k = mine;
             for (int o = 32; o >= groups; o >>= 1) k = max64(k, shfl_xor64(k, o));
             for (int o = groups >> 1; o > 0; o >>= 1) k = min64(k, shfl_xor64(k, o));
@@ -1024,7 +1025,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join
 // gradient of a row's part; `parts` workgroups or one team to a row
 template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void long_backward(RowArgs a)
 {
-    constexpr int NL = 64 * W, VEC = 16 / sizeof(T);
+    constexpr int NL = 64 * W, VEC = 16 / sizeof(T), UL = loads_of(NL);
     __shared__ float q_s[4 / W][KEPT_MAX];
     __shared__ int c_s[4 / W][KEPT_MAX];
     const int team = team_of<W>(), lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;

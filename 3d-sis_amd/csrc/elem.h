@@ -56,7 +56,7 @@ template <typename T, int VEC> __device__ inline void sis3d_unpack(const SisVec<
 }
 template <typename T, int VEC> __device__ inline void sis3d_load(const T *p, float (&out)[VEC]) { sis3d_unpack<T, VEC>(sis3d_raw<T, VEC>(p), out); }
 
-template <typename T, int VEC> __device__ inline void sis3d_store(T *p, const float (&in)[VEC])
+template <typename T, int VEC, bool ONCE = false> __device__ inline void sis3d_store(T *p, const float (&in)[VEC])
 {
     if constexpr (VEC == 1) *p = (T)in[0];
     else {
@@ -67,7 +67,8 @@ template <typename T, int VEC> __device__ inline void sis3d_store(T *p, const fl
             else if constexpr (__is_same(T, __bf16)) v[i] = __builtin_bit_cast(uint32_t, sis3d_bf16x2{(__bf16)in[2 * i], (__bf16)in[2 * i + 1]});
             else v[i] = __builtin_bit_cast(uint32_t, sis3d_f16x2{(_Float16)in[2 * i], (_Float16)in[2 * i + 1]});
         }
-        *reinterpret_cast<sis3d_u32x4 *>(p) = v;
+        if constexpr (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<sis3d_u32x4 *>(p));
+        else *reinterpret_cast<sis3d_u32x4 *>(p) = v;
     }
 }
 
