@@ -166,17 +166,18 @@ template <typename P, typename F> __device__ inline void reduce_tiles(const P *p
 
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2;
 
+__device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }      // two units in the last place
 template <int ACT> __device__ inline float act(float z)
 {
     if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;                 // NaN stays NaN
-    else if constexpr (ACT == ACT_SILU) return z / (1.f + __expf(-z));
+    else if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
     else return z;
 }
 template <int ACT> __device__ inline float act_slope(float z)
 {
     if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
     else if constexpr (ACT == ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-z));
+        const float s = sigmoid(z);
         return s * (1.f + z * (1.f - s));
     } else return 1.f;
 }

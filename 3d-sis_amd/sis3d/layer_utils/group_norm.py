@@ -20,9 +20,8 @@ class GroupNormAct(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, mean, rstd, offsets = ctx.saved_tensors
         try:
-            ops._channel_rows(dy, "dy", offsets)
+            ops._channel_rows(dy.shape, dy.stride(), None if offsets is None else offsets.numel() - 1, "dy")
         except ops._lib.Sis3dError:                 # autograd may hand in any layout (an expanded sum's gradient, a planar one)
-            d = ops._like_rows(x, offsets)
-            dy = d.copy_(dy)
+            dy = torch.empty_strided(x.shape, ops._last_second(x.shape), dtype=x.dtype, device=x.device).copy_(dy)
         dx, dw, db = ops.group_norm_backward(dy, x, mean, rstd, ctx.groups, weight, bias, act=ctx.act, offsets=offsets)
         return dx, dw, db, None, None, None, None

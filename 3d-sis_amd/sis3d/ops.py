@@ -1651,6 +1651,9 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include
 _ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2}
 
 
+_f32, _i64 = torch.float32, torch.int64
+
+
 def _on_device(fn):
     """run on the device of the first tensor argument (and on that device's current stream), whatever the current device is"""
     @_functools.wraps(fn)
@@ -1671,12 +1674,15 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _elem(t, name):
+def _gpu(t, name):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise _lib.Sis3dError("%s must be a CUDA/ROCm tensor (sis3d has no CPU path)" % name)
-    code = _DTYPES.get(t.dtype)
+
+
+def _elem_code(dtype, name):
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise _lib.Sis3dError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+        raise _lib.Sis3dError("%s must be float32, bfloat16 or float16, got %s" % (name, dtype))
     return code
 
 
@@ -1684,7 +1690,7 @@ def _side(t, name, like, dtype, shape, optional=True):
     """a contiguous companion tensor of `like`: type, shape and device are checked"""
     if t is None and optional:
         return None
-    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != dtype:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != like.device:
         raise _lib.Sis3dError("%s must be a %s tensor on %s" % (name, dtype, like.device))
     if t.shape != shape:
         raise _lib.Sis3dError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
@@ -1709,9 +1715,21 @@ def _one_stride(sizes, strides):
     return step
 
 
+def _last_second(shape):
+    """strides of a dense tensor of this shape with dimension 1 last in memory"""
+    strides, step = [0] * len(shape), shape[1]
+    for i in range(len(shape) - 1, 1, -1):
+        strides[i] = step
+        step *= shape[i]
+    strides[0], strides[1] = step, 1
+    return tuple(strides)
+
+
+# What follows from shapes, strides and types alone is worked out once for each combination that a program uses.
 @_functools.lru_cache(maxsize=1024)
-def _channel_rows_of(shape, stride, samples, name):
-    """the answer of _channel_rows for tensors of this shape and these strides; samples: their number with offsets, or None"""
+def _channel_rows(shape, stride, samples, name):
+    """(samples, rows, channels, sample stride, row stride) of (N,C,*spatial) in channels-last memory, or, with a number of samples, of the
+    (rows, C) that offsets divide among them"""
     if samples is not None:
         if len(shape) != 2:
             raise _lib.Sis3dError("%s must be (rows, C) with offsets" % name)
@@ -1733,46 +1751,32 @@ def _channel_rows_of(shape, stride, samples, name):
     return S, V, C, sn, sv if sv is not None else C
 
 
-def _channel_rows(t, name, offsets):
-    """(samples, rows, channels, sample stride, row stride) of (N,C,*spatial) in channels-last memory, or of (rows, C) with offsets"""
-    return _channel_rows_of(tuple(t.shape), t.stride(), None if offsets is None else offsets.numel() - 1, name)
-
-
-def _like_rows(x, offsets):
-    """an uninitialised tensor of x's shape and type, dense channels-last"""
-    n = x.dim()
-    if offsets is not None or n == 2:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    shape = tuple(x.shape)
-    C = shape[1]
-    strides, step = [0] * n, C
-    for i in range(n - 1, 1, -1):
-        strides[i] = step
-        step *= shape[i]
-    strides[0], strides[1] = step, 1
-    return torch.empty_strided(shape, strides, dtype=x.dtype, device=x.device)
-
-
 @_functools.lru_cache(maxsize=1024)
-def _norm_workspace(code, S, V, ragged, C, groups, backward):
-    return lib().sis3d_group_norm_workspace_bytes(code, S, V, ragged, C, groups, backward)
-
-
-def _norm_args(x, groups, weight, bias, act, offsets):
-    code = _elem(x, "x")
-    if offsets is not None:
-        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 1:
-            raise _lib.Sis3dError("offsets must be (samples + 1,) row offsets")
-        offsets = _side(offsets, "offsets", x, torch.int64, offsets.shape)
-    S, V, C, sn, sv = _channel_rows(x, "x", offsets)
+def _norm_plan(dtype, shape, stride, samples, groups, act):
+    """(type, samples, rows, channels, sample stride, row stride, groups, activation, strides of a dense result, workspace bytes forward and
+    backward) of a group norm"""
+    code = _elem_code(dtype, "x")
+    S, V, C, sn, sv = _channel_rows(shape, stride, samples, "x")
     groups = int(groups)
     if groups < 1 or C < 1 or C % groups:
         raise _lib.Sis3dError("group norm: %d channels do not split into %d groups" % (C, groups))
     if act not in _ACTS:
         raise _lib.Sis3dError("group norm: act must be one of 'none', 'relu', 'silu', got %r" % (act,))
-    weight = _side(weight, "weight", x, torch.float32, (C,))
-    bias = _side(bias, "bias", x, torch.float32, (C,))
-    return code, S, V, C, sn, sv, groups, weight, bias, offsets
+    ws = [lib().sis3d_group_norm_workspace_bytes(code, S, V, 0 if samples is None else 1, C, groups, back) for back in (0, 1)]
+    return code, S, V, C, sn, sv, groups, _ACTS[act], _last_second(shape), ws[0], ws[1]
+
+
+def _norm_args(x, groups, weight, bias, act, offsets):
+    _gpu(x, "x")
+    samples = None
+    if offsets is not None:
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 1:
+            raise _lib.Sis3dError("offsets must be (samples + 1,) row offsets")
+        offsets = _side(offsets, "offsets", x, _i64, offsets.shape)
+        samples = offsets.numel() - 1
+    plan = _norm_plan(x.dtype, x.shape, x.stride(), samples, groups, act)
+    C = plan[3]
+    return plan, samples, offsets, _side(weight, "weight", x, _f32, (C,)), _side(bias, "bias", x, _f32, (C,))
 
 
 def _norm_check(rc, what, C, groups):
@@ -1790,24 +1794,25 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act=None, offsets=No
     RaggedBatch.  weight / bias (C,) fp32 or None; act: None / 'none', 'relu', 'silu'.  out: where to write (x itself is allowed, any
     other overlap is not); rows behind offsets[-1] are left as they are in `out`, and zero without it.
     -> y, or (y, mean, rstd) with want_stats: (samples, groups) fp32 for group_norm_backward."""
-    code, S, V, C, sn, sv, groups, weight, bias, offsets = _norm_args(x, groups, weight, bias, act, offsets)
+    (code, S, V, C, sn, sv, groups, actc, dense, wsb, _), samples, offsets, weight, bias = _norm_args(x, groups, weight, bias, act, offsets)
     if out is None:
-        y, yn, yv = _like_rows(x, offsets), V * C, C
+        y, yn, yv = torch.empty_strided(x.shape, dense, dtype=x.dtype, device=x.device), V * C, C
     else:
         y = out
-        if _elem(out, "out") != code or out.shape != x.shape or out.device != x.device:
+        _gpu(out, "out")
+        if out.dtype is not x.dtype or out.shape != x.shape or out.device != x.device:
             raise _lib.Sis3dError("group norm: `out` must have x's shape, type and device")
-        _, _, _, yn, yv = _channel_rows(out, "out", offsets)
+        _, _, _, yn, yv = _channel_rows(out.shape, out.stride(), samples, "out")
         if offsets is None and S > 1 and V > 0 and yn < (V - 1) * yv + C and (yn < C or yv < (S - 1) * yn + C):
             raise _lib.Sis3dError("group norm: the samples of `out` overlap in memory")
     mean = rstd = None
     if want_stats:
-        mean, rstd = torch.empty(S, groups, dtype=torch.float32, device=x.device), torch.empty(S, groups, dtype=torch.float32, device=x.device)
-    wsb = _norm_workspace(code, S, V, 0 if offsets is None else 1, C, groups, 0)
+        mean, rstd = torch.empty((S, groups), dtype=_f32, device=x.device), torch.empty((S, groups), dtype=_f32, device=x.device)
     ws = _workspace(wsb, x)
-    _norm_check(lib().sis3d_group_norm_forward(_at(x), code, S, V, _at(offsets), sn, sv, C, groups, _at(weight), _at(bias), float(eps),
-                                               _ACTS[act], _at(y), yn, yv, 1 if out is None else 0, _at(mean), _at(rstd), _at(ws), wsb,
-                                               _raw_stream(x)), "sis3d_group_norm_forward", C, groups)
+    rc = lib().sis3d_group_norm_forward(x.data_ptr(), code, S, V, _at(offsets), sn, sv, C, groups, _at(weight), _at(bias), eps, actc,
+                                        y.data_ptr(), yn, yv, 1 if out is None else 0, _at(mean), _at(rstd), _at(ws), wsb, _raw_stream(x))
+    if rc:
+        _norm_check(rc, "sis3d_group_norm_forward", C, groups)
     return (y, mean, rstd) if want_stats else y
 
 
@@ -1815,54 +1820,60 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act=None, offsets=No
 def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, act=None, offsets=None):
     """gradients of group_norm (sis3d_group_norm_backward): dy like y, the call's own x, mean, rstd, weight, bias, act, offsets
     -> (dx, dweight, dbias), the last two fp32, None where the parameter is None.  Sums are deterministic."""
-    code, S, V, C, sn, sv, groups, weight, bias, offsets = _norm_args(x, groups, weight, bias, act, offsets)
-    if _elem(dy, "dy") != code or dy.shape != x.shape or dy.device != x.device:
+    (code, S, V, C, sn, sv, groups, actc, dense, _, wsb), samples, offsets, weight, bias = _norm_args(x, groups, weight, bias, act, offsets)
+    _gpu(dy, "dy")
+    if dy.dtype is not x.dtype or dy.shape != x.shape or dy.device != x.device:
         raise _lib.Sis3dError("group norm: dy must have x's shape, type and device")
-    _, _, _, dn, dv = _channel_rows(dy, "dy", offsets)
-    mean = _side(mean, "mean", x, torch.float32, (S, groups), optional=False)
-    rstd = _side(rstd, "rstd", x, torch.float32, (S, groups), optional=False)
-    dx = _like_rows(x, offsets)
-    dw = torch.empty(C, dtype=torch.float32, device=x.device) if weight is not None else None
-    db = torch.empty(C, dtype=torch.float32, device=x.device) if bias is not None else None
-    wsb = _norm_workspace(code, S, V, 0 if offsets is None else 1, C, groups, 1)
+    _, _, _, dn, dv = _channel_rows(dy.shape, dy.stride(), samples, "dy")
+    mean = _side(mean, "mean", x, _f32, (S, groups), optional=False)
+    rstd = _side(rstd, "rstd", x, _f32, (S, groups), optional=False)
+    dev = x.device
+    dx = torch.empty_strided(x.shape, dense, dtype=x.dtype, device=dev)
+    dw = torch.empty(C, dtype=_f32, device=dev) if weight is not None else None
+    db = torch.empty(C, dtype=_f32, device=dev) if bias is not None else None
     ws = _workspace(wsb, x)
-    _norm_check(lib().sis3d_group_norm_backward(_at(dy), dn, dv, _at(x), code, S, V, _at(offsets), sn, sv, C, groups, _at(mean), _at(rstd),
-                                                _at(weight), _at(bias), _ACTS[act], _at(dx), V * C, C, _at(dw), _at(db), _at(ws), wsb,
-                                                _raw_stream(x)), "sis3d_group_norm_backward", C, groups)
+    rc = lib().sis3d_group_norm_backward(dy.data_ptr(), dn, dv, x.data_ptr(), code, S, V, _at(offsets), sn, sv, C, groups, mean.data_ptr(),
+                                         rstd.data_ptr(), _at(weight), _at(bias), actc, dx.data_ptr(), V * C, C, _at(dw), _at(db), _at(ws), wsb,
+                                         _raw_stream(x))
+    if rc:
+        _norm_check(rc, "sis3d_group_norm_backward", C, groups)
     return dx, dw, db
 
 
 @_functools.lru_cache(maxsize=1024)
-def _score_rows_of(shape, st):
+def _score_plan(dtype, shape, st, top):
+    """(type, shape of the rows, outer count, rows, classes, three element strides, the same three of a dense tensor with the classes where
+    they are in score -- last in memory, or second --, its strides, workspace bytes) of (R,K) or (N,K,*spatial) class scores"""
+    code = _elem_code(dtype, "score")
     if len(shape) < 2:
         raise _lib.Sis3dError("score must be (rows, classes) or (N, classes, ...)")
     K = shape[1]
     if K < 1:
         raise _lib.Sis3dError("score must have at least one class")
-    if len(shape) == 2:
-        N, V, sn, sv, rows = 1, shape[0], 0, st[0], shape[:1]
-    else:
-        N, sn, rows = shape[0], st[0], shape[:1] + shape[2:]
+
+    def walk(st):
+        if len(shape) == 2:
+            return 1, shape[0], 0, st[0], st[1] if K > 1 else 1
         V = 1
         for n in shape[2:]:
             V *= n
         sv = _one_stride(shape[2:], st[2:])
         if sv is None:
             raise _lib.Sis3dError("score: the dimensions behind the classes must be dense among themselves, got strides %s" % (st,))
-    sc = st[1] if K > 1 else 1
+        return shape[0], V, st[0], sv, st[1] if K > 1 else 1
+
+    N, V, sn, sv, sc = walk(st)
     if K > 1024 and sc != 1:
         raise Sis3dUnsupported("score: more than 1024 classes must be contiguous in memory (class stride %d)" % sc)
-    return rows, N, V, K, sn, sv, sc
-
-
-def _score_rows(score):
-    """(type, shape of the rows, outer count, rows, classes, three element strides) of (R,K) or (N,K,*spatial) class scores"""
-    return (_elem(score, "score"),) + _score_rows_of(tuple(score.shape), score.stride())
-
-
-@_functools.lru_cache(maxsize=1024)
-def _class_workspace(rows, K, sc, top):
-    return lib().sis3d_class_rows_workspace_bytes(rows, K, sc, top)
+    rows = tuple(shape[:1]) + tuple(shape[2:])
+    if sc == 1 and K > 1:
+        dense = _last_second(shape)
+    elif len(shape) == 2:
+        dense = (1, shape[0]) if sc != 1 else (K, 1)
+    else:
+        dense = tuple(torch.empty(shape, device="meta").stride())
+    _, _, dn, dv, dc = walk(dense)
+    return code, rows, N, V, K, sn, sv, sc, dn, dv, dc, dense, lib().sis3d_class_rows_workspace_bytes(N * V, K, sc, top)
 
 
 def _num_rows(num, like):
@@ -1871,17 +1882,6 @@ def _num_rows(num, like):
     if num.numel() != 1:
         raise _lib.Sis3dError("num must hold one int32: the live rows")
     return _side(num, "num", like, torch.int32, num.shape)
-
-
-def _like_score(score, sc):
-    """an uninitialised dense tensor of score's shape with the classes where they are in score: last in memory, or second"""
-    n, dev = score.dim(), score.device
-    shape = tuple(score.shape)
-    if n == 2:
-        return torch.empty(shape, dtype=score.dtype, device=dev) if sc == 1 else torch.empty(shape[::-1], dtype=score.dtype, device=dev).t()
-    if sc == 1 and shape[1] > 1:
-        return torch.empty(shape[:1] + shape[2:] + shape[1:2], dtype=score.dtype, device=dev).permute(0, n - 1, *range(1, n - 1))
-    return torch.empty(shape, dtype=score.dtype, device=dev)
 
 
 @_on_device
@@ -1893,19 +1893,22 @@ def class_logprobs(score, labels, top=0, num=None):
     -> (logp, entropy, norm, top_logp, top_class): logp / entropy fp32 like labels; norm (...,2) for the backward pass (a row's
     largest score m and the sum s of exp(score - m): m + log s is the row's log-sum-exp); top_logp fp32 / top_class int64
     (...,top), best first, the lowest class first among equal scores; top <= min(32, K)."""
-    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    _gpu(score, "score")
     top = int(top)
+    code, rows, N, V, K, sn, sv, sc, _, _, _, _, wsb = _score_plan(score.dtype, score.shape, score.stride(), top)
     if not 0 <= top <= min(32, K):
         raise _lib.Sis3dError("class_logprobs: top must be 0 to %d, got %d" % (min(32, K), top))
-    labels = _side(labels, "labels", score, torch.int64, rows, optional=False)
+    labels = _side(labels, "labels", score, _i64, rows, optional=False)
     num = _num_rows(num, score)
     dev = score.device
-    logp, ent, norm, tl = (torch.empty(rows + tail, dtype=torch.float32, device=dev) for tail in ((), (), (2,), (top,)))
-    tc = torch.empty(rows + (top,), dtype=torch.int64, device=dev)
-    wsb = _class_workspace(N * V, K, sc, top)
+    logp, ent = torch.empty(rows, dtype=_f32, device=dev), torch.empty(rows, dtype=_f32, device=dev)
+    norm, tl = torch.empty(rows + (2,), dtype=_f32, device=dev), torch.empty(rows + (top,), dtype=_f32, device=dev)
+    tc = torch.empty(rows + (top,), dtype=_i64, device=dev)
     ws = _workspace(wsb, score)
-    check(lib().sis3d_class_logprobs_forward(_at(score), code, N, V, K, sn, sv, sc, _at(labels), _at(num), top, _at(logp), _at(ent),
-                                             _at(norm), _at(tl), _at(tc), _at(ws), wsb, _raw_stream(score)), "sis3d_class_logprobs_forward")
+    rc = lib().sis3d_class_logprobs_forward(score.data_ptr(), code, N, V, K, sn, sv, sc, labels.data_ptr(), _at(num), top, logp.data_ptr(),
+                                            ent.data_ptr(), norm.data_ptr(), tl.data_ptr(), tc.data_ptr(), _at(ws), wsb, _raw_stream(score))
+    if rc:
+        check(rc, "sis3d_class_logprobs_forward")
     return logp, ent, norm, tl, tc
 
 
@@ -1913,30 +1916,31 @@ def class_logprobs(score, labels, top=0, num=None):
 def class_logprobs_backward(score, labels, norm, entropy, grad_logp, grad_entropy=None, num=None):
     """gradient of class_logprobs with respect to the scores, in the scores' type and layout (sis3d_class_logprobs_backward);
     grad_logp / grad_entropy fp32 like labels"""
-    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
-    labels = _side(labels, "labels", score, torch.int64, rows, optional=False)
-    norm = _side(norm, "norm", score, torch.float32, rows + (2,), optional=False)
-    entropy = _side(entropy, "entropy", score, torch.float32, rows, optional=False)
-    grad_logp = _side(grad_logp, "grad_logp", score, torch.float32, rows, optional=False)
-    grad_entropy = _side(grad_entropy, "grad_entropy", score, torch.float32, rows)
+    _gpu(score, "score")
+    code, rows, N, V, K, sn, sv, sc, dn, dv, dc, dense, _ = _score_plan(score.dtype, score.shape, score.stride(), 0)
+    labels = _side(labels, "labels", score, _i64, rows, optional=False)
+    norm = _side(norm, "norm", score, _f32, rows + (2,), optional=False)
+    entropy = _side(entropy, "entropy", score, _f32, rows, optional=False)
+    grad_logp = _side(grad_logp, "grad_logp", score, _f32, rows, optional=False)
+    grad_entropy = _side(grad_entropy, "grad_entropy", score, _f32, rows)
     num = _num_rows(num, score)
-    d = _like_score(score, sc)
-    _, _, _, _, _, dn, dv, dc = _score_rows(d)
-    check(lib().sis3d_class_logprobs_backward(_at(score), code, N, V, K, sn, sv, sc, _at(labels), _at(num), _at(norm), _at(entropy),
-                                              _at(grad_logp), _at(grad_entropy), _at(d), dn, dv, dc, _raw_stream(score)),
-          "sis3d_class_logprobs_backward")
+    d = torch.empty_strided(score.shape, dense, dtype=score.dtype, device=score.device)
+    rc = lib().sis3d_class_logprobs_backward(score.data_ptr(), code, N, V, K, sn, sv, sc, labels.data_ptr(), _at(num), norm.data_ptr(),
+                                             entropy.data_ptr(), grad_logp.data_ptr(), _at(grad_entropy), d.data_ptr(), dn, dv, dc,
+                                             _raw_stream(score))
+    if rc:
+        check(rc, "sis3d_class_logprobs_backward")
     return d
 
 
 def _teacher(score, kept, classes, rows, temperature):
     if not isinstance(kept, torch.Tensor) or kept.dim() != len(rows) + 1 or not 1 <= kept.shape[-1] <= 128:
-        raise _lib.Sis3dError("kept must be %s + (1 to 128 logits,)" % (tuple(rows),))
+        raise _lib.Sis3dError("kept must be %s + (1 to 128 logits,)" % (rows,))
     shape = rows + (kept.shape[-1],)
     temperature = float(temperature)
     if not 1e-3 <= temperature <= 1e3:
         raise _lib.Sis3dError("temperature must be within 1e-3 and 1e3, got %r" % temperature)
-    return (_side(kept, "kept", score, torch.float32, shape, optional=False), _side(classes, "classes", score, torch.int64, shape, optional=False),
-            temperature)
+    return _side(kept, "kept", score, _f32, shape, optional=False), _side(classes, "classes", score, _i64, shape, optional=False), temperature
 
 
 @_on_device
@@ -1947,14 +1951,17 @@ def distill_loss(score, kept, classes, temperature=1.0, num=None):
     int64; negative = absent, equal classes add up), k <= 128.  The teacher's distribution is the softmax of kept / T over the entries
     that are present, the student's the softmax of score / T over all classes; a row without entries has loss 0.
     -> (loss fp32 (R,) / (N,*spatial), norm for the backward pass)."""
-    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    _gpu(score, "score")
+    code, rows, N, V, K, sn, sv, sc, _, _, _, _, wsb = _score_plan(score.dtype, score.shape, score.stride(), 0)
     kept, classes, temperature = _teacher(score, kept, classes, rows, temperature)
     num = _num_rows(num, score)
-    loss, norm = (torch.empty(rows + tail, dtype=torch.float32, device=score.device) for tail in ((), (2,)))
-    wsb = _class_workspace(N * V, K, sc, 0)
+    dev = score.device
+    loss, norm = torch.empty(rows, dtype=_f32, device=dev), torch.empty(rows + (2,), dtype=_f32, device=dev)
     ws = _workspace(wsb, score)
-    check(lib().sis3d_distill_forward(_at(score), code, N, V, K, sn, sv, sc, _at(kept), _at(classes), kept.shape[-1], _at(num), temperature,
-                                      _at(loss), _at(norm), _at(ws), wsb, _raw_stream(score)), "sis3d_distill_forward")
+    rc = lib().sis3d_distill_forward(score.data_ptr(), code, N, V, K, sn, sv, sc, kept.data_ptr(), classes.data_ptr(), kept.shape[-1], _at(num),
+                                     temperature, loss.data_ptr(), norm.data_ptr(), _at(ws), wsb, _raw_stream(score))
+    if rc:
+        check(rc, "sis3d_distill_forward")
     return loss, norm
 
 
@@ -1962,13 +1969,15 @@ def distill_loss(score, kept, classes, temperature=1.0, num=None):
 def distill_loss_backward(score, kept, classes, norm, grad_loss, temperature=1.0, num=None):
     """gradient of distill_loss with respect to the scores, in the scores' type and layout (sis3d_distill_backward); grad_loss fp32
     like the loss"""
-    code, rows, N, V, K, sn, sv, sc = _score_rows(score)
+    _gpu(score, "score")
+    code, rows, N, V, K, sn, sv, sc, dn, dv, dc, dense, _ = _score_plan(score.dtype, score.shape, score.stride(), 0)
     kept, classes, temperature = _teacher(score, kept, classes, rows, temperature)
-    norm = _side(norm, "norm", score, torch.float32, rows + (2,), optional=False)
-    grad_loss = _side(grad_loss, "grad_loss", score, torch.float32, rows, optional=False)
+    norm = _side(norm, "norm", score, _f32, rows + (2,), optional=False)
+    grad_loss = _side(grad_loss, "grad_loss", score, _f32, rows, optional=False)
     num = _num_rows(num, score)
-    d = _like_score(score, sc)
-    _, _, _, _, _, dn, dv, dc = _score_rows(d)
-    check(lib().sis3d_distill_backward(_at(score), code, N, V, K, sn, sv, sc, _at(kept), _at(classes), kept.shape[-1], _at(num), temperature,
-                                       _at(norm), _at(grad_loss), _at(d), dn, dv, dc, _raw_stream(score)), "sis3d_distill_backward")
+    d = torch.empty_strided(score.shape, dense, dtype=score.dtype, device=score.device)
+    rc = lib().sis3d_distill_backward(score.data_ptr(), code, N, V, K, sn, sv, sc, kept.data_ptr(), classes.data_ptr(), kept.shape[-1], _at(num),
+                                      temperature, norm.data_ptr(), grad_loss.data_ptr(), d.data_ptr(), dn, dv, dc, _raw_stream(score))
+    if rc:
+        check(rc, "sis3d_distill_backward")
     return d
