@@ -237,9 +237,8 @@ __device__ inline float log_p(float l, Norm n, float inv, float inv_lo)
     return n.ls == -INFINITY ? -INFINITY : fmaf(d, inv, fmaf(fmaxf(d, LOWEST), inv_lo, -n.ls));
 }
 
-__device__ inline float label_logp(const RowArgs &a, int64_t r, float ly, Norm n)
+__device__ inline float label_logp(const RowArgs &a, int64_t y, float ly, Norm n)
 {
-    const int64_t y = a.labels[r];
     return y < 0 ? 0.f : (y >= a.K ? NAN : log_p(ly, n, 1.f, 0.f));
 }
 
@@ -402,7 +401,7 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     }
     if (g.sub == 0 && g.in) {
         const int64_t y = a.labels[g.at];
-        a.logp[g.r] = g.live ? label_logp(a, g.r, y >= 0 && y < a.K ? sis3d_f32(p[y * a.s_c]) : 0.f, norm) : 0.f;
+        a.logp[g.r] = g.live ? label_logp(a, y, y >= 0 && y < a.K ? sis3d_f32(p[y * a.s_c]) : 0.f, norm) : 0.f;
         a.entropy[g.r] = g.live ? so.entropy() : 0.f;
         a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
     }
@@ -557,7 +556,7 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     static constexpr int NL = 64 * W, ROOM = 256, VEC = 16 / sizeof(T), UL = loads_of(NL);
     struct Vec { float m; int v; };            // a vector and its largest score
     struct Shared {
-        uint64_t cand[W][ROOM], bound[W];      // a wave's elements
+        uint64_t cand[TOP ? W : 1][TOP ? ROOM : 1], bound[W];       // a wave's elements
         Vec vecs[TOP ? W : 1][TOP ? ROOM : 1]; // and the vectors they are in
         float red[W][5];
         int lanes[W][64], count[W], total;
@@ -854,30 +853,38 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     }
 };
 
-// A row's kept entries in the lanes of a wave, at most two a lane: asked for before the row is read, used behind it
+// A row's kept entries in the lanes of a wave, at most two a lane.  Loads return in the order in which they were asked for: first the
+// entries, then the row's vectors, then the scores of the entries' classes, which need wait for the entries alone.
 struct Kept {
     float x[2], l[2];                          // teacher's logit, student's score; -inf: no such entry
     int c[2];                                  // class, -1: none
+    int64_t k[2];
     bool bad;
-    template <typename T> __device__ Kept(const RowArgs &a, int64_t r, const T *row, bool on = true) : bad(false)
+    __device__ Kept(const RowArgs &a, int64_t r, bool on = true) : bad(false)
     {
-        const int nk = on ? a.nk : 0;
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, nk = on ? a.nk : 0;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int i = lane + 64 * j;
             x[j] = -INFINITY;
-            l[j] = 0.f;
+            k[j] = -1;
+            if (lane + 64 * j < nk) {
+                k[j] = a.cls[r * a.nk + lane + 64 * j];
+                x[j] = a.kept[r * a.nk + lane + 64 * j];
+            }
+        }
+    }
+    template <typename T> __device__ void scores(const RowArgs &a, const T *row)
+    {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
             c[j] = -1;
-            if (j * 64 >= nk) break;
-            if (i >= nk) continue;
-            const int64_t k = a.cls[r * a.nk + i];
-            const float v = a.kept[r * a.nk + i];
-            if (k < 0) continue;
-            x[j] = v;
-            if (k >= a.K || v != v) { bad = true; continue; }
-            c[j] = (int)k;
-            l[j] = sis3d_f32(row[k]);
+            l[j] = 0.f;
+            if (k[j] < 0) x[j] = -INFINITY;
+            else if (k[j] >= a.K || x[j] != x[j]) bad = true;
+            else {
+                c[j] = (int)k[j];
+                l[j] = sis3d_f32(row[k[j]]);
+            }
         }
     }
     __device__ Teacher teacher(const RowArgs &a) const
@@ -909,10 +916,18 @@ template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t
     }
 }
 
-template <typename T> __device__ inline void row_outputs(const RowArgs &a, int64_t r, const T *row, const Soft<true> &so, Norm norm)
+// A row's label and, behind the row's vectors, its score
+struct Label {
+    int64_t y;
+    float l;
+    __device__ Label() : y(-1), l(0.f) {}
+    __device__ Label(const RowArgs &a, int64_t r) : y(a.labels[r]), l(0.f) {}
+    template <typename T> __device__ void score(const RowArgs &a, const T *row) { l = y >= 0 && y < a.K ? sis3d_f32(row[y]) : 0.f; }
+};
+
+__device__ inline void row_outputs(const RowArgs &a, int64_t r, const Label &label, const Soft<true> &so, Norm norm)
 {
-    const int64_t y = a.labels[r];
-    a.logp[r] = label_logp(a, r, y >= 0 && y < a.K ? sis3d_f32(row[y]) : 0.f, norm);
+    a.logp[r] = label_logp(a, label.y, label.l, norm);
     a.entropy[r] = so.entropy();
     a.norm[r] = make_float2(so.m, so.s);
 }
@@ -942,17 +957,21 @@ template <typename T, int W, int MODE, bool TOP> __global__ __launch_bounds__(25
     if (r >= live_rows(a)) { zero_row<MODE>(a, r, L::lane(), L::NL); return; }
     const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
     const Span<T> sp(row, 0, a.K);
-    Stream<T, L::NL, !TOP> st(sp, L::lane());
     typename L::Noted nt;
     if constexpr (MODE == KD) {
         const bool first = W == 1 || threadIdx.x < 64;
-        const Kept kept(a, r, row, first);
+        Kept kept(a, r, first);
+        Stream<T, L::NL, !TOP> st(sp, L::lane());
+        kept.scores(a, row);
         const auto so = L::pass(a, sp, st, sh, nt);
         if (first) wave_loss<T>(a, r, kept, so);
     } else {
+        Label label(a, r);
+        Stream<T, L::NL, !TOP> st(sp, L::lane());
+        label.score(a, row);
         const auto so = L::pass(a, sp, st, sh, nt);
         const Norm norm{so.m, so.log_s()};
-        if (L::lane() == 0) row_outputs(a, r, row, so, norm);
+        if (L::lane() == 0) row_outputs(a, r, label, so, norm);
         if constexpr (TOP)
             L::alternatives(a, sp, sh, nt, [&](int rank, uint64_t k) {
                 a.top_class[r * a.top + rank] = key_class(k);
@@ -997,9 +1016,13 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join
     so.join_wave(a.c2);
     const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
-        wave_loss<T>(a, r, Kept(a, r, row), so);
+        Kept kept(a, r);
+        kept.scores(a, row);
+        wave_loss<T>(a, r, kept, so);
     } else {
-        if (lane == 0) row_outputs(a, r, row, so, norm);
+        Label label(a, r);
+        label.score(a, row);
+        if (lane == 0) row_outputs(a, r, label, so, norm);
         if (!a.top) return;
         // a part's last alternative bounds the row's from below: only keys that reach the largest of these bounds are ranked
         const uint64_t *keys = a.part_keys + (size_t)r * a.parts * a.top;
@@ -1026,8 +1049,8 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join
 template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void long_backward(RowArgs a)
 {
     constexpr int NL = 64 * W, VEC = 16 / sizeof(T), UL = loads_of(NL);
-    __shared__ float q_s[4 / W][KEPT_MAX];
-    __shared__ int c_s[4 / W][KEPT_MAX];
+    __shared__ float q_s[4 / W][MODE == KD ? KEPT_MAX : 1], l_s[4 / W][MODE == KD ? KEPT_MAX : 1];
+    __shared__ int c_s[4 / W][MODE == KD ? KEPT_MAX : 1];
     const int team = team_of<W>(), lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
     const int64_t item = (int64_t)blockIdx.x * (4 / W) + team, r = a.parts == 1 ? item : item / a.parts;
     if (r >= a.R) return;
@@ -1044,23 +1067,29 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
         return;
     }
     const Span<T> sp(row, k0, k1);
-    Stream<T, NL, true> st(sp, lane);
-    const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : 0.f;
     Back<MODE> k;
     int y = -1;
+    float ly = 0.f;
+    const float2 norm = a.norm_in[r];
+    const float g1 = a.g1[r];
+    const Label label = MODE == LP ? Label(a, r) : Label();
+    Kept kept(a, r, MODE == KD);
+    Stream<T, NL, true> st(sp, lane);
+    const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : 0.f;
     if constexpr (MODE == LP) {
-        const int64_t label = a.labels[r];
-        k.scores(a.norm_in[r], a.entropy_in[r], label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[r]), a.g2 ? a.g2[r] : 0.f);
-        y = label >= k0 && label < k1 ? (int)label : -1;
+        y = label.y >= k0 && label.y < k1 ? (int)label.y : -1;
+        if (y >= 0) ly = sis3d_f32(row[y]);
+        k.scores(norm, a.entropy_in[r], label.y < 0 ? 0.f : (label.y >= a.K ? NAN : g1), a.g2 ? a.g2[r] : 0.f);
     } else {
-        const Kept kept(a, r, row);
+        kept.scores(a, row);
         const Teacher t = kept.teacher(a);
-        k.loss(a.norm_in[r], t.bad ? NAN : (t.any ? a.g1[r] * a.tau : 0.f), a.c2);
+        k.loss(norm, t.bad ? NAN : (t.any ? g1 * a.tau : 0.f), a.c2);
         if (W == 1 || threadIdx.x < 64)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 c_s[team][lane + 64 * j] = kept.c[j];
                 q_s[team][lane + 64 * j] = t.any ? exp2_((kept.x[j] - t.m) * a.c2) * rcp_(t.s) : 0.f;
+                l_s[team][lane + 64 * j] = kept.l[j];
             }
     }
     const bool wide = ((uintptr_t)(out + k0 + sp.head) & 15) == 0;
@@ -1088,7 +1117,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     // is kept twice is written by its first entry with the sum of both.
     team_sync<W>();
     if constexpr (MODE == LP) {
-        if (lane == 0 && y >= 0) out[y] = sis3d_from_f32<T>(k.exact(sis3d_f32(row[y])) + k.ga);
+        if (lane == 0 && y >= 0) out[y] = sis3d_from_f32<T>(k.exact(ly) + k.ga);
     } else {
         for (int i = lane; i < a.nk; i += NL) {
             const int c = c_s[team][i];
@@ -1100,7 +1129,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
                     q += q_s[team][j];
                     first = first && j >= i;
                 }
-            if (first) out[c] = sis3d_from_f32<T>(k.exact(sis3d_f32(row[c])) - k.ga * q);
+            if (first) out[c] = sis3d_from_f32<T>(k.exact(l_s[team][i]) - k.ga * q);
         }
     }
 }
