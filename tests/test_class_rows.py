@@ -147,7 +147,7 @@ def check_logprobs(l, labels, ga, ge, top, dtype, how="rows", N=1, num=None):
     return logp, h, norm, tl, tc, d
 
 
-KS = [1, 2, 3, 19, 41, 64, 65, 257, 1000, 1024, 1025, 1203, 4095, 4096, 4097, 8192, 20011, 65536]
+KS = [1, 2, 3, 19, 41, 64, 65, 257, 272, 273, 528, 529, 537, 1000, 1024, 1025, 1203, 4095, 4096, 4097, 8192, 20011, 65536]
 
 
 @pytest.mark.gpu
@@ -188,7 +188,7 @@ def special_rows(K, device="cuda"):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("K", [2, 19, 64, 1000, 1025, 4096, 5000, 20011])
+@pytest.mark.parametrize("K", [2, 19, 64, 300, 530, 1000, 1025, 4096, 5000, 20011])
 def test_masked_tied_and_extreme_rows(K):
     l = special_rows(K)
     R = l.shape[0]
