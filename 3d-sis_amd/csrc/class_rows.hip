@@ -53,6 +53,8 @@ struct RowArgs {
     const float2 *norm_in;
     const float *entropy_in;
     int lpr_log, planar, parts;
+    int g_log, sk, chunk;                      // tiles: lanes per row, floats of a row in LDS, classes of a lane
+    uint32_t per4;                             // 2^32 / (K / 4), rounded up
     float *part;                               // [R * parts][4]
     uint64_t *part_keys;                       // [R * parts][top]
 };
@@ -193,11 +195,13 @@ template <bool ENT> struct Soft {
 };
 
 // The same sums for one lane of a long row, x = l c2 - M in one fused operation (its rounding is that of x; one of M would be common to all
-// classes and cancels).  M, in units of x, need only be near the largest: it follows it when it is exceeded by more than 2.  Scores
-// whose product with c2 leaves the range of a float end in sums of 0, inf or NaN: such rows are taken again by exact_row.
+// classes and cancels).  M, in units of x, need only be near the largest: it follows it when it is exceeded by more than 2.  It starts at
+// -NEAR: scores that far below 0 (masks) add 0.  Where the largest lies outside +-NEAR the rounding of M itself is no longer small in x; such
+// rows, masked ones and those that are not finite end in a sum of 0, inf or NaN and are taken again class by class.
+constexpr float NEAR = 4194304.f;          // 2^22: M is rounded by at most 1/4
 template <bool ENT> struct Lane {
     float M, s, t;
-    __device__ void init() { M = -3e38f; s = t = 0.f; }
+    __device__ void init() { M = -NEAR; s = t = 0.f; }
     __device__ void raise(float to)
     {
         const float x = M - to, f = exp2_(x);
@@ -220,11 +224,11 @@ template <bool ENT> struct Lane {
     __device__ Soft<ENT> join_wave(float largest, float c2)
     {
         const float m = fmaxf(wave_max(largest), LOWEST);
-        raise(mul_rounded(m, c2));
+        raise(fmaxf(mul_rounded(m, c2), -NEAR));
         s = wave_sum(s);
         if constexpr (ENT) t = wave_sum(t);
         const float x = fmaf(m, c2, -M), e = exp2_(x);
-        return Soft<ENT>{m, s / e, ENT ? fmaf(-x, s, t) / e : 0.f};
+        return Soft<ENT>{m, M < NEAR ? s / e : NAN, ENT ? fmaf(-x, s, t) / e : 0.f};
     }
 };
 
@@ -247,14 +251,14 @@ __device__ inline float label_logp(const RowArgs &a, int64_t y, float ly, Norm n
 //     log probabilities   -p (ga + ge (log p + H)) = 2^x (k1 max(x, -288) + k0),  x = (l - m) log2(e)
 //     distillation        ga p = 2^x k0,  x = (l - m) log2(e) / T
 // (p is 0 from x = -288 on, and 0 * inf is not wanted; a row of nothing but -inf has 1 / s = 0).  `near` takes x from one fused operation
-// with M = m c2 rounded, whose rounding is taken out of k0 and k1 beforehand; `exact` serves rows whose m c2 leaves the range.
+// with M = m c2 rounded, whose rounding is taken out of k0 and k1 beforehand; `exact` serves rows where that is not small.
 template <int MODE> struct Back {
     float m, ga, k0, k1, c2, M, n0, n1;
     bool in_range;
     __device__ void finish()
     {
         M = mul_rounded(m, c2);
-        in_range = fabsf(M) < 1e37f;
+        in_range = fabsf(M) < NEAR;
         const float off = fmaf(m, c2, -M), f = exp2_(-off);        // l c2 - M = x + off
         n1 = MODE == LP ? k1 * f : 0.f;
         n0 = MODE == LP ? f * fmaf(-k1, off, k0) : f * k0;
@@ -363,12 +367,12 @@ __device__ inline float entry_loss(const RowArgs &a, const Teacher &t, float ls,
     return q != 0.f ? q * (x * LN2 - ls - log_p(l, norm, a.inv, a.inv_lo)) : 0.f;
 }
 
-template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void small_forward(RowArgs a)
+template <typename T, int E> __global__ __launch_bounds__(256) void small_forward(RowArgs a)
 {
     const Group g = group_of(a);
     const T *p = (const T *)a.score + row_at(a, g.at, a.s_n, a.s_v);
     float v[E];
-    Soft<MODE == LP> so;
+    Soft<true> so;
     so.init();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -383,23 +387,6 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     so.s = group_sum(so.s, g);
     so.t = group_sum(so.t, g);
     const Norm norm{so.m, so.log_s()};
-    if constexpr (MODE == KD) {
-        const Teacher t = group_teacher(a, g);
-        float loss = 0.f;
-        if (t.any && g.live) {
-            const float ls = log_(t.s);
-            for (int i = g.sub; i < a.nk; i += g.lpr) {
-                const int64_t c = a.cls[g.at * a.nk + i];
-                if (entry(a, c) == 1) loss += entry_loss(a, t, ls, a.kept[g.at * a.nk + i], sis3d_f32(p[c * a.s_c]), norm);
-            }
-        }
-        loss = a.tau * a.tau * group_sum(loss, g);
-        if (g.sub == 0 && g.in) {
-            a.loss[g.r] = !g.live ? 0.f : (t.bad ? NAN : loss);
-            a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
-        }
-        return;
-    }
     if (g.sub == 0 && g.in) {
         const int64_t y = a.labels[g.at];
         a.logp[g.r] = g.live ? label_logp(a, y, y >= 0 && y < a.K ? sis3d_f32(p[y * a.s_c]) : 0.f, norm) : 0.f;
@@ -426,43 +413,6 @@ template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void sm
     }
 }
 
-template <typename T, int E, int MODE> __global__ __launch_bounds__(256) void small_backward(RowArgs a)
-{
-    const Group g = group_of(a);
-    const T *p = (const T *)a.score + row_at(a, g.at, a.s_n, a.s_v);
-    T *d = (T *)a.dscore + row_at(a, g.in ? g.r : 0, a.d_n, a.d_v);
-    float q[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = 0.f;
-    Back<MODE> k;
-    if constexpr (MODE == LP) {
-        const int64_t y = a.labels[g.at];
-        k.scores(a.norm_in[g.at], a.entropy_in[g.at], y < 0 ? 0.f : (y >= a.K ? NAN : a.g1[g.at]), a.g2 ? a.g2[g.at] : 0.f);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (g.sub + e * g.lpr == y) q[e] = k.ga;
-    } else {
-        const Teacher t = group_teacher(a, g);
-        k.loss(a.norm_in[g.at], t.bad ? NAN : (t.any ? a.g1[g.at] * a.tau : 0.f), a.c2);
-        if (t.any)
-            for (int i = 0; i < a.nk; ++i) {
-                const int64_t c = a.cls[g.at * a.nk + i];
-                const float w = entry(a, c) == 1 ? exp2_((a.kept[g.at * a.nk + i] - t.m) * a.c2) * rcp_(t.s) : 0.f;
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (g.sub + e * g.lpr == c) q[e] -= w * k.ga;
-            }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = g.sub + e * g.lpr;
-        if (c >= a.K || !g.in) continue;
-        d[c * a.d_c] = sis3d_from_f32<T>(g.live ? k.exact(sis3d_f32(p[c * a.s_c])) + q[e] : 0.f);
-    }
-}
-
-// ---------------------------------------------------------------------------- long rows, classes contiguous --
-// A team of W waves (1: four teams to a workgroup; 4: the workgroup) has a row or a part of one.
 template <int W> __device__ inline int team_of() { return W == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0; }
 template <int W> __device__ inline void team_sync()
 {
@@ -472,6 +422,303 @@ template <int W> __device__ inline void team_sync()
     } else __syncthreads();
 }
 
+// ------------------------------------------------------------------------- short rows: a lane, or a few, to a row --
+// A workgroup has 256 / G rows.  Dense rows are one run of memory: it is read by vectors into LDS, as floats, and G neighbouring lanes take
+// a row from there, a stretch of classes each -- no shuffle within a stretch, and with G = 1 none at all.  Scores in any other layout are
+// read in place, neighbouring lanes having neighbouring rows.  The gradient of a dense tile is made in LDS and leaves as it came.
+// LDS rows are K floats apart where K is no multiple of 4 (banks differ from row to row by themselves), else an odd number of fours.
+struct TileRow {
+    Group g;
+    int row, lo, n;                            // row of the tile; this lane's classes are lo .. lo + n - 1
+};
+constexpr int IN_PLACE = 0, BY_ONE = 1, BY_FOUR = 2;
+
+template <int HOW> __device__ inline TileRow tile_row(const RowArgs &a)
+{
+    TileRow t;
+    const int G = 1 << a.g_log, rpw_log = 6 - a.g_log, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    t.g.lpr = G;
+    if (HOW == IN_PLACE && a.planar) {
+        t.row = (w << rpw_log) + (lane & ((1 << rpw_log) - 1));
+        t.g.sub = lane >> rpw_log;
+        t.g.step = 1 << rpw_log;
+    } else {
+        t.row = threadIdx.x >> a.g_log;
+        t.g.sub = lane & (G - 1);
+        t.g.step = 1;
+    }
+    t.g.r = (int64_t)blockIdx.x * (256 >> a.g_log) + t.row;
+    t.g.in = t.g.r < a.R;
+    t.g.live = t.g.in && t.g.r < live_rows(a);
+    t.g.at = t.g.live ? t.g.r : 0;
+    t.lo = t.g.sub * a.chunk;
+    t.n = t.g.live ? max(0, min(a.chunk, a.K - t.lo)) : 0;
+    return t;
+}
+
+// rows of the tile that are live, times K, between memory and LDS
+template <typename T, int HOW, bool IN> __device__ inline void move_tile(const RowArgs &a, T *mem, float *lds)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    const int rb = 256 >> a.g_log;
+    const int64_t r0 = (int64_t)blockIdx.x * rb, left = (IN ? live_rows(a) : a.R) - r0;
+    const int total = left <= 0 ? 0 : (int)(left < rb ? left : rb) * a.K;
+    mem += r0 * a.K;
+    auto place = [&](int i) {                      // of the float with number i, a multiple of 4
+        if constexpr (HOW == BY_ONE) return i;
+        const int row = __umulhi((uint32_t)i >> 2, a.per4);
+        return i + row * (a.sk - a.K);
+    };
+    for (int i = threadIdx.x * VEC; i < total; i += 256 * VEC) {
+        float x[VEC];
+        if (i + VEC <= total) {
+            if constexpr (IN) {
+                sis3d_unpack<T, VEC>(sis3d_load_once<T, VEC>(mem + i), x);
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) *(float4 *)(lds + place(i + j)) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) *(float4 *)(x + j) = *(const float4 *)(lds + place(i + j));
+                sis3d_store<T, VEC>(mem + i, x);
+            }
+        } else
+            for (int j = 0; i + j < total; ++j) {
+                const int at = place((i + j) & ~3) + ((i + j) & 3);
+                if constexpr (IN) lds[at] = sis3d_f32(mem[i + j]);
+                else mem[i + j] = sis3d_from_f32<T>(lds[at]);
+            }
+    }
+    __syncthreads();
+}
+
+// A lane's classes, eight at a time: f(first class, x[8], how many of them there are)
+template <typename T, int HOW, typename F> __device__ inline void each_eight(const RowArgs &a, const TileRow &t, const T *p, const float *row, F f)
+{
+    const int all = a.K - (((1 << a.g_log) - 1) * a.chunk);        // classes that every lane of a row has
+    for (int i = 0; i < a.chunk; i += 8) {
+        float x[8];
+        const bool whole = i + 8 <= all;
+        if constexpr (HOW == IN_PLACE) {
+            if (t.n > i) {
+                const T *q = p + (t.lo + i) * a.s_c;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = sis3d_f32(q[min(j, t.n - 1 - i) * a.s_c]);
+            }
+        } else if constexpr (HOW == BY_FOUR) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) *(float4 *)(x + j) = *(const float4 *)(row + t.lo + i + j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = row[t.lo + i + j];
+        }
+        if (!whole || !t.g.live)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = i + j < t.n ? x[j] : -INFINITY;
+        f(i, x);
+    }
+}
+
+template <typename T, int MODE, int HOW, int TK> __global__ __launch_bounds__(256) void tile_forward(RowArgs a)
+{
+    extern __shared__ float4 lds4[];
+    float *lds = (float *)lds4;
+    const TileRow t = tile_row<HOW>(a);
+    const Group &g = t.g;
+    const T *p = (const T *)a.score + (HOW == IN_PLACE ? row_at(a, g.at, a.s_n, a.s_v) : 0);
+    const float *row = lds + t.row * a.sk;
+    if constexpr (HOW != IN_PLACE) move_tile<T, HOW, true>(a, (T *)a.score, lds);
+    auto score = [&](int64_t c) { return HOW == IN_PLACE ? sis3d_f32(p[c * a.s_c]) : row[c]; };
+    Lane<MODE == LP> ln;
+    ln.init();
+    float best = -INFINITY, tv[TK ? TK : 1];
+    int tc[TK ? TK : 1];
+#pragma unroll
+    for (int k = 0; k < TK; ++k) {
+        tv[k] = -INFINITY;
+        tc[k] = -1;
+    }
+    each_eight<T, HOW>(a, t, p, row, [&](int i, const float (&x)[8]) {
+        const float top = max_of(x);
+        best = fmaxf(best, top);
+        ln.follow(top, a.c2);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ln.add(x[j], a.c2);
+        if constexpr (TK > 0)
+            if (top > tv[TK - 1])
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {          // behind equal ones, which have the lower classes
+                    float v = x[j];
+                    int c = t.lo + i + j;
+                    bool before = false;               // from its place on, all go one place down
+#pragma unroll
+                    for (int k = 0; k < TK; ++k) {
+                        before = before || v > tv[k];
+                        const float v2 = before ? tv[k] : v;
+                        const int c2 = before ? tc[k] : c;
+                        tv[k] = before ? v : tv[k];
+                        tc[k] = before ? c : tc[k];
+                        v = v2;
+                        c = c2;
+                    }
+                }
+    });
+    // the lanes of a row, relative to its largest score, which has s = 1 if it is the only one
+    Soft<MODE == LP> so;
+    so.m = fmaxf(group_max(best, g), LOWEST);
+    ln.raise(fmaxf(mul_rounded(so.m, a.c2), -NEAR));
+    const float x0 = fmaf(so.m, a.c2, -ln.M), e0 = exp2_(x0);
+    so.s = group_sum(ln.s, g);
+    so.t = MODE == LP ? group_sum(ln.t, g) : 0.f;
+    so.t = fmaf(-x0, so.s, so.t) / e0;
+    so.s = so.s / e0;
+    if (!(so.s > 0.f && so.s < INFINITY && ln.M < NEAR)) {
+        so.init();
+        for (int i = 0; i < t.n; ++i) so.m = fmaxf(so.m, score(t.lo + i));
+        so.m = group_max(so.m, g);
+        for (int i = 0; i < t.n; ++i) so.add(score(t.lo + i), a.c2);
+        so.s = group_sum(so.s, g);
+        so.t = group_sum(so.t, g);
+    }
+    const Norm norm{so.m, so.log_s()};
+    if constexpr (MODE == KD) {
+        const Teacher te = group_teacher(a, g);
+        float loss = 0.f;
+        if (te.any && g.live) {
+            const float ls = log_(te.s);
+            for (int i = g.sub; i < a.nk; i += g.lpr) {
+                const int64_t c = a.cls[g.at * a.nk + i];
+                if (entry(a, c) == 1) loss += entry_loss(a, te, ls, a.kept[g.at * a.nk + i], score(c), norm);
+            }
+        }
+        loss = a.tau * a.tau * group_sum(loss, g);
+        if (g.sub == 0 && g.in) {
+            a.loss[g.r] = !g.live ? 0.f : (te.bad ? NAN : loss);
+            a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
+        }
+        return;
+    }
+    if (g.sub == 0 && g.in) {
+        const int64_t y = g.live ? a.labels[g.at] : -1;
+        a.logp[g.r] = label_logp(a, y, y >= 0 && y < a.K ? score(y) : 0.f, norm);
+        a.entropy[g.r] = g.live ? so.entropy() : 0.f;
+        a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
+    }
+    if constexpr (TK > 0) {
+        int none = 0;                                  // next class to look at for one that ranks last: -inf or NaN
+        for (int i = 0; i < a.top; ++i) {
+            // the best of the lanes' first ones; its lane goes on to the next
+            float v = tv[0];
+            int c = tc[0];
+            for (int o = g.lpr >> 1; o > 0; o >>= 1) {
+                const float v2 = __shfl_xor(v, o * g.step);
+                const int c2 = __shfl_xor(c, o * g.step);
+                const bool other = v2 > v || (v2 == v && (uint32_t)c2 < (uint32_t)c);
+                v = other ? v2 : v;
+                c = other ? c2 : c;
+            }
+            if (c >= 0 && c == tc[0]) {
+#pragma unroll
+                for (int k = 0; k + 1 < TK; ++k) {
+                    tv[k] = tv[k + 1];
+                    tc[k] = tc[k + 1];
+                }
+                tv[TK - 1] = -INFINITY;
+                tc[TK - 1] = -1;
+            }
+            if (g.sub == 0 && g.in) {
+                if (g.live && c < 0) {
+                    while (none < a.K - 1 && score(none) > -INFINITY) ++none;
+                    c = none++;
+                    v = c < a.K ? score(c) : -INFINITY;
+                }
+                a.top_class[g.r * a.top + i] = g.live ? c : 0;
+                a.top_logp[g.r * a.top + i] = g.live ? log_p(v, norm, 1.f, 0.f) : 0.f;
+            }
+        }
+    }
+}
+
+template <typename T, int MODE, int HOW> __global__ __launch_bounds__(256) void tile_backward(RowArgs a)
+{
+    extern __shared__ float4 lds4[];
+    float *lds = (float *)lds4;
+    const TileRow t = tile_row<HOW>(a);
+    const Group &g = t.g;
+    const T *p = (const T *)a.score + (HOW == IN_PLACE ? row_at(a, g.at, a.s_n, a.s_v) : 0);
+    T *d = (T *)a.dscore + (HOW == IN_PLACE ? row_at(a, g.in ? g.r : 0, a.d_n, a.d_v) : 0);
+    float *row = lds + t.row * a.sk;
+    if constexpr (HOW != IN_PLACE) move_tile<T, HOW, true>(a, (T *)a.score, lds);
+    Back<MODE> k;
+    Teacher te;
+    int y = -1;
+    if constexpr (MODE == LP) {
+        const int64_t label = a.labels[g.at];
+        k.scores(a.norm_in[g.at], a.entropy_in[g.at], label < 0 ? 0.f : (label >= a.K ? NAN : a.g1[g.at]), a.g2 ? a.g2[g.at] : 0.f);
+        if (g.live && label >= 0 && label < a.K) y = (int)label;
+    } else {
+        te = group_teacher(a, g);
+        k.loss(a.norm_in[g.at], te.bad ? NAN : (te.any ? a.g1[g.at] * a.tau : 0.f), a.c2);
+    }
+    if constexpr (HOW == IN_PLACE) {
+        auto grad = [&](int c) {
+            const float l = sis3d_f32(p[c * a.s_c]);
+            return k.in_range ? k.near(l) : k.exact(l);
+        };
+        if (g.live)
+            each_eight<T, HOW>(a, t, p, row, [&](int i, const float (&x)[8]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (i + j < t.n) d[(t.lo + i + j) * a.d_c] = sis3d_from_f32<T>(k.in_range ? k.near(x[j]) : k.exact(x[j]));
+            });
+        else if (g.in)
+            for (int i = 0; i < max(0, min(a.chunk, a.K - t.lo)); ++i) d[(t.lo + i) * a.d_c] = sis3d_from_f32<T>(0.f);
+        // the label's class, or the kept ones, again by the lane that has written it
+        if constexpr (MODE == LP) {
+            if (y >= t.lo && y < t.lo + t.n) d[y * a.d_c] = sis3d_from_f32<T>(grad(y) + k.ga);
+        } else if (g.live && te.any) {
+            const int64_t *cls = a.cls + g.at * a.nk;
+            const float *kept = a.kept + g.at * a.nk;
+            for (int i = 0; i < a.nk; ++i) {
+                const int64_t c = cls[i];
+                if (c < t.lo || c >= t.lo + t.n) continue;
+                float q = 0.f;
+                bool first = true;
+                for (int j = 0; j < a.nk; ++j)
+                    if (cls[j] == c) {
+                        q += exp2_((kept[j] - te.m) * a.c2) * rcp_(te.s);
+                        first = first && j >= i;
+                    }
+                if (first) d[c * a.d_c] = sis3d_from_f32<T>(grad((int)c) - k.ga * q);
+            }
+        }
+    } else {
+        if (g.live) {
+            // the lane's stretch in place, then the label's or the teacher's share by the row's first lane: the same wave, in that order
+            float *mine = row + t.lo;
+            if (k.in_range) {
+#pragma unroll 4
+                for (int i = 0; i < t.n; ++i) mine[i] = k.near(mine[i]);
+            } else
+                for (int i = 0; i < t.n; ++i) mine[i] = k.exact(mine[i]);
+        } else if (g.in)
+            for (int i = 0; i < max(0, min(a.chunk, a.K - t.lo)); ++i) row[t.lo + i] = 0.f;
+        team_sync<1>();
+        if (g.sub == 0) {
+            if constexpr (MODE == LP) {
+                if (y >= 0) row[y] += k.ga;
+            } else if (g.live && te.any)
+                for (int i = 0; i < a.nk; ++i) {
+                    const int64_t c = a.cls[g.at * a.nk + i];
+                    if (entry(a, c) == 1) row[c] -= k.ga * (exp2_((a.kept[g.at * a.nk + i] - te.m) * a.c2) * rcp_(te.s));
+                }
+        }
+        __syncthreads();
+        move_tile<T, HOW, false>(a, (T *)a.dscore, lds);
+    }
+}
+
+// ---------------------------------------------------------------------------- long rows, classes contiguous --
+// A team of W waves (1: four teams to a workgroup; 4: the workgroup) has a row or a part of one.
 // [k0, k1) of a row: elements in front of the first 16-byte boundary and behind the last whole vector are taken one by one
 template <typename T> struct Span {
     static constexpr int VEC = 16 / sizeof(T);
@@ -1148,23 +1395,64 @@ int parts_of(int64_t R, int K, int64_t s_c)
     return (int)(p > 64 ? 64 : (p < 1 ? 1 : p));
 }
 
+// a wave to a row rather than a workgroup: up to 4096 classes, or 1024 vectors where there are rows enough (10000 x 5000 fp16, three
+// alternatives: 1.6 TB/s by workgroups)
+bool wave_rows(const RowArgs &a, int es) { return a.parts == 1 && (a.K <= K_WAVE || (a.K <= 16384 / es && a.R >= 4096)); }
+
+// how a tile's rows are had, its lanes per row and its LDS; LDS for dense, aligned rows of at most 24 floats a lane
+template <typename T> int plan_tile(RowArgs &a, bool backward)
+{
+    const bool dense = a.s_c == 1 && a.s_v == a.K && (a.N == 1 || a.s_n == a.V * a.K) && ((uintptr_t)a.score & 15) == 0 &&
+                       (!backward || (a.d_c == 1 && a.d_v == a.K && (a.N == 1 || a.d_n == a.V * a.K) && ((uintptr_t)a.dscore & 15) == 0));
+    const int how = !dense ? IN_PLACE : a.K % 4 ? BY_ONE : BY_FOUR;
+    a.sk = how == BY_FOUR ? ((a.K / 4) | 1) * 4 : a.K;
+    a.per4 = how == BY_FOUR ? (uint32_t)((((uint64_t)1 << 32) + a.K / 4 - 1) / (a.K / 4)) : 0;
+    a.g_log = 0;
+    if (dense || !a.planar)
+        while (a.g_log < 5 && 24 << a.g_log < a.K) ++a.g_log;
+    // more lanes to a row while there are CUs without a workgroup
+    while (a.g_log < 4 && 8 << a.g_log < a.K && (a.R << a.g_log) < 256 * 256) ++a.g_log;
+    a.chunk = (a.K + (1 << a.g_log) - 1) >> a.g_log;
+    if (how == BY_FOUR) a.chunk = (a.chunk + 3) / 4 * 4;
+    return how;
+}
+size_t tile_lds(const RowArgs &a, int how) { return how == IN_PLACE ? 0 : ((size_t)(256 >> a.g_log) * a.sk + ((size_t)a.chunk << a.g_log) + 16) * sizeof(float); }
+
+template <typename T, int MODE, int TK> void tile_launch(RowArgs &a, int how, hipStream_t st)
+{
+    const int rb = 256 >> a.g_log;
+    const dim3 grid((unsigned)((a.R + rb - 1) / rb)), block(256);
+    const size_t lds = tile_lds(a, how);
+    if (how == IN_PLACE) hipLaunchKernelGGL((tile_forward<T, MODE, IN_PLACE, TK>), grid, block, lds, st, a);
+    else if (how == BY_ONE) hipLaunchKernelGGL((tile_forward<T, MODE, BY_ONE, TK>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((tile_forward<T, MODE, BY_FOUR, TK>), grid, block, lds, st, a);
+}
+
 template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
 {
     if (is_short(a.K, a.s_c, sizeof(T))) {
-        const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
-        const dim3 grid((unsigned)((waves + 3) / 4));
-        const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
-        if (e <= 2) hipLaunchKernelGGL((small_forward<T, 2, MODE>), grid, dim3(256), 0, st, a);
-        else if (e <= 4) hipLaunchKernelGGL((small_forward<T, 4, MODE>), grid, dim3(256), 0, st, a);
-        else if (e <= 8) hipLaunchKernelGGL((small_forward<T, 8, MODE>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((small_forward<T, 16, MODE>), grid, dim3(256), 0, st, a);
+        if (a.top > 4) {                               // lists of a lane get long: a row in the registers of a group, `top` maxima of it
+            const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
+            const dim3 grid((unsigned)((waves + 3) / 4));
+            const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
+            if constexpr (MODE == LP) {
+                if (e <= 8) hipLaunchKernelGGL((small_forward<T, 8>), grid, dim3(256), 0, st, a);
+                else hipLaunchKernelGGL((small_forward<T, 16>), grid, dim3(256), 0, st, a);
+            }
+            return sis3d_check_launch();
+        }
+        const int how = plan_tile<T>(a, false);
+        if (MODE == KD || a.top == 0) tile_launch<T, MODE, 0>(a, how, st);
+        else if (a.top == 1) tile_launch<T, LP, 1>(a, how, st);
+        else tile_launch<T, LP, 4>(a, how, st);
         return sis3d_check_launch();
     }
-    const dim3 block(256), each(a.parts > 1 ? (unsigned)(a.R * a.parts) : a.K <= K_WAVE ? (unsigned)((a.R + 3) / 4) : (unsigned)a.R);
+    const bool by_wave = wave_rows(a, sizeof(T));
+    const dim3 block(256), each(a.parts > 1 ? (unsigned)(a.R * a.parts) : by_wave ? (unsigned)((a.R + 3) / 4) : (unsigned)a.R);
     auto launch = [&](auto top) {
         constexpr bool TOP = decltype(top)::value && MODE == LP;
         if (a.parts > 1) hipLaunchKernelGGL((split_forward<T, MODE, TOP>), each, block, 0, st, a);
-        else if (a.K <= K_WAVE) hipLaunchKernelGGL((long_forward<T, 1, MODE, TOP>), each, block, 0, st, a);
+        else if (by_wave) hipLaunchKernelGGL((long_forward<T, 1, MODE, TOP>), each, block, 0, st, a);
         else hipLaunchKernelGGL((long_forward<T, 4, MODE, TOP>), each, block, 0, st, a);
     };
     if (a.top) launch(Count<1>());
@@ -1177,17 +1465,16 @@ template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
 
 template <typename T, int MODE> int run_backward(RowArgs &a, hipStream_t st)
 {
-    if (is_short(a.K, a.s_c, sizeof(T))) {
-        const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
-        const dim3 grid((unsigned)((waves + 3) / 4));
-        const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
-        if (e <= 2) hipLaunchKernelGGL((small_backward<T, 2, MODE>), grid, dim3(256), 0, st, a);
-        else if (e <= 4) hipLaunchKernelGGL((small_backward<T, 4, MODE>), grid, dim3(256), 0, st, a);
-        else if (e <= 8) hipLaunchKernelGGL((small_backward<T, 8, MODE>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((small_backward<T, 16, MODE>), grid, dim3(256), 0, st, a);
+    if (is_short(a.K, a.s_c, sizeof(T)) || a.d_c != 1) {
+        const int how = plan_tile<T>(a, true), rb = 256 >> a.g_log;
+        const dim3 grid((unsigned)((a.R + rb - 1) / rb)), block(256);
+        const size_t lds = tile_lds(a, how);
+        if (how == IN_PLACE) hipLaunchKernelGGL((tile_backward<T, MODE, IN_PLACE>), grid, block, lds, st, a);
+        else if (how == BY_ONE) hipLaunchKernelGGL((tile_backward<T, MODE, BY_ONE>), grid, block, lds, st, a);
+        else hipLaunchKernelGGL((tile_backward<T, MODE, BY_FOUR>), grid, block, lds, st, a);
         return sis3d_check_launch();
     }
-    if (a.K <= K_WAVE) hipLaunchKernelGGL((long_backward<T, 1, MODE>), dim3((unsigned)((a.R + 3) / 4)), dim3(256), 0, st, a);
+    if (wave_rows(a, sizeof(T))) hipLaunchKernelGGL((long_backward<T, 1, MODE>), dim3((unsigned)((a.R + 3) / 4)), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((long_backward<T, 4, MODE>), dim3((unsigned)(a.R * a.parts)), dim3(256), 0, st, a);
     return sis3d_check_launch();
 }
