@@ -14,10 +14,10 @@
 // value come out as what they are (all classes alike).
 //
 // Three forms, by the number of classes:
-//   short rows       (contiguous: as long as 64 lanes would not have a vector each; class-strided: K <= 1024)  a group of 1 .. 64 lanes
-//                    holds a row in registers; class-strided (planar) scores give neighbouring rows to neighbouring lanes, contiguous
-//                    rows give neighbouring classes to them
-//   longer rows      a wave (K <= 4096) or a workgroup streams a row with 16-byte loads from its first aligned element on
+//   short rows       (contiguous: as long as 64 lanes would not have a vector each; class-strided: K <= 1024)  a lane, or up to 32 of them,
+//                    takes a row; contiguous rows come through LDS in vectors, class-strided (planar) scores are read in place, with
+//                    neighbouring rows on neighbouring lanes.  More than four alternatives: a row in the registers of 1 .. 64 lanes
+//   longer rows      a wave or a workgroup streams a row with 16-byte loads from its first aligned element on
 //   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
 //
 // Alternatives of a long row without sorting it or reading it twice: every lane knows the largest score it has seen.  The lanes of a wave
@@ -299,7 +299,7 @@ template <int MODE> struct Back {
 // a teacher's entry: 0 = absent, 1 = present, 2 = no such class
 __device__ inline int entry(const RowArgs &a, int64_t c) { return c < 0 ? 0 : (c >= a.K ? 2 : 1); }
 
-// ---------------------------------------------------------------- K <= 1024: a row in the registers of 1 .. 64 lanes --
+// ------------------------------------ short rows, more than four alternatives: a row in the registers of 1 .. 64 lanes --
 struct Group {
     int64_t r, at;                             // row; the row that may be read (0 where r is none: such lanes take part in the shuffles only)
     int sub, lpr, step;                        // lane of the row, lanes per row, distance of neighbouring row lanes
@@ -1383,6 +1383,9 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
 }
 
 // ------------------------------------------------------------------------------------------------------ host --
+// a launch has at most 2^32 - 1 threads
+bool too_many(int64_t workgroups) { return workgroups > 0xffffffffll / 256; }
+
 // 50000 x 1000 fp16, log probabilities: 0.81 TB/s as a short row, 2.5 TB/s as a longer one
 bool is_short(int K, int64_t s_c, int es) { return s_c != 1 ? K <= K_STRIDED : K <= 64 * (16 / es) + 16; }
 
@@ -1407,7 +1410,8 @@ template <typename T> int plan_tile(RowArgs &a, bool backward)
     const int how = !dense ? IN_PLACE : a.K % 4 ? BY_ONE : BY_FOUR;
     a.sk = how == BY_FOUR ? ((a.K / 4) | 1) * 4 : a.K;
     a.per4 = how == BY_FOUR ? (uint32_t)((((uint64_t)1 << 32) + a.K / 4 - 1) / (a.K / 4)) : 0;
-    a.g_log = 0;
+    // two lanes share the teacher's entries (1.3 million x 19 planar fp32, 4 entries: 0.89 TB/s by one lane, 1.59 by two, 1.45 by four)
+    a.g_log = a.nk > 1 && a.K > 1 && !backward ? 1 : 0;
     if (dense || !a.planar)
         while (a.g_log < 5 && 24 << a.g_log < a.K) ++a.g_log;
     // more lanes to a row while there are CUs without a workgroup
@@ -1433,6 +1437,7 @@ template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
     if (is_short(a.K, a.s_c, sizeof(T))) {
         if (a.top > 4) {                               // lists of a lane get long: a row in the registers of a group, `top` maxima of it
             const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
+            if (too_many((waves + 3) / 4)) return SIS3D_EUNSUPPORTED;
             const dim3 grid((unsigned)((waves + 3) / 4));
             const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
             if constexpr (MODE == LP) {
@@ -1442,13 +1447,16 @@ template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
             return sis3d_check_launch();
         }
         const int how = plan_tile<T>(a, false);
+        if (too_many((a.R + (256 >> a.g_log) - 1) / (256 >> a.g_log))) return SIS3D_EUNSUPPORTED;
         if (MODE == KD || a.top == 0) tile_launch<T, MODE, 0>(a, how, st);
         else if (a.top == 1) tile_launch<T, LP, 1>(a, how, st);
         else tile_launch<T, LP, 4>(a, how, st);
         return sis3d_check_launch();
     }
     const bool by_wave = wave_rows(a, sizeof(T));
-    const dim3 block(256), each(a.parts > 1 ? (unsigned)(a.R * a.parts) : by_wave ? (unsigned)((a.R + 3) / 4) : (unsigned)a.R);
+    const int64_t workgroups = by_wave ? (a.R + 3) / 4 : a.R * a.parts;
+    if (too_many(workgroups)) return SIS3D_EUNSUPPORTED;
+    const dim3 block(256), each((unsigned)workgroups);
     auto launch = [&](auto top) {
         constexpr bool TOP = decltype(top)::value && MODE == LP;
         if (a.parts > 1) hipLaunchKernelGGL((split_forward<T, MODE, TOP>), each, block, 0, st, a);
@@ -1467,6 +1475,7 @@ template <typename T, int MODE> int run_backward(RowArgs &a, hipStream_t st)
 {
     if (is_short(a.K, a.s_c, sizeof(T)) || a.d_c != 1) {
         const int how = plan_tile<T>(a, true), rb = 256 >> a.g_log;
+        if (too_many((a.R + rb - 1) / rb)) return SIS3D_EUNSUPPORTED;
         const dim3 grid((unsigned)((a.R + rb - 1) / rb)), block(256);
         const size_t lds = tile_lds(a, how);
         if (how == IN_PLACE) hipLaunchKernelGGL((tile_backward<T, MODE, IN_PLACE>), grid, block, lds, st, a);
@@ -1474,8 +1483,12 @@ template <typename T, int MODE> int run_backward(RowArgs &a, hipStream_t st)
         else hipLaunchKernelGGL((tile_backward<T, MODE, BY_FOUR>), grid, block, lds, st, a);
         return sis3d_check_launch();
     }
-    if (wave_rows(a, sizeof(T))) hipLaunchKernelGGL((long_backward<T, 1, MODE>), dim3((unsigned)((a.R + 3) / 4)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((long_backward<T, 4, MODE>), dim3((unsigned)(a.R * a.parts)), dim3(256), 0, st, a);
+    const bool by_wave = wave_rows(a, sizeof(T));
+    const int64_t workgroups = by_wave ? (a.R + 3) / 4 : a.R * a.parts;
+    if (too_many(workgroups)) return SIS3D_EUNSUPPORTED;
+    const dim3 each((unsigned)workgroups);
+    if (by_wave) hipLaunchKernelGGL((long_backward<T, 1, MODE>), each, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((long_backward<T, 4, MODE>), each, dim3(256), 0, st, a);
     return sis3d_check_launch();
 }
 

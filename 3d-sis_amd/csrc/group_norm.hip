@@ -15,7 +15,7 @@
 // workgroup numbers from  floor(off[s] / T) + s  on, which leaves it at least ceil(n_s / T) of them whatever the lengths are, so the grid
 // and the workspace depend on the row count and the number of samples alone and the call captures into a graph.
 //
-// Sums: a thread adds d = x - K and d^2 in 32 bits over its (at most a few hundred) rows, K its own first row, so a mean that is large
+// Sums: a thread adds d = x - K and d^2 in 32 bits over its rows (at most 2048, a few hundred mostly), K its own first row, so a mean that is large
 // against the deviation does not cancel; everything across threads is added in 64 bits.
 #include "elem.h"
 
@@ -165,6 +165,15 @@ template <typename P, typename F> __device__ inline void reduce_tiles(const P *p
 }
 
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2;
+
+// h w + b.  ReLU's slope is 0 or 1 by its sign, so it is taken there as written, the product rounded, and forward and backward take the same
+// steps: a row's gradient then passes exactly where its output does, and where it does when the formula is written out one operation a time.
+template <int ACT> __device__ inline float affine(float h, float w, float b)
+{
+#pragma clang fp contract(off)
+    if constexpr (ACT == ACT_RELU) return h * w + b;
+    else return __builtin_fmaf(h, w, b);
+}
 
 __device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }      // two units in the last place
 template <int ACT> __device__ inline float act(float z)
@@ -316,17 +325,18 @@ template <typename T, int VEC, int ACT, bool ONCE> struct Apply {
     }
     __device__ void run(const GnArgs &a, const Cols &k, const float *st, T *y)
     {
-        float mu[VEC];
+        float mu[VEC], rs[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             mu[i] = st[g.g[i]];
-            w[i] *= st[k.gl + g.g[i]];
+            rs[i] = st[k.gl + g.g[i]];
+            if constexpr (ACT != ACT_RELU) w[i] *= rs[i];
         }
         each_row(x, [&](int r, bool there, const SisVec<T, VEC> &v) {
             float o[VEC];
             sis3d_unpack<T, VEC>(v, o);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = act<ACT>(fmaf(o[i] - mu[i], w[i], b[i]));
+            for (int i = 0; i < VEC; ++i) o[i] = act<ACT>(affine<ACT>(ACT == ACT_RELU ? (o[i] - mu[i]) * rs[i] : o[i] - mu[i], w[i], b[i]));
             if (there) sis3d_store<T, VEC, ONCE>(y + r * a.y_v, o);
         });
     }
@@ -428,7 +438,7 @@ __device__ inline void tile_grad_sums(const GnArgs &a, const Cols &k, const Tile
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float h = (xf[i] - c.mu[i]) * c.rs[i];
-                const float e = df[i] * act_slope<ACT>(fmaf(h, c.w[i], c.b[i]));
+                const float e = df[i] * act_slope<ACT>(affine<ACT>(h, c.w[i], c.b[i]));
                 s0[i] += there ? e : 0.f;
                 s1[i] += there ? e * h : 0.f;
             }
@@ -486,7 +496,7 @@ template <typename T, int VEC, int ACT, bool ONCE> struct ApplyGrad {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float h = (o[i] - c.mu[i]) * c.rs[i];
-                const float e = df[i] * act_slope<ACT>(fmaf(h, c.w[i], c.b[i])) * c.w[i];
+                const float e = df[i] * act_slope<ACT>(affine<ACT>(h, c.w[i], c.b[i])) * c.w[i];
                 o[i] = c.rs[i] * (e - fmaf(h, m2[i], m1[i]));
             }
             if (there) sis3d_store<T, VEC, ONCE>(dx + r * a.y_v, o);
@@ -612,16 +622,17 @@ Plan make_plan(int dtype, int S, int64_t rows, int ragged, int C, int G, bool wi
         T = (total * p.ncol + blocks - 1) / blocks;
         const int rpb = (int)(NT / (p.gpb * cpg / p.vec));
         if (T < rpb) T = rpb;
+        if (T > 1024 * rpb) T = 1024 * rpb;                // rows of a thread, which adds them in 32 bits
     }
     if (T < 1) T = 1;                                      // no rows
-    if (T > (1 << 24)) T = 1 << 24;
     p.once = total * C * es > 16 << 20;                    // half of what the eight L2s hold
     p.t_log = 0;
     while (((int64_t)1 << p.t_log) < T) ++p.t_log;
     if (ragged) T = (int64_t)1 << p.t_log;                 // a shift in place of divisions by T
     p.T = (int)T;
     p.tiles = ragged ? (rows >> p.t_log) + S + 1 : S * ((rows + T - 1) / T);
-    if (p.tiles > 0x7fffff00 || p.ncol > 65535) p.rc = SIS3D_EUNSUPPORTED;
+    // a launch has at most 2^32 - 1 threads in one dimension and 65535 workgroups in the other
+    if (p.tiles + (C + 31) / 32 > 0xffffffffll / NT || p.ncol > 65535) p.rc = SIS3D_EUNSUPPORTED;
     return p;
 }
 

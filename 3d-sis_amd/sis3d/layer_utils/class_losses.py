@@ -8,7 +8,8 @@ from .. import ops
 
 class ClassLogProbs(torch.autograd.Function):
     """`ClassLogProbs.apply(score, labels, top, num)` -> (logp, entropy, top_logp, top_class); gradients reach score through logp and
-    entropy, the alternatives are reported and carry none."""
+    entropy, the alternatives are reported and carry none.  A training step may be captured into a graph as any of torch's: no eager
+    backward graph of the same parameters may be alive then."""
 
     @staticmethod
     def forward(ctx, score, labels, top=0, num=None):

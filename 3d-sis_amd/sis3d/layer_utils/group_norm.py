@@ -6,7 +6,9 @@ from .. import ops
 
 
 class GroupNormAct(torch.autograd.Function):
-    """`GroupNormAct.apply(x, weight, bias, groups, eps, act, offsets)` -> y: ops.group_norm with gradients for x, weight and bias."""
+    """`GroupNormAct.apply(x, weight, bias, groups, eps, act, offsets)` -> y: ops.group_norm with gradients for x, weight and bias.
+
+    A training step may be captured into a graph as any of torch's: no eager backward graph of the same parameters may be alive then."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps=1e-5, act=None, offsets=None):

@@ -1655,13 +1655,14 @@ _f32, _i64 = torch.float32, torch.int64
 
 
 def _on_device(fn):
-    """run on the device of the first tensor argument (and on that device's current stream), whatever the current device is"""
+    """run on the device of the first argument (and on that device's current stream), whatever the current device is"""
     @_functools.wraps(fn)
-    def call(x, *args, **kwargs):
+    def call(*args, **kwargs):
+        x = args[0] if args else next(iter(kwargs.values()), None)
         if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() != torch.cuda.current_device():
             with torch.cuda.device(x.device):
-                return fn(x, *args, **kwargs)
-        return fn(x, *args, **kwargs)
+                return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
     return call
 
 
@@ -1757,7 +1758,6 @@ def _norm_plan(dtype, shape, stride, samples, groups, act):
     backward) of a group norm"""
     code = _elem_code(dtype, "x")
     S, V, C, sn, sv = _channel_rows(shape, stride, samples, "x")
-    groups = int(groups)
     if groups < 1 or C < 1 or C % groups:
         raise _lib.Sis3dError("group norm: %d channels do not split into %d groups" % (C, groups))
     if act not in _ACTS:
@@ -1774,14 +1774,14 @@ def _norm_args(x, groups, weight, bias, act, offsets):
             raise _lib.Sis3dError("offsets must be (samples + 1,) row offsets")
         offsets = _side(offsets, "offsets", x, _i64, offsets.shape)
         samples = offsets.numel() - 1
-    plan = _norm_plan(x.dtype, x.shape, x.stride(), samples, groups, act)
+    plan = _norm_plan(x.dtype, x.shape, x.stride(), samples, int(groups), act if act is None else str(act))
     C = plan[3]
     return plan, samples, offsets, _side(weight, "weight", x, _f32, (C,)), _side(bias, "bias", x, _f32, (C,))
 
 
 def _norm_check(rc, what, C, groups):
     if rc == -4:
-        raise Sis3dUnsupported("%s: %d channels in %d groups are more than a workgroup takes" % (what, C, groups))
+        raise Sis3dUnsupported("%s: %d channels in %d groups, or so many samples, are more than a launch takes" % (what, C, groups))
     check(rc, what)
 
 
@@ -1879,7 +1879,7 @@ def _score_plan(dtype, shape, st, top):
 def _num_rows(num, like):
     if num is None:
         return None
-    if num.numel() != 1:
+    if not isinstance(num, torch.Tensor) or num.numel() != 1:
         raise _lib.Sis3dError("num must hold one int32: the live rows")
     return _side(num, "num", like, torch.int32, num.shape)
 

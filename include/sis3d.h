@@ -569,7 +569,7 @@ int sis3d_maxpool3d_3x3x3(const float *in, int X, int Y, int Z, int C, float *ou
  * Statistics: 32-bit sums of differences to a nearby value per thread, 64-bit across threads; no atomics, results do not vary.
  * backward also writes dweight / dbias [C] fp32 (each may be NULL), summed over all samples.  y may be x (in place); dx may be dy, not x.
  * SIS3D_EUNSUPPORTED: more than 512 * (16 bytes / element) channels per group (512 where a pointer, a stride or C is not a multiple of
- * 16 bytes).  workspace: 16-byte aligned, sis3d_group_norm_workspace_bytes (ragged: 0 / 1), any content. */
+ * 16 bytes), or more samples than a launch has workgroups (millions).  workspace: 16-byte aligned, sis3d_group_norm_workspace_bytes (ragged: 0 / 1), any content. */
 #define SIS3D_ACT_NONE 0
 #define SIS3D_ACT_RELU 1
 #define SIS3D_ACT_SILU 2
@@ -600,6 +600,8 @@ int sis3d_group_norm_backward(const void *dy, int64_t dy_sample, int64_t dy_row,
  *                                  [R][nkept] fp32 teacher logits of classes [R][nkept] int64, negative = absent, >= K makes the row NaN,
  *                                  equal classes add up; no present entry: loss 0.  nkept <= 128, 1e-3 <= T <= 1e3.
  *   sis3d_distill_backward         dscore = grad_loss T (p - q)
+ * dscore: score's type, strides of its own (d_c = 1 where K > 1024), not score's memory.  EUNSUPPORTED also for more rows than a launch
+ * has threads for (67 million of the longer ones).
  * workspace: 16-byte aligned, sis3d_class_rows_workspace_bytes(N * V, K, s_c, top) (0 for most calls; top = 0 for distillation). */
 size_t sis3d_class_rows_workspace_bytes(int64_t rows, int K, int64_t s_c, int top);
 int sis3d_class_logprobs_forward(const void *score, int dtype, int N, int64_t V, int K, int64_t s_n, int64_t s_v, int64_t s_c,

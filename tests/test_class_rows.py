@@ -454,6 +454,9 @@ def test_refusals():
             pytest.fail("refusal %d" % i)
     with pytest.raises(ops.Sis3dUnsupported):
         ops.class_logprobs(torch.zeros(1, 1025, 8, device="cuda"), torch.zeros(1, 8, dtype=torch.int64, device="cuda"))
+    with pytest.raises(_lib.Sis3dError):
+        ops.class_logprobs(l, labels, num=3)
+    assert torch.equal(ops.class_logprobs(labels=labels, score=l)[0], ops.class_logprobs(score=l, labels=labels)[0])
     # empty batches give empty outputs
     e = ops.class_logprobs(l[:0], labels[:0], top=2)
     assert e[0].shape == (0,) and e[4].shape == (0, 2)
@@ -486,6 +489,12 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
     e0 = dict(score=p, dtype=0, N=1, V=4, K=10, sn=0, sv=10, sc=1, kept=p, cls=p, nk=3, num=None, T=1.0, norm=p, g=p, d=p, dn=0, dv=10, dc=1, st=None)
     for k in (dict(nk=0), dict(T=0.0), dict(norm=None), dict(g=None), dict(d=None)):
         assert l.sis3d_distill_backward(*dict(e0, **k).values()) == -1, k
+    # more rows than a launch has threads for
+    many = dict(V=1 << 30, K=5000, sv=5000, top=0)
+    assert fwd(**many) == -4 and fwd(**dict(many, K=600)) == -4 and fwd(**dict(many, K=100, top=5)) == -4 and fwd(**dict(many, K=400)) == -4
+    many = dict(V=1 << 30, K=5000, sv=5000)
+    assert l.sis3d_class_logprobs_backward(*dict(b0, **many).values()) == -4 and l.sis3d_distill_backward(*dict(e0, **many, ).values()) == -4
+    assert l.sis3d_distill_backward(*dict(e0, **dict(many, K=400)).values()) == -4
     assert l.sis3d_class_rows_workspace_bytes(200, 19, 1, 3) == 0 and l.sis3d_class_rows_workspace_bytes(2, 65536, 1, 3) > 0
 
 

@@ -325,6 +325,24 @@ def test_more_than_two_to_the_31_elements():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dims,C,G", [((10, 9, 11), 32, 8), ((3, 2, 2), 12, 4), ((40, 33, 31), 64, 16)])
+def test_relu_passes_a_gradient_exactly_where_it_passes_a_value(dims, C, G):
+    """with dy = 1, dbias counts the elements whose gradient passes: whole numbers below 2^24, so no tolerance"""
+    from sis3d import ops
+    g = torch.Generator(device="cuda").manual_seed(C)
+    # few different values: many elements within rounding of 0 after the bias, on both sides
+    x = torch.randint(-3, 4, (2,) + dims + (C,), device="cuda", generator=g).float().permute(0, 4, 1, 2, 3)
+    w = 1 + torch.rand(C, device="cuda", generator=g)
+    b = torch.zeros(C, device="cuda")
+    for _ in range(2):
+        y, mean, rstd = ops.group_norm(x, G, w, b, act="relu", want_stats=True)
+        dx, dw, db = ops.group_norm_backward(torch.ones_like(x), x, mean, rstd, G, w, b, act="relu")
+        assert torch.equal(db, (y > 0).sum((0, 2, 3, 4)).float())
+        h = (1.0 - mean.view(2, G, 1)) * rstd.view(2, G, 1)                  # of the value 1: a bias that takes it to 0, but for a rounding
+        b = -(h.expand(2, G, C // G).reshape(2, C)[0] * w)
+
+
+@pytest.mark.gpu
 def test_autograd_module_and_differences():
     """HipGroupNorm in a training step: autograd's gradients are the operator's, and they are the slope of the loss"""
     from sis3d import ops
@@ -399,6 +417,11 @@ def test_refusals():
             pytest.fail("refusal %d" % i)
     with pytest.raises(ops.Sis3dUnsupported):
         ops.group_norm(torch.zeros(1, 4099, 2, device="cuda").permute(0, 2, 1).contiguous().permute(0, 2, 1), 1)
+    # keywords throughout; a group count that is a tensor counts by its value
+    n = torch.tensor(4)
+    y = ops.group_norm(x=x + torch.arange(32., device="cuda").view(1, 32, 1, 1, 1), groups=n)
+    n.fill_(32)
+    assert float(y.abs().max()) > 1 and float(ops.group_norm(x=x + torch.arange(32., device="cuda").view(1, 32, 1, 1, 1), groups=n).abs().max()) == 0
 
 
 def test_abi_refuses_bad_arguments_without_a_gpu():
@@ -425,6 +448,8 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
     for k in (dict(dtype=-1), dict(dy=None), dict(dx=None), dict(mean=None), dict(rstd=None), dict(G=3), dict(ws=None)):
         assert backward(**k) == -1, k
     assert backward(wsb=16) == -3 and backward(rows=0) == 0
+    # more samples than a launch has workgroups
+    assert forward(S=1 << 23, rows=1, wsb=1 << 50) == -4 and backward(S=1 << 23, rows=1, wsb=1 << 50) == -4
     assert l.sis3d_group_norm_workspace_bytes(0, 1, 10, 0, 32, 5, 0) == 0
     for ragged in (0, 1):
         for backward in (0, 1):
