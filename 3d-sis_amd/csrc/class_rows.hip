@@ -17,7 +17,8 @@
 //   short rows       (contiguous: as long as 64 lanes would not have a vector each; class-strided: K <= 1024)  a lane, or up to 32 of them,
 //                    takes a row; contiguous rows come through LDS in vectors, class-strided (planar) scores are read in place, with
 //                    neighbouring rows on neighbouring lanes.  More than four alternatives: a row in the registers of 1 .. 64 lanes
-//   longer rows      a wave or a workgroup streams a row with 16-byte loads from its first aligned element on
+//   longer rows      a wave or a workgroup streams a row with 16-byte loads from its first aligned element on; distillation of up to 4 KB
+//                    by 16 lanes, so that four rows share what is done once a row
 //   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
 //
 // Alternatives of a long row without sorting it or reading it twice: every lane knows the largest score it has seen.  The lanes of a wave
@@ -147,8 +148,25 @@ __device__ inline float wave_max(float v)
     return max3_(lane_at(v, 0), lane_at(v, 16), fmaxf(lane_at(v, 32), lane_at(v, 48)));
 }
 __device__ inline float wave_min(float v) { return -wave_max(-v); }
+// the same over 16 lanes: rotated and added, every lane gets the same bits
+__device__ inline float row_sum(float v)
+{
+    v += dpp<0x128, 0xf>(0.f, v);
+    v += dpp<0x124, 0xf>(0.f, v);
+    v += dpp<0x122, 0xf>(0.f, v);
+    return v + dpp<0x121, 0xf>(0.f, v);
+}
+__device__ inline float row_max(float v) { return max_ror<1>(max_ror<2>(max_ror<4>(max_ror<8>(v)))); }
+// of the L lanes that a row has
+template <int L> __device__ inline float lanes_sum(float v) { return L == 16 ? row_sum(v) : wave_sum(v); }
+template <int L> __device__ inline float lanes_max(float v) { return L == 16 ? row_max(v) : wave_max(v); }
+template <int L> __device__ inline bool lanes_any(bool v)
+{
+    const uint64_t mask = __ballot(v);
+    return L == 16 ? (mask >> (threadIdx.x & 48) & 0xffff) != 0 : mask != 0;
+}
 // the largest of the 2, 4, 8 or 16 neighbouring lanes that v's lane is one of: quads by permutation, then mirrored halves and rows
-__device__ inline float lanes_max(float v, int lanes)
+__device__ inline float neighbours_max(float v, int lanes)
 {
     v = fmaxf(v, dpp<0xb1, 0xf>(v, v));
     if (lanes >= 4) v = fmaxf(v, dpp<0x4e, 0xf>(v, v));
@@ -220,13 +238,13 @@ template <bool ENT> struct Lane {
         s += e;
         if constexpr (ENT) t = fmaf(fmaxf(x, -200.f), e, t);
     }
-    // all lanes of a wave, relative to its largest score m: divided by m's own term, so that a row of one class has s = 1 exactly
-    __device__ Soft<ENT> join_wave(float largest, float c2)
+    // L lanes, relative to their largest score m: divided by m's own term, so that a row of one class has s = 1 exactly
+    template <int L> __device__ Soft<ENT> join(float largest, float c2)
     {
-        const float m = fmaxf(wave_max(largest), LOWEST);
+        const float m = fmaxf(lanes_max<L>(largest), LOWEST);
         raise(fmaxf(mul_rounded(m, c2), -NEAR));
-        s = wave_sum(s);
-        if constexpr (ENT) t = wave_sum(t);
+        s = lanes_sum<L>(s);
+        if constexpr (ENT) t = lanes_sum<L>(t);
         const float x = fmaf(m, c2, -M), e = exp2_(x);
         return Soft<ENT>{m, M < NEAR ? s / e : NAN, ENT ? fmaf(-x, s, t) / e : 0.f};
     }
@@ -359,6 +377,24 @@ __device__ inline Teacher group_teacher(const RowArgs &a, const Group &g)
             if (entry(a, cls[i])) t.s += exp2_((kept[i] - t.m) * a.c2);
     t.s = group_sum(t.s, g);
     return t;
+}
+// Every entry of a row, in their order, to all lanes of the group: f(number, class or -1, q).  Each is read and its q made by one lane.
+template <typename F> __device__ inline void each_entry(const RowArgs &a, const Group &g, const Teacher &t, F f)
+{
+    const int first = g.step == 1 ? (threadIdx.x & 63) - g.sub : (threadIdx.x & (g.step - 1));      // the wave's lane with sub = 0
+    const float is = t.any ? rcp_(t.s) : 0.f;
+    for (int i0 = 0; i0 < a.nk; i0 += g.lpr) {
+        int c = -1;
+        float q = 0.f;
+        if (i0 + g.sub < a.nk) {
+            const int64_t k = a.cls[g.at * a.nk + i0 + g.sub];
+            if (entry(a, k) == 1) {
+                c = (int)k;
+                q = exp2_((a.kept[g.at * a.nk + i0 + g.sub] - t.m) * a.c2) * is;
+            }
+        }
+        for (int s = 0; s < g.lpr && i0 + s < a.nk; ++s) f(i0 + s, __shfl(c, first + s * g.step), __shfl(q, first + s * g.step));
+    }
 }
 // an entry's share of the loss; q log q is 0 at q = 0
 __device__ inline float entry_loss(const RowArgs &a, const Teacher &t, float ls, float kept, float l, Norm norm)
@@ -675,25 +711,22 @@ template <typename T, int MODE, int HOW> __global__ __launch_bounds__(256) void 
         // the label's class, or the kept ones, again by the lane that has written it
         if constexpr (MODE == LP) {
             if (y >= t.lo && y < t.lo + t.n) d[y * a.d_c] = sis3d_from_f32<T>(grad(y) + k.ga);
-        } else if (g.live && te.any) {
-            const int64_t *cls = a.cls + g.at * a.nk;
-            const float *kept = a.kept + g.at * a.nk;
-            for (int i = 0; i < a.nk; ++i) {
-                const int64_t c = cls[i];
-                if (c < t.lo || c >= t.lo + t.n) continue;
-                float q = 0.f;
-                bool first = true;
-                for (int j = 0; j < a.nk; ++j)
-                    if (cls[j] == c) {
-                        q += exp2_((kept[j] - te.m) * a.c2) * rcp_(te.s);
-                        first = first && j >= i;
-                    }
-                if (first) d[c * a.d_c] = sis3d_from_f32<T>(grad((int)c) - k.ga * q);
-            }
+        } else {
+            // a class that may have been kept before is written once more, with the sum so far; `seen` is of classes modulo 64
+            uint64_t seen = 0;
+            each_entry(a, g, te, [&](int i, int c, float q) {
+                if (!te.any || c < t.lo || c >= t.lo + t.n) return;
+                const uint64_t bit = 1ull << (c & 63);
+                if (seen & bit)
+                    for (int j = i - 1; j >= 0; --j)
+                        if (a.cls[g.at * a.nk + j] == c) q += exp2_((a.kept[g.at * a.nk + j] - te.m) * a.c2) * rcp_(te.s);
+                seen |= bit;
+                d[c * a.d_c] = sis3d_from_f32<T>(grad(c) - k.ga * q);
+            });
         }
     } else {
         if (g.live) {
-            // the lane's stretch in place, then the label's or the teacher's share by the row's first lane: the same wave, in that order
+            // the lane's stretch in place, then the label's or the teacher's share by the lane that has that class
             float *mine = row + t.lo;
             if (k.in_range) {
 #pragma unroll 4
@@ -702,16 +735,12 @@ template <typename T, int MODE, int HOW> __global__ __launch_bounds__(256) void 
                 for (int i = 0; i < t.n; ++i) mine[i] = k.exact(mine[i]);
         } else if (g.in)
             for (int i = 0; i < max(0, min(a.chunk, a.K - t.lo)); ++i) row[t.lo + i] = 0.f;
-        team_sync<1>();
-        if (g.sub == 0) {
-            if constexpr (MODE == LP) {
-                if (y >= 0) row[y] += k.ga;
-            } else if (g.live && te.any)
-                for (int i = 0; i < a.nk; ++i) {
-                    const int64_t c = a.cls[g.at * a.nk + i];
-                    if (entry(a, c) == 1) row[c] -= k.ga * (exp2_((a.kept[g.at * a.nk + i] - te.m) * a.c2) * rcp_(te.s));
-                }
-        }
+        if constexpr (MODE == LP) {
+            if (y >= t.lo && y < t.lo + t.n) row[y] += k.ga;
+        } else
+            each_entry(a, g, te, [&](int, int c, float q) {
+                if (te.any && c >= t.lo && c < t.lo + t.n) row[c] -= k.ga * q;
+            });
         __syncthreads();
         move_tile<T, HOW, false>(a, (T *)a.dscore, lds);
     }
@@ -742,15 +771,17 @@ template <typename T> struct Span {
 // A lane's vectors lane, lane + NL, ... of a span, UL at a time and the next UL on their way while these are worked on; the first are
 // asked for when the object is made, so that a row's other loads travel with them.  f(count, v, vectors): `count` of them from v on, all
 // there but perhaps the last one of the last batch.
-// UL: 4 where a workgroup has a row, 2 where a wave has a short one (40000 x 1203 fp16, distillation forward: 39.4 us with 4, 36.5 with 2)
+// UL: 4 where a workgroup has a row, 2 where fewer lanes have one (40000 x 1203 fp16, distillation forward, a wave to a row: 39.4 us with 4,
+// 36.5 with 2; 16 lanes to a row: 27.6 with 4, 24.1 with 2)
 constexpr int loads_of(int NL) { return NL > 64 ? 4 : 2; }
 template <int N> struct Count { static constexpr int value = N; };
 template <typename T, int NL, bool ONCE> struct Stream {
     static constexpr int VEC = 16 / sizeof(T), UL = loads_of(NL);
     const Span<T> &sp;
-    const int lane;
+    const int lane, steps;                                     // steps of NL vectors, the same for all lanes of a wave
     SisVec<T, VEC> raw[UL];
-    __device__ Stream(const Span<T> &s, int l) : sp(s), lane(l) { load(raw, l); }
+    __device__ Stream(const Span<T> &s, int l) : Stream(s, l, s.nvec) {}
+    __device__ Stream(const Span<T> &s, int l, int vectors) : sp(s), lane(l), steps((vectors + NL - 1) / NL) { load(raw, l); }
     __device__ void load(SisVec<T, VEC> (&r)[UL], int v) const
     {
 #pragma unroll
@@ -758,7 +789,7 @@ template <typename T, int NL, bool ONCE> struct Stream {
     }
     template <typename F> __device__ void each(F f)
     {
-        int v = lane, left = (sp.nvec + NL - 1) / NL;          // steps of NL vectors
+        int v = lane, left = steps;
         SisVec<T, VEC> next[UL];
         while (left > UL) {
             load(next, v + UL * NL);
@@ -774,7 +805,7 @@ template <typename T, int NL, bool ONCE> struct Stream {
     // the same with less code (one batch and one vector of it), for work that takes more instructions than a cache of them holds ten times
     template <typename F> __device__ void each_compact(F f)
     {
-        int v = lane, left = (sp.nvec + NL - 1) / NL;
+        int v = lane, left = steps;
         for (; left > UL; left -= UL, v += UL * NL) {
             SisVec<T, VEC> next[UL];
             load(next, v + UL * NL);
@@ -825,7 +856,7 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
             next = 1;
             over = false;
         }
-        __device__ void tighten() { b = fmaxf(b, wave_min(lanes_max(best, lanes))); }
+        __device__ void tighten() { b = fmaxf(b, wave_min(neighbours_max(best, lanes))); }
         // puts entries of the lanes that have one behind the list's others
         template <typename E> __device__ void note(E *list, bool there, E entry)
         {
@@ -921,9 +952,9 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
         float block = INFINITY;                 // a bound from all waves' groups together, a quarter as many of each
         if constexpr (TOP) {
             nt.tighten();
-            if (W > 1) block = wave_min(lanes_max(nt.best, a.top > 16 ? 8 : 16));
+            if (W > 1) block = wave_min(neighbours_max(nt.best, a.top > 16 ? 8 : 16));
         }
-        auto so = ln.join_wave(fmaxf(nt.best, edge), a.c2);
+        auto so = ln.template join<64>(fmaxf(nt.best, edge), a.c2);
         if constexpr (W > 1) {
             if ((threadIdx.x & 63) == 0) {
                 sh.red[threadIdx.x >> 6][0] = so.m;
@@ -1101,23 +1132,23 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     }
 };
 
-// A row's kept entries in the lanes of a wave, at most two a lane.  Loads return in the order in which they were asked for: first the
+// A row's kept entries in the L lanes that it has, at most two a lane.  Loads return in the order in which they were asked for: first the
 // entries, then the row's vectors, then the scores of the entries' classes, which need wait for the entries alone.
-struct Kept {
+template <int L> struct Kept {
     float x[2], l[2];                          // teacher's logit, student's score; -inf: no such entry
     int c[2];                                  // class, -1: none
     int64_t k[2];
     bool bad;
     __device__ Kept(const RowArgs &a, int64_t r, bool on = true) : bad(false)
     {
-        const int lane = threadIdx.x & 63, nk = on ? a.nk : 0;
+        const int lane = threadIdx.x & (L - 1), nk = on ? a.nk : 0;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             x[j] = -INFINITY;
             k[j] = -1;
-            if (lane + 64 * j < nk) {
-                k[j] = a.cls[r * a.nk + lane + 64 * j];
-                x[j] = a.kept[r * a.nk + lane + 64 * j];
+            if (lane + L * j < nk) {
+                k[j] = a.cls[r * a.nk + lane + L * j];
+                x[j] = a.kept[r * a.nk + lane + L * j];
             }
         }
     }
@@ -1138,15 +1169,15 @@ struct Kept {
     __device__ Teacher teacher(const RowArgs &a) const
     {
         Teacher t;
-        t.m = wave_max(fmaxf(x[0], x[1]));
-        t.bad = __any(bad);
+        t.m = lanes_max<L>(fmaxf(x[0], x[1]));
+        t.bad = lanes_any<L>(bad);
         t.any = t.m > -INFINITY;
-        t.s = t.any ? wave_sum(exp2_((x[0] - t.m) * a.c2) + exp2_((x[1] - t.m) * a.c2)) : 0.f;
+        t.s = t.any ? lanes_sum<L>(exp2_((x[0] - t.m) * a.c2) + exp2_((x[1] - t.m) * a.c2)) : 0.f;
         return t;
     }
 };
 
-template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t r, const Kept &kept, const Soft<false> &so)
+template <int L> __device__ inline void row_loss(const RowArgs &a, int64_t r, const Kept<L> &kept, const Soft<false> &so)
 {
     const Norm norm{so.m, so.log_s()};
     const Teacher t = kept.teacher(a);
@@ -1157,8 +1188,8 @@ template <typename T> __device__ inline void wave_loss(const RowArgs &a, int64_t
         for (int j = 0; j < 2; ++j)
             if (kept.c[j] >= 0) loss += entry_loss(a, t, ls, kept.x[j], kept.l[j], norm);
     }
-    loss = a.tau * a.tau * wave_sum(loss);
-    if ((threadIdx.x & 63) == 0) {
+    loss = a.tau * a.tau * lanes_sum<L>(loss);
+    if ((threadIdx.x & (L - 1)) == 0) {
         a.loss[r] = t.bad ? NAN : loss;
         a.norm[r] = make_float2(so.m, so.s);
     }
@@ -1208,11 +1239,11 @@ template <typename T, int W, int MODE, bool TOP> __global__ __launch_bounds__(25
     typename L::Noted nt;
     if constexpr (MODE == KD) {
         const bool first = W == 1 || threadIdx.x < 64;
-        Kept kept(a, r, first);
+        Kept<64> kept(a, r, first);
         Stream<T, L::NL, !TOP> st(sp, L::lane());
         kept.scores(a, row);
         const auto so = L::pass(a, sp, st, sh, nt);
-        if (first) wave_loss<T>(a, r, kept, so);
+        if (first) row_loss(a, r, kept, so);
     } else {
         Label label(a, r);
         Stream<T, L::NL, !TOP> st(sp, L::lane());
@@ -1226,6 +1257,57 @@ template <typename T, int W, int MODE, bool TOP> __global__ __launch_bounds__(25
                 a.top_logp[r * a.top + rank] = log_p(key_score(k), norm, 1.f, 0.f);
             });
     }
+}
+
+// Distillation of rows that are not so long: 16 lanes to a row, four rows to a wave, which share all that is done once a row
+template <typename T> __global__ __launch_bounds__(256) void four_distill(RowArgs a)
+{
+    constexpr int L = 16, VEC = 16 / sizeof(T), UL = loads_of(L);
+    const int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4, r = r0 + ((threadIdx.x & 63) >> 4), live = live_rows(a);
+    const int lane = threadIdx.x & (L - 1);
+    if (r >= live && r < a.R) zero_row<KD>(a, r, lane, L);
+    if (r0 >= live) return;                                    // the whole wave
+    const int64_t at = r < live ? r : live - 1;                // lanes of a row that is not there go over the last one and write nothing
+    const T *row = (const T *)a.score + row_at(a, at, a.s_n, a.s_v);
+    const Span<T> sp(row, 0, a.K);
+    Kept<L> kept(a, at);
+    Stream<T, L, true> st(sp, lane, a.K / VEC);
+    kept.scores(a, row);
+    const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : -INFINITY;
+    Lane<false> ln;
+    ln.init();
+    float best = edge;
+    st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
+        constexpr int N = decltype(count)::value;
+        const bool last = v + (N - 1) * L < sp.nvec;
+        float x[N][VEC], top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            sis3d_unpack<T, VEC>(raw[u], x[u]);
+            if (u == N - 1)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[u][i] = last ? x[u][i] : -INFINITY;
+            top = fmaxf(top, max_of(x[u]));
+        }
+        best = fmaxf(best, top);
+        ln.follow(top, a.c2);
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ln.add(x[u][i], a.c2);
+    });
+    ln.follow(edge, a.c2);
+    if (lane < sp.edges()) ln.add(edge, a.c2);
+    Soft<false> so = ln.join<L>(best, a.c2);
+    if (!(so.s > 0.f && so.s < INFINITY)) {                    // class by class, as exact_row; the same for the row's lanes
+        so.init();
+        for (int c = lane; c < a.K; c += L) so.m = fmaxf(so.m, sis3d_f32(row[c]));
+        so.m = row_max(so.m);
+        for (int c = lane; c < a.K; c += L) so.add(sis3d_f32(row[c]), a.c2);
+        so.s = row_sum(so.s);
+    }
+    const int64_t out = r < live ? r : a.R;
+    if (out < a.R) row_loss(a, out, kept, so);
 }
 
 // one part of a row to a workgroup
@@ -1264,9 +1346,9 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void split_join
     so.join_wave(a.c2);
     const Norm norm{so.m, so.log_s()};
     if constexpr (MODE == KD) {
-        Kept kept(a, r);
+        Kept<64> kept(a, r);
         kept.scores(a, row);
-        wave_loss<T>(a, r, kept, so);
+        row_loss(a, r, kept, so);
     } else {
         Label label(a, r);
         label.score(a, row);
@@ -1321,7 +1403,7 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     const float2 norm = a.norm_in[r];
     const float g1 = a.g1[r];
     const Label label = MODE == LP ? Label(a, r) : Label();
-    Kept kept(a, r, MODE == KD);
+    Kept<64> kept(a, r, MODE == KD);
     Stream<T, NL, true> st(sp, lane);
     const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : 0.f;
     if constexpr (MODE == LP) {
@@ -1402,6 +1484,11 @@ int parts_of(int64_t R, int K, int64_t s_c)
 // alternatives: 1.6 TB/s by workgroups)
 bool wave_rows(const RowArgs &a, int es) { return a.parts == 1 && (a.K <= K_WAVE || (a.K <= 16384 / es && a.R >= 4096)); }
 
+// distillation with 16 lanes to a row: rows of up to 4 KB, of 96 classes at least (tiles and waves against it, 8 entries, 100 MB:  fp32
+// x 64 31 / 41 us, x 100 41 / 32, x 300 38 / 23, x 1000 21 / 22;  fp16 x 100 61 / 56, x 300 52 / 31, x 600 46 / 23, x 1203 36 / 24, x 2000
+// 26 / 24, x 4000 23 / 25)
+bool four_rows(const RowArgs &a, int es) { return a.s_c == 1 && a.nk <= 32 && a.K >= 96 && a.K * es <= 4096 && a.R >= 16 * 256; }
+
 // how a tile's rows are had, its lanes per row and its LDS; LDS for dense, aligned rows of at most 24 floats a lane
 template <typename T> int plan_tile(RowArgs &a, bool backward)
 {
@@ -1410,8 +1497,11 @@ template <typename T> int plan_tile(RowArgs &a, bool backward)
     const int how = !dense ? IN_PLACE : a.K % 4 ? BY_ONE : BY_FOUR;
     a.sk = how == BY_FOUR ? ((a.K / 4) | 1) * 4 : a.K;
     a.per4 = how == BY_FOUR ? (uint32_t)((((uint64_t)1 << 32) + a.K / 4 - 1) / (a.K / 4)) : 0;
-    // two lanes share the teacher's entries (1.3 million x 19 planar fp32, 4 entries: 0.89 TB/s by one lane, 1.59 by two, 1.45 by four)
-    a.g_log = a.nk > 1 && a.K > 1 && !backward ? 1 : 0;
+    // a teacher's entries are shared by up to eight lanes, two or, where the row's gradient is made in LDS, four of them a lane.  Half a
+    // million x 41 fp32, planar, 16 entries: forward 361 us by two lanes, 147 by four, 100 by eight, backward 467, 262, 178; 32 entries:
+    // 183 / 196 us forward by eight / sixteen, 356 / 455 backward.  Rows, 16 entries, backward: 276 us by two, 81 by four, 93 by eight.
+    a.g_log = 0;
+    while (a.g_log < 3 && (backward && dense ? 4 : 2) << a.g_log < a.nk && 4 << a.g_log < a.K) ++a.g_log;
     if (dense || !a.planar)
         while (a.g_log < 5 && 24 << a.g_log < a.K) ++a.g_log;
     // more lanes to a row while there are CUs without a workgroup
@@ -1434,6 +1524,12 @@ template <typename T, int MODE, int TK> void tile_launch(RowArgs &a, int how, hi
 
 template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
 {
+    if constexpr (MODE == KD)
+        if (four_rows(a, sizeof(T))) {
+            if (too_many((a.R + 15) / 16)) return SIS3D_EUNSUPPORTED;
+            hipLaunchKernelGGL((four_distill<T>), dim3((unsigned)((a.R + 15) / 16)), dim3(256), 0, st, a);
+            return sis3d_check_launch();
+        }
     if (is_short(a.K, a.s_c, sizeof(T))) {
         if (a.top > 4) {                               // lists of a lane get long: a row in the registers of a group, `top` maxima of it
             const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);

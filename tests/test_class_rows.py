@@ -86,6 +86,9 @@ def ref_distill(l, kept, cls, T, g=None):
 
 def near(got, want, tol, dtype, name):
     got = got.double()
+    # a value beyond the largest 32-bit number rounds to infinity (the loss of a row whose student rules out, by the lowest fp32 score, what
+    # the teacher keeps: T^2 q 3.4e38 / T)
+    want = torch.where(want.abs() > torch.finfo(torch.float32).max, want * math.inf, want)
     same = (got == want) | (torch.isnan(got) & torch.isnan(want))
     bound = tol + (torch.finfo(dtype).eps / 2 * want.abs() if dtype else U * want.abs()) + (U if dtype == torch.float16 else 1e-37)
     bad = ~same & ~((got - want).abs() <= bound)
@@ -301,6 +304,48 @@ def test_distillation_edges(K):
     bd = ops.distill_loss_backward(l, bad_kept, bad_cls, bn, torch.ones(R, device="cuda"), 2.0)
     assert torch.isnan(bl[[0, 2]]).all() and torch.isnan(bd[[0, 2]]).all()
     assert torch.equal(bl[[1, 3, 5]], loss[[1, 3, 5]]) and torch.isfinite(bd[[1, 3, 5]]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how,K,k", [("rows", 5, 5), ("rows", 96, 6), ("rows", 97, 16), ("wide", 333, 32), ("rows", 1000, 17), ("rows", 1001, 33), ("rows", 2047, 8),
+                                     ("rows", 4100, 6), ("planar", 19, 16), ("planar", 41, 32), ("planar", 200, 70), ("transposed", 130, 9)])
+@pytest.mark.parametrize("dt", list(DT))
+def test_distillation_of_many_rows_with_edges(how, K, k, dt):
+    """more rows than there are lanes to take one each: masked rows, equal classes (and such that are equal modulo 64), absent and bad
+    entries beside ordinary rows, live rows that end inside a group of four"""
+    from sis3d import ops
+    R = 4099
+    l, _, _, _, g = make(R, K, DT[dt], seed=K)
+    kept = torch.randn(R, k, device="cuda", generator=g)
+    cls = torch.randint(0, K, (R, k), device="cuda", generator=g)
+    cls[0::11] = cls[0::11] % 64 + 64 * torch.randint(0, max(1, K // 64), (R, k), device="cuda", generator=g)[0::11]
+    cls = torch.where(cls < K, cls, 0)
+    cls[1::11] = -1                                                             # nothing kept
+    cls[2::11] = cls[2::11, :1]                                                 # one class, many times
+    cls[3::11, k // 2:] = -1
+    kept[4::11, 1:] = -math.inf                                                 # a teacher that allows one class
+    kept[5::11] = -math.inf                                                     # one that allows none
+    l[6::11] = -math.inf                                                        # a student row that allows nothing
+    l[7::11, 1:] = -math.inf
+    big = torch.finfo(DT[dt]).max
+    l[8::11] = -big                                                             # the type's lowest value throughout
+    l[9::11, ::2] = -big
+    l = l.contiguous()
+    num = torch.tensor([4094], dtype=torch.int32, device="cuda")
+    for n in (None, num, num * 0, num * 0 + 3):
+        loss, norm, d = check_distill(l, kept, cls, 2.0, DT[dt], how, 1, n)
+    loss, norm, d = check_distill(l, kept, cls, 2.0, DT[dt], how)
+    bad_cls, bad_kept = cls.clone(), kept.clone()
+    bad_cls[10::11, k - 1] = K
+    bad_kept[21::11, 0] = math.nan                                              # (some of these entries are absent, and do not count)
+    score, _ = lay(l, how)
+    one = score.dim() - 2
+    bl, bn = ops.distill_loss(score, bad_kept[None] if one else bad_kept, bad_cls[None] if one else bad_cls, 2.0)
+    bd = score_rows(ops.distill_loss_backward(score, bad_kept[None] if one else bad_kept, bad_cls[None] if one else bad_cls, bn, torch.linspace(-2, 3, R, device="cuda").view(bl.shape), 2.0))
+    bl, loss = bl.reshape(-1), loss.reshape(-1)
+    bad = (bad_cls >= K).any(1) | (torch.isnan(bad_kept) & (bad_cls >= 0)).any(1)
+    assert bad.any() and torch.isnan(bl[bad]).all() and torch.isnan(bd[bad]).all()
+    assert torch.equal(bl[~bad], loss[~bad]) and torch.equal(bd[~bad], score_rows(d)[~bad])
 
 
 @pytest.mark.gpu
