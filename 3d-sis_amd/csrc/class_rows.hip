@@ -16,7 +16,7 @@
 // Three forms, by the number of classes:
 //   short rows       (contiguous: as long as 64 lanes would not have a vector each; class-strided: K <= 1024)  a lane, or up to 32 of them,
 //                    takes a row; contiguous rows come through LDS in vectors, class-strided (planar) scores are read in place, with
-//                    neighbouring rows on neighbouring lanes.  More than four alternatives: a row in the registers of 1 .. 64 lanes
+//                    neighbouring rows on neighbouring lanes
 //   longer rows      a wave or a workgroup streams a row with 16-byte loads from its first aligned element on; distillation of up to 4 KB
 //                    by 16 lanes, so that four rows share what is done once a row
 //   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
@@ -53,7 +53,7 @@ struct RowArgs {
     const float *g1, *g2;                      // gradients: of logp and entropy, or of the loss
     const float2 *norm_in;
     const float *entropy_in;
-    int lpr_log, planar, parts;
+    int planar, parts;
     int g_log, sk, chunk;                      // tiles: lanes per row, floats of a row in LDS, classes of a lane
     uint32_t per4;                             // 2^32 / (K / 4), rounded up
     float *part;                               // [R * parts][4]
@@ -83,20 +83,17 @@ __device__ inline float mul_rounded(float a, float b)
 }
 __device__ inline float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// (score, class) as one number: larger score first, then the lower class; -0 counts as 0, NaN as -inf
-__device__ inline uint64_t key_of(float v, int c)
+// a score as a whole number of the same order; -0 counts as 0, NaN as -inf
+__device__ inline uint32_t ordered(float v)
 {
-    v = v != v ? -INFINITY : v + 0.f;
-    const uint32_t b = __float_as_uint(v);
-    const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    return ((uint64_t)o << 32) | (uint32_t)~c;
+    const uint32_t b = __float_as_uint(fmaxf(v, -INFINITY) + 0.f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ inline float score_of(uint32_t o) { return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xffffffffu)); }
+// (score, class) as one number: larger score first, then the lower class
+__device__ inline uint64_t key_of(float v, int c) { return ((uint64_t)ordered(v) << 32) | (uint32_t)~c; }
 __device__ inline int key_class(uint64_t k) { return (int)~(uint32_t)k; }
-__device__ inline float key_score(uint64_t k)
-{
-    const uint32_t o = (uint32_t)(k >> 32);
-    return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xffffffffu));
-}
+__device__ inline float key_score(uint64_t k) { return score_of((uint32_t)(k >> 32)); }
 __device__ inline uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__shfl_xor((unsigned long long)v, o); }
 __device__ inline uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ inline uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
@@ -317,34 +314,12 @@ template <int MODE> struct Back {
 // a teacher's entry: 0 = absent, 1 = present, 2 = no such class
 __device__ inline int entry(const RowArgs &a, int64_t c) { return c < 0 ? 0 : (c >= a.K ? 2 : 1); }
 
-// ------------------------------------ short rows, more than four alternatives: a row in the registers of 1 .. 64 lanes --
+// --------------------------------------------------------------------------- the lanes that share a short row --
 struct Group {
     int64_t r, at;                             // row; the row that may be read (0 where r is none: such lanes take part in the shuffles only)
     int sub, lpr, step;                        // lane of the row, lanes per row, distance of neighbouring row lanes
     bool in, live;                             // a row of the call; a live one
 };
-__device__ inline Group group_of(const RowArgs &a)
-{
-    Group g;
-    const int lane = threadIdx.x & 63, rpw_log = 6 - a.lpr_log;
-    g.lpr = 1 << a.lpr_log;
-    const int64_t wave = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
-    int row;
-    if (a.planar) {
-        row = lane & ((1 << rpw_log) - 1);
-        g.sub = lane >> rpw_log;
-        g.step = 1 << rpw_log;
-    } else {
-        row = lane >> a.lpr_log;
-        g.sub = lane & (g.lpr - 1);
-        g.step = 1;
-    }
-    g.r = (wave << rpw_log) + row;
-    g.in = g.r < a.R;
-    g.live = g.in && g.r < live_rows(a);
-    g.at = g.live ? g.r : 0;
-    return g;
-}
 __device__ inline float group_sum(float v, const Group &g)
 {
     for (int o = g.lpr >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o * g.step);
@@ -403,52 +378,6 @@ __device__ inline float entry_loss(const RowArgs &a, const Teacher &t, float ls,
     return q != 0.f ? q * (x * LN2 - ls - log_p(l, norm, a.inv, a.inv_lo)) : 0.f;
 }
 
-template <typename T, int E> __global__ __launch_bounds__(256) void small_forward(RowArgs a)
-{
-    const Group g = group_of(a);
-    const T *p = (const T *)a.score + row_at(a, g.at, a.s_n, a.s_v);
-    float v[E];
-    Soft<true> so;
-    so.init();
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = g.sub + e * g.lpr;
-        v[e] = c < a.K && g.live ? sis3d_f32(p[c * a.s_c]) : -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) so.m = fmaxf(so.m, v[e]);
-    so.m = group_max(so.m, g);
-#pragma unroll
-    for (int e = 0; e < E; ++e) so.add(v[e], a.c2);
-    so.s = group_sum(so.s, g);
-    so.t = group_sum(so.t, g);
-    const Norm norm{so.m, so.log_s()};
-    if (g.sub == 0 && g.in) {
-        const int64_t y = a.labels[g.at];
-        a.logp[g.r] = g.live ? label_logp(a, y, y >= 0 && y < a.K ? sis3d_f32(p[y * a.s_c]) : 0.f, norm) : 0.f;
-        a.entropy[g.r] = g.live ? so.entropy() : 0.f;
-        a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
-    }
-    uint32_t taken = 0;
-    for (int i = 0; i < a.top; ++i) {
-        uint64_t best = 0;
-        int at = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = g.sub + e * g.lpr;
-            const uint64_t k = c < a.K && !(taken >> e & 1) ? key_of(v[e], c) : 0;
-            if (k > best) { best = k; at = e; }
-        }
-        uint64_t all = best;
-        for (int o = g.lpr >> 1; o > 0; o >>= 1) all = max64(all, shfl_xor64(all, o * g.step));
-        if (best == all) taken |= 1u << at;
-        if (g.sub == 0 && g.in) {
-            a.top_class[g.r * a.top + i] = g.live ? key_class(all) : 0;
-            a.top_logp[g.r * a.top + i] = g.live ? log_p(key_score(all), norm, 1.f, 0.f) : 0.f;
-        }
-    }
-}
-
 template <int W> __device__ inline int team_of() { return W == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0; }
 template <int W> __device__ inline void team_sync()
 {
@@ -468,6 +397,46 @@ struct TileRow {
     int row, lo, n;                            // row of the tile; this lane's classes are lo .. lo + n - 1
 };
 constexpr int IN_PLACE = 0, BY_ONE = 1, BY_FOUR = 2;
+
+// (score, class) of a short row as one number, a larger one for a larger score and then for a lower class; 0 is none.  Scores of 16 bits,
+// as floats, are 0 in their last 13 bits and more, where the class (below 1024) goes; 32-bit scores take the mantissa of a double, whose maximum
+// and minimum are one instruction each.
+static_assert(K_STRIDED <= 1024, "10 bits of a key are the class");
+template <typename T> struct Rank {
+    using Key = uint32_t;
+    static __device__ Key key(float v, int c) { return (ordered(v) & ~1023u) | (uint32_t)(1023 - c); }
+    static __device__ int cls(Key k) { return 1023 - (int)(k & 1023u); }
+    static __device__ float score(Key k) { return __uint_as_float(__float_as_uint(score_of(k)) & ~1023u); }
+    static __device__ Key larger(Key a, Key b) { return a > b ? a : b; }
+    template <int N> static __device__ void insert(Key (&t)[N], Key k)       // t descending: the middle of a place, the one above it and k
+    {
+#pragma unroll
+        for (int i = N - 1; i > 0; --i) t[i] = larger(t[i], k < t[i - 1] ? k : t[i - 1]);
+        t[0] = larger(t[0], k);
+    }
+    static __device__ Key other(Key k, int o) { return __shfl_xor(k, o); }
+};
+template <> struct Rank<float> {
+    using Key = double;
+    static __device__ Key key(float v, int c)
+    {
+        const uint32_t o = ordered(v);
+        return __hiloint2double((int)(0x3ff00000u | o >> 22), (int)(o << 10 | (uint32_t)(1023 - c)));
+    }
+    static __device__ int cls(Key k) { return 1023 - (__double2loint(k) & 1023); }
+    static __device__ float score(Key k) { return score_of((uint32_t)__double2hiint(k) << 22 | (uint32_t)__double2loint(k) >> 10); }
+    static __device__ Key larger(Key a, Key b) { return fmax(a, b); }
+    template <int N> static __device__ void insert(Key (&t)[N], Key k)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const Key a = fmax(t[i], k);
+            k = fmin(t[i], k);
+            t[i] = a;
+        }
+    }
+    static __device__ Key other(Key k, int o) { return __hiloint2double(__shfl_xor(__double2hiint(k), o), __shfl_xor(__double2loint(k), o)); }
+};
 
 template <int HOW> __device__ inline TileRow tile_row(const RowArgs &a)
 {
@@ -566,38 +535,30 @@ template <typename T, int MODE, int HOW, int TK> __global__ __launch_bounds__(25
     auto score = [&](int64_t c) { return HOW == IN_PLACE ? sis3d_f32(p[c * a.s_c]) : row[c]; };
     Lane<MODE == LP> ln;
     ln.init();
-    float best = -INFINITY, tv[TK ? TK : 1];
-    int tc[TK ? TK : 1];
+    float best = -INFINITY;
+    using Key = typename Rank<T>::Key;
+    Key first[TK ? TK : 1];                            // this lane's best ones
 #pragma unroll
-    for (int k = 0; k < TK; ++k) {
-        tv[k] = -INFINITY;
-        tc[k] = -1;
-    }
+    for (int k = 0; k < TK; ++k) first[k] = 0;
     each_eight<T, HOW>(a, t, p, row, [&](int i, const float (&x)[8]) {
         const float top = max_of(x);
+        if constexpr (TK == 1)
+            if (top > best) {
+                int at = 0;
+#pragma unroll
+                for (int j = 7; j > 0; --j) at = x[j] == top ? j : at;
+                at = x[0] == top ? 0 : at;
+                first[0] = Rank<T>::key(top, t.lo + i + at);
+            }
         best = fmaxf(best, top);
         ln.follow(top, a.c2);
 #pragma unroll
         for (int j = 0; j < 8; ++j) ln.add(x[j], a.c2);
-        if constexpr (TK > 0)
-            if (top > tv[TK - 1])
+        if constexpr (TK > 1)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {          // behind equal ones, which have the lower classes
-                    float v = x[j];
-                    int c = t.lo + i + j;
-                    bool before = false;               // from its place on, all go one place down
-#pragma unroll
-                    for (int k = 0; k < TK; ++k) {
-                        before = before || v > tv[k];
-                        const float v2 = before ? tv[k] : v;
-                        const int c2 = before ? tc[k] : c;
-                        tv[k] = before ? v : tv[k];
-                        tc[k] = before ? c : tc[k];
-                        v = v2;
-                        c = c2;
-                    }
-                }
+            for (int j = 0; j < 8; ++j) Rank<T>::insert(first, i + j < t.n ? Rank<T>::key(x[j], t.lo + i + j) : (Key)0);
     });
+    if (TK == 1 && t.n > 0 && best == -INFINITY) first[0] = Rank<T>::key(best, t.lo);         // nothing was more than -inf
     // the lanes of a row, relative to its largest score, which has s = 1 if it is the only one
     Soft<MODE == LP> so;
     so.m = fmaxf(group_max(best, g), LOWEST);
@@ -639,39 +600,20 @@ template <typename T, int MODE, int HOW, int TK> __global__ __launch_bounds__(25
         a.entropy[g.r] = g.live ? so.entropy() : 0.f;
         a.norm[g.r] = g.live ? make_float2(so.m, so.s) : make_float2(0.f, 0.f);
     }
-    if constexpr (TK > 0) {
-        int none = 0;                                  // next class to look at for one that ranks last: -inf or NaN
+    if constexpr (TK > 0)
         for (int i = 0; i < a.top; ++i) {
             // the best of the lanes' first ones; its lane goes on to the next
-            float v = tv[0];
-            int c = tc[0];
-            for (int o = g.lpr >> 1; o > 0; o >>= 1) {
-                const float v2 = __shfl_xor(v, o * g.step);
-                const int c2 = __shfl_xor(c, o * g.step);
-                const bool other = v2 > v || (v2 == v && (uint32_t)c2 < (uint32_t)c);
-                v = other ? v2 : v;
-                c = other ? c2 : c;
-            }
-            if (c >= 0 && c == tc[0]) {
+            Key k = first[0];
+            for (int o = g.lpr >> 1; o > 0; o >>= 1) k = Rank<T>::larger(k, Rank<T>::other(k, o * g.step));
+            const bool mine = k == first[0];
 #pragma unroll
-                for (int k = 0; k + 1 < TK; ++k) {
-                    tv[k] = tv[k + 1];
-                    tc[k] = tc[k + 1];
-                }
-                tv[TK - 1] = -INFINITY;
-                tc[TK - 1] = -1;
-            }
+            for (int j = 0; j + 1 < TK; ++j) first[j] = mine ? first[j + 1] : first[j];
+            first[TK - 1] = mine ? (Key)0 : first[TK - 1];
             if (g.sub == 0 && g.in) {
-                if (g.live && c < 0) {
-                    while (none < a.K - 1 && score(none) > -INFINITY) ++none;
-                    c = none++;
-                    v = c < a.K ? score(c) : -INFINITY;
-                }
-                a.top_class[g.r * a.top + i] = g.live ? c : 0;
-                a.top_logp[g.r * a.top + i] = g.live ? log_p(v, norm, 1.f, 0.f) : 0.f;
+                a.top_class[g.r * a.top + i] = g.live ? Rank<T>::cls(k) : 0;
+                a.top_logp[g.r * a.top + i] = g.live ? log_p(Rank<T>::score(k), norm, 1.f, 0.f) : 0.f;
             }
         }
-    }
 }
 
 template <typename T, int MODE, int HOW> __global__ __launch_bounds__(256) void tile_backward(RowArgs a)
@@ -1489,7 +1431,7 @@ bool wave_rows(const RowArgs &a, int es) { return a.parts == 1 && (a.K <= K_WAVE
 // 26 / 24, x 4000 23 / 25)
 bool four_rows(const RowArgs &a, int es) { return a.s_c == 1 && a.nk <= 32 && a.K >= 96 && a.K * es <= 4096 && a.R >= 16 * 256; }
 
-// how a tile's rows are had, its lanes per row and its LDS; LDS for dense, aligned rows of at most 24 floats a lane
+// how a tile's rows are had, its lanes per row and its LDS; LDS for dense, aligned rows of at most 56 floats a lane
 template <typename T> int plan_tile(RowArgs &a, bool backward)
 {
     const bool dense = a.s_c == 1 && a.s_v == a.K && (a.N == 1 || a.s_n == a.V * a.K) && ((uintptr_t)a.score & 15) == 0 &&
@@ -1502,8 +1444,11 @@ template <typename T> int plan_tile(RowArgs &a, bool backward)
     // 183 / 196 us forward by eight / sixteen, 356 / 455 backward.  Rows, 16 entries, backward: 276 us by two, 81 by four, 93 by eight.
     a.g_log = 0;
     while (a.g_log < 3 && (backward && dense ? 4 : 2) << a.g_log < a.nk && 4 << a.g_log < a.K) ++a.g_log;
+    // 24 classes a lane; 56 where the lanes' lists of alternatives have to be joined (400000 x 100 bf16, ten alternatives: 120 us by 24, 99 by
+    // 48, 90 by 96, which is 64 KB of LDS and more)
+    const int stretch = a.top > 4 && a.K > 48 ? 56 : 24;
     if (dense || !a.planar)
-        while (a.g_log < 5 && 24 << a.g_log < a.K) ++a.g_log;
+        while (a.g_log < 5 && stretch << a.g_log < a.K) ++a.g_log;
     // more lanes to a row while there are CUs without a workgroup
     while (a.g_log < 4 && 8 << a.g_log < a.K && (a.R << a.g_log) < 256 * 256) ++a.g_log;
     a.chunk = (a.K + (1 << a.g_log) - 1) >> a.g_log;
@@ -1531,22 +1476,14 @@ template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
             return sis3d_check_launch();
         }
     if (is_short(a.K, a.s_c, sizeof(T))) {
-        if (a.top > 4) {                               // lists of a lane get long: a row in the registers of a group, `top` maxima of it
-            const int64_t waves = (a.R + (64 >> a.lpr_log) - 1) / (64 >> a.lpr_log);
-            if (too_many((waves + 3) / 4)) return SIS3D_EUNSUPPORTED;
-            const dim3 grid((unsigned)((waves + 3) / 4));
-            const int e = (a.K + (1 << a.lpr_log) - 1) >> a.lpr_log;
-            if constexpr (MODE == LP) {
-                if (e <= 8) hipLaunchKernelGGL((small_forward<T, 8>), grid, dim3(256), 0, st, a);
-                else hipLaunchKernelGGL((small_forward<T, 16>), grid, dim3(256), 0, st, a);
-            }
-            return sis3d_check_launch();
-        }
         const int how = plan_tile<T>(a, false);
         if (too_many((a.R + (256 >> a.g_log) - 1) / (256 >> a.g_log))) return SIS3D_EUNSUPPORTED;
         if (MODE == KD || a.top == 0) tile_launch<T, MODE, 0>(a, how, st);
         else if (a.top == 1) tile_launch<T, LP, 1>(a, how, st);
-        else tile_launch<T, LP, 4>(a, how, st);
+        else if (a.top <= 4) tile_launch<T, LP, 4>(a, how, st);
+        else if (a.top <= 8) tile_launch<T, LP, 8>(a, how, st);
+        else if (a.top <= 16) tile_launch<T, LP, 16>(a, how, st);
+        else tile_launch<T, LP, 32>(a, how, st);
         return sis3d_check_launch();
     }
     const bool by_wave = wave_rows(a, sizeof(T));
@@ -1606,8 +1543,6 @@ int fill(RowArgs &a, const void *score, int dtype, int N, int64_t V, int K, int6
     if (K > K_STRIDED && s_c != 1) return SIS3D_EUNSUPPORTED;
     if (((uintptr_t)score) % sis3d_elem_bytes(dtype)) return SIS3D_EINVAL;
     a.planar = s_c != 1 && s_v < s_c;
-    a.lpr_log = 0;
-    while (a.lpr_log < 6 && (8 << a.lpr_log) < K) ++a.lpr_log;
     a.parts = parts_of(a.R, K, s_c);
     if (a.R * a.parts > 0x7fffffff) return SIS3D_EUNSUPPORTED;
     return SIS3D_OK;
