@@ -1444,15 +1444,17 @@ template <typename T> int plan_tile(RowArgs &a, bool backward)
     // 183 / 196 us forward by eight / sixteen, 356 / 455 backward.  Rows, 16 entries, backward: 276 us by two, 81 by four, 93 by eight.
     a.g_log = 0;
     while (a.g_log < 3 && (backward && dense ? 4 : 2) << a.g_log < a.nk && 4 << a.g_log < a.K) ++a.g_log;
-    // 24 classes a lane; 56 where the lanes' lists of alternatives have to be joined (400000 x 100 bf16, ten alternatives: 120 us by 24, 99 by
+    // 32 classes a lane (400000 x 41 fp32: 20 us by two lanes, 28 by one); 56 where the lanes' lists of alternatives have to be joined (400000 x 100 bf16, ten alternatives: 120 us by 24, 99 by
     // 48, 90 by 96, which is 64 KB of LDS and more)
-    const int stretch = a.top > 4 && a.K > 48 ? 56 : 24;
+    const int stretch = a.top > 4 && a.K > 48 ? 56 : 32;
     if (dense || !a.planar)
         while (a.g_log < 5 && stretch << a.g_log < a.K) ++a.g_log;
     // more lanes to a row while there are CUs without a workgroup
     while (a.g_log < 4 && 8 << a.g_log < a.K && (a.R << a.g_log) < 256 * 256) ++a.g_log;
     a.chunk = (a.K + (1 << a.g_log) - 1) >> a.g_log;
-    if (how == BY_FOUR) a.chunk = (a.chunk + 3) / 4 * 4;
+    // the lanes of a row meet different banks (125000 x 400 bf16 with stretches of 16: backward 105 us, of 28: 54)
+    if (how == BY_FOUR) a.chunk = ((a.chunk + 3) / 4 | 1) * 4;
+    if (how == BY_ONE) a.chunk |= 1;
     return how;
 }
 size_t tile_lds(const RowArgs &a, int how) { return how == IN_PLACE ? 0 : ((size_t)(256 >> a.g_log) * a.sk + ((size_t)a.chunk << a.g_log) + 16) * sizeof(float); }
