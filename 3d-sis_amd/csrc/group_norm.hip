@@ -67,19 +67,15 @@ __device__ inline Tile find_tile(const GnArgs &a, int b)
         r.len = a.rows;
         begin = 0;
     } else {
-        // the last s with floor(off[s] / T) + s <= b: one load a thread, or a search where there are more samples than threads
-        int lo;
-        if (a.S < NT) {
-            const int s = threadIdx.x;
-            lo = __syncthreads_count(s <= a.S && (clamp_off(a, s) >> a.t_log) + s <= b) - 1;
-        } else {
-            lo = 0;
-            int hi = a.S + 1;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if ((clamp_off(a, mid) >> a.t_log) + mid <= b) lo = mid;
-                else hi = mid;
-            }
+        // the last s with floor(off[s] / T) + s <= b, which is one of b - floor(rows / T) .. b: a thread looks at one of every `step` of
+        // these (one of each, mostly), then at those in between
+        int lo = max(0, b - (int)(a.rows >> a.t_log)), n = min(a.S, b) + 1 - lo;
+        while (n > 1) {
+            const int step = (n + NT - 1) / NT, s = lo + threadIdx.x * step;
+            const bool before = (int)threadIdx.x * step < n && (clamp_off(a, s) >> a.t_log) + s <= b;
+            const int up = (max(__syncthreads_count(before), 1) - 1) * step;
+            lo += up;
+            n = min(step, n - up);
         }
         r.s = lo;
         begin = clamp_off(a, lo);
@@ -149,17 +145,33 @@ template <typename P, typename F> __device__ inline void reduce_groups(const P *
     }
 }
 
+// p[i * stride] for i = from, from + step, ...: added in that order, eight of them on their way at a time
+template <typename P> __device__ inline void sum_pairs(const P *p, int64_t stride, int from, int n, int step, double &s0, double &s1)
+{
+    int i = from;
+    for (; i + step < n; i += 8 * step) {
+        P v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = p[min(i + u * step, n - 1) * stride];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            s0 += i + u * step < n ? v[u].x : 0;
+            s1 += i + u * step < n ? v[u].y : 0;
+        }
+    }
+    if (i < n) {                                     // all there is, mostly, where samples are small
+        s0 += p[i * stride].x;
+        s1 += p[i * stride].y;
+    }
+}
+
 // The same over the tiles of one sample: part[g * tiles + first + p], so that a wave reads neighbouring tiles
 template <typename P, typename F> __device__ inline void reduce_tiles(const P *part, int tiles, int first, int ntiles, int g0, int gl, F out)
 {
     const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
         double s0 = 0, s1 = 0;
-        for (int p = l; p < ntiles; p += lp) {
-            const P v = part[(size_t)(g0 + g) * tiles + first + p];
-            s0 += v.x;
-            s1 += v.y;
-        }
+        sum_pairs(part + (size_t)(g0 + g) * tiles + first, 1, l, ntiles, lp, s0, s1);
         finish_group(s0, s1, lp, l, g, out);
     }
 }
@@ -529,11 +541,7 @@ template <typename T, int VEC, int ACT, bool ONCE> __global__ __launch_bounds__(
         const int c = ((int)blockIdx.x - a.tiles) * 32 + (threadIdx.x & 31), l = threadIdx.x >> 5;
         double s0 = 0, s1 = 0;
         if (c < a.C)
-            for (int p = l; p < a.tiles; p += NT / 32) {
-                const float2 v = a.part_c[(size_t)p * a.C + c];
-                s0 += v.x;
-                s1 += v.y;
-            }
+            sum_pairs(a.part_c + c, a.C, l, a.tiles, NT / 32, s0, s1);
         acc[threadIdx.x][0] = s0;
         acc[threadIdx.x][1] = s1;
         __syncthreads();
@@ -610,7 +618,12 @@ Plan make_plan(int dtype, int S, int64_t rows, int ragged, int C, int G, bool wi
     // one workgroup takes a whole sample where that is little: up to 128 KB of a line it is sooner done than a second launch.  Its column
     // blocks are narrower than a line while there are fewer than 512 of them: the rows come from cache, and more CUs take part
     p.one = rows * (cpg * gu * es > 128 ? cpg * gu * es : 128) <= 128 * 1024 && !(backward && (S != 1 || ragged));
-    while (p.gpb < G && p.gpb * cpg * es < 128 && p.gpb + gu <= most && !(p.one && (int64_t)S * G / p.gpb <= 512)) p.gpb += gu;
+    // Samples of few rows: wider, so that a workgroup has 64 KB to work on (5000 samples of 31 rows of
+    // 256 fp32 channels: forward 385 us by lines, 76 by whole rows; 1000 of 156: 90 us by lines, 53 by 16 KB, 38 by 64)
+    const int64_t mean_rows = S ? total / S : total;
+    while (p.gpb < G && (p.gpb * cpg * es < 128 || mean_rows * p.gpb * cpg * es < 64 << 10) && p.gpb + gu <= most &&
+           !(p.one && (int64_t)S * G / p.gpb <= 512))
+        p.gpb += gu;
     if (p.gpb > G) p.gpb = G;
     p.ncol = (G + p.gpb - 1) / p.gpb;
     int64_t T;

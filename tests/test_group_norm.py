@@ -245,6 +245,19 @@ def test_many_samples_and_one_row_each():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C,G", [(256, 32), (96, 32), (20, 4)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_small_samples_around_a_large_one(dtype, C, G):
+    """workgroups with whole rows, offsets that are far from their even places"""
+    lens = [(i * 37) % 6 for i in range(300)] + [40000] + [(i * 11) % 5 for i in range(400)] + [0, 0]
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    x, dy, w, b = make(offsets[-1], C, dtype, seed=C)
+    compare_rows(run_rows(x, dy, offsets, G, w, b, "silu"), reference(x.double(), dy.double(), offsets, G, w, b, "silu"), dtype)
+
+
+@pytest.mark.gpu
 def test_large_mean_constant_and_non_finite_inputs():
     from sis3d import ops
     g = torch.Generator(device="cuda").manual_seed(0)
