@@ -1406,6 +1406,87 @@ template <typename T, int W, int MODE> __global__ __launch_bounds__(256) void lo
     }
 }
 
+// The same with 16 lanes to a row, four rows to a wave, as four_distill
+template <typename T, int MODE> __global__ __launch_bounds__(256) void four_backward(RowArgs a)
+{
+    constexpr int L = 16, VEC = 16 / sizeof(T), UL = loads_of(L);
+    __shared__ float q_s[16][MODE == KD ? 2 * L : 1];
+    __shared__ int c_s[16][MODE == KD ? 2 * L : 1];
+    const int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4, r = r0 + ((threadIdx.x & 63) >> 4), n = live_rows(a);
+    const int lane = threadIdx.x & (L - 1), team = threadIdx.x >> 4;
+    if (r0 >= a.R) return;                                     // the whole wave
+    T *out = (T *)a.dscore + row_at(a, r < a.R ? r : 0, a.d_n, a.d_v);
+    if (r >= n) {
+        if (r < a.R)
+            for (int c = lane; c < a.K; c += L) out[c] = sis3d_from_f32<T>(0.f);
+        return;                                                // all lanes of the row
+    }
+    const T *row = (const T *)a.score + row_at(a, r, a.s_n, a.s_v);
+    const Span<T> sp(row, 0, a.K);
+    Back<MODE> k;
+    const float2 norm = a.norm_in[r];
+    const float g1 = a.g1[r];
+    const Label label = MODE == LP ? Label(a, r) : Label();
+    Kept<L> kept(a, r, MODE == KD);
+    Stream<T, L, true> st(sp, lane, a.K / VEC);
+    const float edge = lane < sp.edges() ? sis3d_f32(row[sp.edge_class(lane)]) : 0.f;
+    float ly = 0.f;
+    if constexpr (MODE == LP) {
+        if (label.y >= 0 && label.y < a.K) ly = sis3d_f32(row[label.y]);
+        k.scores(norm, a.entropy_in[r], label.y < 0 ? 0.f : (label.y >= a.K ? NAN : g1), a.g2 ? a.g2[r] : 0.f);
+    } else {
+        kept.scores(a, row);
+        const Teacher t = kept.teacher(a);
+        k.loss(norm, t.bad ? NAN : (t.any ? g1 * a.tau : 0.f), a.c2);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            c_s[team][lane + L * j] = kept.c[j];
+            q_s[team][lane + L * j] = t.any ? exp2_((kept.x[j] - t.m) * a.c2) * rcp_(t.s) : 0.f;
+        }
+    }
+    const bool wide = ((uintptr_t)(out + sp.head) & 15) == 0;
+    if (!k.in_range) {
+        for (int c = lane; c < a.K; c += L) out[c] = sis3d_from_f32<T>(k.exact(sis3d_f32(row[c])));
+    } else {
+        st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
+            constexpr int N = decltype(count)::value;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int c = sp.first_class(v + u * L);
+                float x[VEC];
+                sis3d_unpack<T, VEC>(raw[u], x);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[i] = k.near(x[i]);
+                if (u == N - 1 && v + u * L >= sp.nvec) continue;
+                if (wide) sis3d_store<T, VEC>(out + c, x);
+                else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) out[c + i] = sis3d_from_f32<T>(x[i]);
+                }
+            }
+        });
+        if (lane < sp.edges()) out[sp.edge_class(lane)] = sis3d_from_f32<T>(k.exact(edge));
+    }
+    team_sync<1>();                                            // the label's class or the kept ones again, behind the row's other stores
+    if constexpr (MODE == LP) {
+        if (lane == 0 && label.y >= 0 && label.y < a.K) out[label.y] = sis3d_from_f32<T>(k.exact(ly) + k.ga);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = lane + L * j, c = kept.c[j];
+            if (i >= a.nk || c < 0) continue;
+            float q = 0.f;
+            bool first = true;
+            for (int m = 0; m < a.nk; ++m)
+                if (c_s[team][m] == c) {
+                    q += q_s[team][m];
+                    first = first && m >= i;
+                }
+            if (first) out[c] = sis3d_from_f32<T>(k.exact(kept.l[j]) - k.ga * q);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------ host --
 // a launch has at most 2^32 - 1 threads
 bool too_many(int64_t workgroups) { return workgroups > 0xffffffffll / 256; }
@@ -1508,6 +1589,13 @@ template <typename T, int MODE> int run_forward(RowArgs &a, hipStream_t st)
 
 template <typename T, int MODE> int run_backward(RowArgs &a, hipStream_t st)
 {
+    // 16 lanes to a row where a wave has too little of it and a tile too few rows (100 MB bf16, log probabilities: x 100 50 us by tiles, 60 by
+    // 16 lanes; x 200 54 / 42, x 400 54 / 40, x 600 44 / 42, x 1000 37 by waves, 40; fp32 x 200 47 / 40, x 300 40 / 40)
+    if (a.d_c == 1 && a.K >= 200 && a.K * (int)sizeof(T) <= 1200 && four_rows(a, sizeof(T))) {
+        if (too_many((a.R + 15) / 16)) return SIS3D_EUNSUPPORTED;
+        hipLaunchKernelGGL((four_backward<T, MODE>), dim3((unsigned)((a.R + 15) / 16)), dim3(256), 0, st, a);
+        return sis3d_check_launch();
+    }
     if (is_short(a.K, a.s_c, sizeof(T)) || a.d_c != 1) {
         const int how = plan_tile<T>(a, true), rb = 256 >> a.g_log;
         if (too_many((a.R + rb - 1) / rb)) return SIS3D_EUNSUPPORTED;
