@@ -17,6 +17,13 @@
 //
 // Sums: a thread adds d = x - K and d^2 in 32 bits over its rows (at most 2048, a few hundred mostly), K its own first row, so a mean that is large
 // against the deviation does not cancel; everything across threads is added in 64 bits.
+//
+// Measured (kernel alone; rate of the bytes that it moves itself, the rows' second reading included):
+//   96 x 48 x 96 x 32 fp32, ReLU   gn_stats 13.1 us (4.3 TB/s), gn_apply 17.4 (6.5), gn_back_sums 22.6 (5.0), gn_back_apply 25.2 (6.7):  78 us
+//                                  for 226 MB that have to move once
+//   24 x 12 x 24 x 128 fp32, ReLU  4.9, 5.6, 7.0, 7.0 us: the loads' way and back, twice a launch; the calls take the host 35 us
+//   16 crops, 43995 x 64 in all    7.3, 8.0, 9.2, 9.2 us
+//   12 x 6 x 12 x 128 fp32         gn_one 6.9 us
 #include "elem.h"
 
 namespace {
