@@ -536,7 +536,7 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
         assert l.sis3d_distill_backward(*dict(e0, **k).values()) == -1, k
     # more rows than a launch has threads for
     many = dict(V=1 << 30, K=5000, sv=5000, top=0)
-    assert fwd(**many) == -4 and fwd(**dict(many, K=600)) == -4 and fwd(**dict(many, K=100, top=5)) == -4 and fwd(**dict(many, K=400)) == -4
+    assert fwd(**many) == -4 and fwd(**dict(many, K=600)) == -4 and fwd(**dict(many, K=400, top=5)) == -4 and fwd(**dict(many, K=400)) == -4
     many = dict(V=1 << 30, K=5000, sv=5000)
     assert l.sis3d_class_logprobs_backward(*dict(b0, **many).values()) == -4 and l.sis3d_distill_backward(*dict(e0, **many, ).values()) == -4
     assert l.sis3d_distill_backward(*dict(e0, **dict(many, K=400)).values()) == -4
