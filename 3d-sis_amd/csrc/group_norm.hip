@@ -616,7 +616,7 @@ Plan make_plan(int dtype, int S, int64_t rows, int ragged, int C, int G, bool wi
     const int es = sis3d_elem_bytes(dtype), cpg = C / G;
     p.vec = wide && C % (16 / es) == 0 ? 16 / es : 1;
     const int gu = p.vec / gcd_(cpg, p.vec);               // groups whose channels are whole vectors
-    const int most = (int)((int64_t)NT * p.vec / cpg) / gu * gu;
+    const int fit = (int)((int64_t)NT * p.vec / cpg), most = (fit < NT ? fit : NT) / gu * gu;        // a block has at most NT groups
     if (most < 1) { p.rc = SIS3D_EUNSUPPORTED; return p; }
     // a column block is one 128-byte line of a row, or one group if that is wider: the narrower it is, the fewer groups a workgroup of
     // the second launch has to add the tiles' sums of
@@ -673,10 +673,15 @@ size_t ws_bytes_of(const Plan &p, int C, int G, bool backward)
 
 template <typename T, int VEC> int launch(const GnArgs &a, const Plan &p, int act, bool backward, hipStream_t st)
 {
-    const int cl = p.gpb * a.cpg, rpb = NT / (cl / VEC);
     dim3 grid((unsigned)p.tiles, p.ncol);
-    // forward: a pair of doubles a thread, or a channel where groups are not whole vectors; backward: a pair of floats a channel
-    size_t lds = backward ? (size_t)rpb * cl * sizeof(float2) : (size_t)rpb * (a.cpg % VEC ? cl : cl / VEC) * sizeof(double2);
+    // forward: a pair of doubles a thread, or a channel where groups are not whole vectors; backward: a pair of floats a channel.  The last
+    // column block may have fewer groups, and then more rows in parallel, than the others
+    size_t lds = 0;
+    for (int groups : {p.gpb, a.G - (p.ncol - 1) * p.gpb}) {
+        const int cl = groups * a.cpg, rpb = NT / (cl / VEC);
+        const size_t need = backward ? (size_t)rpb * cl * sizeof(float2) : (size_t)rpb * (a.cpg % VEC ? cl : cl / VEC) * sizeof(double2);
+        if (need > lds) lds = need;
+    }
     if (p.one) {
         if (backward) { GN_ACT(gn_back_one) }
         else { GN_ACT(gn_one) }

@@ -349,6 +349,43 @@ def test_distillation_of_many_rows_with_edges(how, K, k, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how,K", [("rows", 1), ("rows", 3), ("planar", 2), ("planar", 19), ("rows", 19), ("wide", 300), ("rows", 400), ("rows", 1203), ("rows", 5000), ("rows", 9000)])
+@pytest.mark.parametrize("R", [5, 4500])
+def test_the_most_entries_that_a_row_may_keep(how, K, R):
+    """128 entries, most of them of the same few classes"""
+    if R * K > 1e7:
+        R = 300
+    l, _, _, _, g = make(R, K, torch.float32, seed=K + R)
+    kept = torch.randn(R, 128, device="cuda", generator=g)
+    cls = torch.randint(0, min(K, 40), (R, 128), device="cuda", generator=g)
+    cls[:, ::3] = torch.randint(0, K, (R, 43), device="cuda", generator=g)
+    cls[:, 5] = -1
+    check_distill(l, kept, cls, 1.5, torch.float32, how)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [19, 300, 2000, 9000])
+def test_one_row_of_scores_for_many_labels(K):
+    """an expanded tensor: rows that share their memory"""
+    from sis3d import ops
+    l, _, _, _, g = make(1, K, torch.float32, seed=K)
+    R = 4200 if K < 9000 else 200
+    labels = torch.randint(0, K, (R,), device="cuda", generator=g)
+    ga = torch.randn(R, device="cuda", generator=g)
+    kept, cls = torch.randn(R, 4, device="cuda", generator=g), torch.randint(0, K, (R, 4), device="cuda", generator=g)
+    for a, b in ((l.expand(R, K), l.expand(R, K).contiguous()),):
+        fa, fb = ops.class_logprobs(a, labels, 5), ops.class_logprobs(b, labels, 5)
+        assert torch.equal(fa[4], fb[4])
+        near(fa[0], fb[0].double(), 8 * U * (1 + fb[0].double().abs()) + chain(K), None, "logp")
+        da, db = ops.class_logprobs_backward(a, labels, fa[2], fa[1], ga), ops.class_logprobs_backward(b, labels, fb[2], fb[1], ga)
+        near(da, db.double(), ga.double().abs()[:, None] * (32 * U + 2 * chain(K)), None, "dscore")
+        (la, na), (lb, nb) = ops.distill_loss(a, kept, cls), ops.distill_loss(b, kept, cls)
+        near(la, lb.double(), 32 * U * (1 + lb.double().abs()) + chain(K), None, "loss")
+        near(ops.distill_loss_backward(a, kept, cls, na, ga), ops.distill_loss_backward(b, kept, cls, nb, ga).double(),
+             ga.double().abs()[:, None] * (64 * U + 2 * chain(K)), None, "dscore")
+
+
+@pytest.mark.gpu
 def test_streams_graph_and_determinism():
     from sis3d import ops
     for R, K, top in ((200, 19, 3), (64, 3000, 8), (2, 60000, 8), (300, 20011, 32)):

@@ -258,6 +258,49 @@ def test_small_samples_around_a_large_one(dtype, C, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C,G", [(96, 32), (48, 16), (40, 8), (80, 16), (160, 32)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens", [(1872, 700, 40, 2028), (600, 171, 510)])
+@pytest.mark.parametrize("odd", [0, 1])
+def test_last_channels_narrower_than_the_others(dtype, C, G, lens, odd):
+    """the groups that are left over have more rows in parallel than the others: all of them count.  odd: rows off 16 bytes"""
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    x, dy, w, b = make(offsets[-1], C, dtype, seed=C)
+    if odd:
+        wide = torch.zeros(2, offsets[-1], C + 3, dtype=dtype, device="cuda")
+        wide[0, :, 1:1 + C], wide[1, :, 1:1 + C] = x, dy
+        x, dy = wide[0, :, 1:1 + C], wide[1, :, 1:1 + C]
+    compare_rows(run_rows(x, dy, offsets, G, w, b, "silu"), reference(x.double(), dy.double(), offsets, G, w, b, "silu"), dtype)
+    from sis3d import ops
+    dense = x[:600][None].permute(0, 2, 1)                                      # a dense sample, one launch or two
+    y = ops.group_norm(dense, G, w, b, EPS, act="silu")
+    want = reference(x[:600].double(), dy[:600].double(), [0, 600], G, w, b, "silu")
+    check_close(y[0].t(), want["y"], want["ty"] + half_of(dtype) * want["y"].abs(), "dense y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,G", [(1024, 1024), (2048, 1024), (520, 520)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_groups_than_threads(dtype, C, G):
+    lens = [3, 0, 1, 5, 2]
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    x, dy, w, b = make(offsets[-1], C, dtype, seed=C)
+    want = reference(x.double(), dy.double(), offsets, G, w, b, "silu")
+    compare_rows(run_rows(x, dy, offsets, G, w, b, "silu"), want, dtype)
+    from sis3d import ops
+    for n, v in ((1, 11), (11, 1)):                                              # dense: one sample of all rows, and one of each
+        off = list(range(0, 12, v))
+        want = reference(x.double(), dy.double(), off, G, w, b, "silu")
+        y, mean, rstd = ops.group_norm(x.view(n, v, C).permute(0, 2, 1), G, w, b, EPS, act="silu", want_stats=True)
+        dx, dw, db = ops.group_norm_backward(dy.view(n, v, C).permute(0, 2, 1), x.view(n, v, C).permute(0, 2, 1), mean, rstd, G, w, b, act="silu")
+        compare_rows((rows_of(y), mean, rstd, rows_of(dx), dw, db), want, dtype)
+
+
+@pytest.mark.gpu
 def test_large_mean_constant_and_non_finite_inputs():
     from sis3d import ops
     g = torch.Generator(device="cuda").manual_seed(0)
