@@ -22,9 +22,10 @@
 //   few long rows    the class axis is split over workgroups and a second launch joins their sums and alternatives
 //
 // Alternatives of a long row without sorting it or reading it twice: every lane knows the largest score it has seen.  The lanes of a wave
-// are put into >= k groups; the smallest of the group maxima is a bound that at least k elements reach.  It is taken after 1, 2, 4, ...
-// batches of loads, and vectors with an element that reaches it are noted while they pass -- k log k of them or so a time.  Those that still
-// reach the last bound, one or two a lane, are read again and their elements at or above it ranked by counting, by (score, class).
+// are put into >= k groups; the smallest of the group maxima is a bound that at least k elements reach, and so is any number that k lanes'
+// maxima reach.  It is taken after 1, 2, 4, ... batches of loads, and vectors with an element that reaches it are noted while they pass.
+// Those that still reach the last bound, a few more than k, are read again and their elements at or above it ranked by counting, by
+// (score, class).
 //
 // Measured (kernel alone):
 //   tile_forward / tile_backward   55296 x 41 fp32 planar, one alternative: 6.8 / 7.9 us.  200 x 19 fp32: 5 / 5 us, the loads' way and back
@@ -798,17 +799,46 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     // What a wave notes while it reads; all but `best` is the same in all lanes
     struct Noted {
         float best, b;                         // this lane's largest score; the bound
-        int lanes, count, batch, next;
+        int want, lanes, count, batch, next;
         bool over;                             // there was no room
-        __device__ void init(int want)
+        __device__ void init(int want_)
         {
+            want = want_;
             best = b = -INFINITY;
             lanes = want > 16 ? 2 : want > 8 ? 4 : want > 4 ? 8 : 16;
             count = batch = 0;
             next = 1;
             over = false;
         }
-        __device__ void tighten() { b = fmaxf(b, wave_min(neighbours_max(best, lanes))); }
+        // The smallest maximum of as many groups of lanes as are wanted.  For more alternatives then closer, by halves, to the largest number
+        // that as many lanes' maxima reach: every step's bound is one (10000 x 2500 fp32: ten alternatives 37 us without, 25 with, 32 of
+        // them 93 and 28; by workgroups, 2500 x 20000 bf16, eight of them 35 and 36)
+        __device__ void tighten()
+        {
+            b = fmaxf(b, wave_min(neighbours_max(best, lanes)));
+            if (want <= (W == 1 ? 4 : 8)) return;
+            float above = wave_max(best);
+            for (int i = 0; i < 6; ++i) {
+                const float mid = 0.5f * b + 0.5f * above;
+                const bool reached = __popcll(__ballot(best >= mid)) >= want;
+                b = reached ? mid : b;
+                above = reached ? above : mid;
+            }
+        }
+        // keeps the vectors that reach the bound
+        __device__ void compact(Vec *list)
+        {
+            const int ln = threadIdx.x & 63;
+            int kept = 0;
+            for (int i = 0; i < count; i += 64) {
+                const Vec e = list[min(i + ln, count - 1)];
+                const uint64_t mask = __ballot(i + ln < count && e.m >= b);
+                if (mask >> ln & 1) list[kept + __popcll(mask & ((1ull << ln) - 1))] = e;         // not behind its own place
+                kept += __popcll(mask);
+                team_sync<1>();
+            }
+            count = kept;
+        }
         // puts entries of the lanes that have one behind the list's others
         template <typename E> __device__ void note(E *list, bool there, E entry)
         {
@@ -872,7 +902,7 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
         auto batch = [&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
             constexpr int N = decltype(count)::value;
             const bool last = v + (N - 1) * NL < sp.nvec;       // no vector: -inf adds nothing
-            float x[N][VEC], mx[N], top = -INFINITY;
+            float x[N][VEC], mx[N];
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 sis3d_unpack<T, VEC>(raw[u], x[u]);
@@ -880,14 +910,19 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) x[u][i] = last ? x[u][i] : -INFINITY;
                 mx[u] = max_of(x[u]);
-                nt.best = fmaxf(nt.best, mx[u]);
-                top = fmaxf(top, mx[u]);
             }
+            const float top = max_of(mx);
+            nt.best = fmaxf(nt.best, top);
             ln.follow(top, a.c2);
             if constexpr (TOP) {
                 if (++nt.batch == nt.next || nt.b == -INFINITY) {
                     nt.tighten();
                     nt.next = 2 * nt.batch;
+                }
+                // many alternatives: the list may fill before the bound is next due (10000 x 2500 fp32, 32 of them: 93 us, 160 without this)
+                if (nt.count > ROOM - 64 * N) {
+                    nt.tighten();
+                    nt.compact(sh.vecs[wave()]);
                 }
 #pragma unroll
                 for (int u = 0; u < N; ++u) nt.note(sh.vecs[wave()], mx[u] >= nt.b && mx[u] > -INFINITY, Vec{mx[u], v + u * NL});
@@ -897,7 +932,9 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) ln.add(x[u][i], a.c2);
         };
-        if constexpr (MODE == LP) st.each_compact(batch);      // with and without alternatives: the same sums, bit for bit
+        // by the same rule with and without alternatives: the same sums, bit for bit (50000 x 1000 bf16, five alternatives: 61 us compact,
+        // 56 not; by workgroups 5000 x 10000: 43, 50)
+        if constexpr (MODE == LP && W > 1) st.each_compact(batch);
         else st.each(batch);
         ln.follow(edge, a.c2);
         if (lane() < sp.edges()) ln.add(edge, a.c2);
@@ -971,15 +1008,9 @@ template <typename T, int W, int MODE, bool TOP> struct Long {
     {
         const int want = a.top, w = wave(), ln = threadIdx.x & 63;       // a span has far more classes
         // of the vectors noted, those that reach the last bound are read again and their elements that do are noted
-        const int vecs = nt.over ? 0 : nt.count;
-        int kept = 0;
-        for (int i = 0; i < vecs; i += 64) {
-            const Vec e = sh.vecs[w][min(i + ln, vecs - 1)];
-            const uint64_t mask = __ballot(i + ln < vecs && e.m >= nt.b);
-            if (mask >> ln & 1) sh.vecs[w][kept + __popcll(mask & ((1ull << ln) - 1))] = e;         // not behind its own place
-            kept += __popcll(mask);
-            team_sync<1>();
-        }
+        if (nt.over) nt.count = 0;
+        nt.compact(sh.vecs[w]);
+        const int kept = nt.count;
         nt.count = 0;
         for (int i = 0; i < kept; i += 64) {
             const int v = sh.vecs[w][min(i + ln, kept - 1)].v, c = sp.first_class(v);
@@ -1232,15 +1263,16 @@ template <typename T> __global__ __launch_bounds__(256) void four_distill(RowArg
     st.each([&](auto count, int v, const SisVec<T, VEC> (&raw)[UL]) {
         constexpr int N = decltype(count)::value;
         const bool last = v + (N - 1) * L < sp.nvec;
-        float x[N][VEC], top = -INFINITY;
+        float x[N][VEC], mx[N];
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             sis3d_unpack<T, VEC>(raw[u], x[u]);
             if (u == N - 1)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) x[u][i] = last ? x[u][i] : -INFINITY;
-            top = fmaxf(top, max_of(x[u]));
+            mx[u] = max_of(x[u]);
         }
+        const float top = max_of(mx);
         best = fmaxf(best, top);
         ln.follow(top, a.c2);
 #pragma unroll
@@ -1513,9 +1545,9 @@ int parts_of(int64_t R, int K, int64_t s_c)
     return (int)(p > 64 ? 64 : (p < 1 ? 1 : p));
 }
 
-// a wave to a row rather than a workgroup: up to 4096 classes, or 1024 vectors where there are rows enough (10000 x 5000 fp16, three
-// alternatives: 1.6 TB/s by workgroups)
-bool wave_rows(const RowArgs &a, int es) { return a.parts == 1 && (a.K <= K_WAVE || (a.K <= 16384 / es && a.R >= 4096)); }
+// a wave to a row rather than a workgroup: up to 4096 classes, or 1536 vectors where there are rows enough (5000 x 10000 bf16, five
+// alternatives: 46 us by workgroups, 27 by waves; 5000 x 5000 fp32 38 and 22)
+bool wave_rows(const RowArgs &a, int es) { return a.parts == 1 && (a.K <= K_WAVE || (a.K <= 24576 / es && a.R >= 4096)); }
 
 // distillation with 16 lanes to a row: rows of up to 4 KB, of 96 classes at least (tiles and waves against it, 8 entries, 100 MB:  fp32
 // x 64 31 / 41 us, x 100 41 / 32, x 300 38 / 23, x 1000 21 / 22;  fp16 x 100 61 / 56, x 300 52 / 31, x 600 46 / 23, x 1203 36 / 24, x 2000

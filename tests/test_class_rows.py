@@ -386,6 +386,29 @@ def test_one_row_of_scores_for_many_labels(K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K", [300, 1000, 3001, 6000])
+@pytest.mark.parametrize("dt", list(DT))
+def test_alternatives_of_many_rows(K, dt):
+    """every number of alternatives, rows by lanes and waves; among them ascending rows, of which every vector is a new best, and rows of few
+    different scores, of which many are at the bound"""
+    from sis3d import ops
+    R = 4100
+    l, labels, _, _, g = make(R, K, DT[dt], seed=K)
+    ramp = torch.arange(K, device="cuda", dtype=torch.float32)
+    l[0::5] = ramp.to(DT[dt])
+    l[1::5] = torch.randint(0, 6, (R, K), device="cuda", generator=g)[1::5].to(DT[dt])
+    l[2::5, K // 50:] = -math.inf
+    l[3::50] = -ramp.to(DT[dt])
+    # the order by (score, class): a stable sort of the scores, largest first
+    order = l.float().sort(dim=1, descending=True, stable=True)[1]
+    for top in (1, 2, 4, 5, 8, 9, 16, 17, 32):
+        logp, _, norm, tl, tc = ops.class_logprobs(l, labels, top)
+        assert torch.equal(tc, order[:, :top]), top
+        ls = log_softmax64(l.double())[0]
+        near(tl, ls.gather(1, tc), 4 * U * torch.where(torch.isfinite(ls), ls.abs(), 0.0).gather(1, tc) + chain(K) + 4 * U * (l.double().amax(1, True) - l.double()).gather(1, tc).nan_to_num(0, 0, 0), None, "top")
+
+
+@pytest.mark.gpu
 def test_streams_graph_and_determinism():
     from sis3d import ops
     for R, K, top in ((200, 19, 3), (64, 3000, 8), (2, 60000, 8), (300, 20011, 32)):
