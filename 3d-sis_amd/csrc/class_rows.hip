@@ -253,6 +253,7 @@ template <bool ENT> struct Lane {
         raise(fmaxf(mul_rounded(m, c2), -NEAR));
         s = lanes_sum<L>(s);
         if constexpr (ENT) t = lanes_sum<L>(t);
+        if (s == 0.f) return Soft<ENT>{LOWEST, 0.f, 0.f};              // nothing but masks here
         const float x = fmaf(m, c2, -M), e = exp2_(x);
         return Soft<ENT>{m, M < NEAR ? s / e : NAN, ENT ? fmaf(-x, s, t) / e : 0.f};
     }
