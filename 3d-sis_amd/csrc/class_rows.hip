@@ -32,8 +32,8 @@
 //   four_distill                   40000 x 1203 fp16, 8 entries: 21.6 us (4.6 TB/s)
 //   long_backward by waves         the same: 44.9 us (4.4 TB/s)
 //   long_forward by workgroups     4096 x 32768 bf16, 32 entries: 57 us (4.7 TB/s), backward 86 (6.3: what the L2s and the memory-side cache
-//                                  keep of the scores).  2000 x 20011 bf16: 24 us without alternatives, 31 with eight
-//   split_forward, split_join      3 x 65536 fp32, five alternatives: 7.9 + 3.8 us
+//                                  keep of the scores).  2000 x 20011 bf16: 21 us without alternatives, 31 with eight
+//   split_forward, split_join      3 x 65536 fp32, five alternatives: 8.4 + 4.0 us
 // What bounds the 16-bit forms next to memory is arithmetic: an exponential is four instructions' time, and with conversion, maximum and
 // the sums an element takes about ten.
 #include "elem.h"
