@@ -1540,7 +1540,7 @@ bool is_short(int K, int64_t s_c, int es) { return s_c != 1 ? K <= K_STRIDED : K
 // few long rows: parts of at least 4096 classes, enough for two workgroups per CU, at most one per lane of the joining wave
 int parts_of(int64_t R, int K, int64_t s_c)
 {
-    if (K <= K_WAVE || s_c != 1 || R >= 256) return 1;
+    if (K <= K_WAVE || s_c != 1 || R >= 256 || R <= 0) return 1;
     int64_t p = (512 + R - 1) / R;
     if (p > K / 4096) p = K / 4096;
     return (int)(p > 64 ? 64 : (p < 1 ? 1 : p));

@@ -625,3 +625,36 @@ def test_reference_gradients_are_slopes():
     want, = torch.autograd.grad((loss * ga).sum(), l)
     got = ref_distill(l.detach(), kept, cls, T, ga)
     assert torch.allclose(got["loss"], loss.detach()) and torch.allclose(got["dscore"], want, atol=1e-13)
+
+
+def test_abi_takes_empty_batches_of_any_number_of_classes():
+    """no rows: nothing to do, whatever the class list is (the rule that splits few long rows divides by their number)"""
+    from sis3d import _lib
+    l = _lib.lib()
+    p = ctypes.c_void_p(4096)                                                # never dereferenced
+    for N, V in ((1, 0), (0, 1), (0, 0), (0, 200)):
+        for K in (1, 1000, 1025, 4096, 4097, 20011, 65536):
+            rows = [p, 0, N, V, K, K * V, K, 1]
+            assert l.sis3d_class_logprobs_forward(*rows, p, None, 1, p, p, p, p, p, None, 0, None) == 0, (N, V, K)
+            assert l.sis3d_class_logprobs_backward(*rows, p, None, p, p, p, None, p, K * V, K, 1, None) == 0, (N, V, K)
+            assert l.sis3d_distill_forward(*rows, p, p, 3, None, 1.0, p, p, None, 0, None) == 0, (N, V, K)
+            assert l.sis3d_distill_backward(*rows, p, p, 3, None, 1.0, p, p, p, K * V, K, 1, None) == 0, (N, V, K)
+            assert l.sis3d_class_rows_workspace_bytes(N * V, K, 1, 5) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 10), (0, 4097), (0, 20011), (2, 20011, 0), (0, 20011, 7), (2, 41, 0), (0, 41, 3, 2)])
+def test_empty_batches(shape):
+    """a scene without detections, against short and long class lists: empty outputs, empty gradients"""
+    from sis3d import ops
+    rows = shape[:1] + shape[2:]
+    n = len(shape)
+    score = torch.empty(rows + shape[1:2], device="cuda").permute(0, n - 1, *range(1, n - 1))       # classes last in memory
+    assert score.shape == shape
+    labels = torch.empty(rows, dtype=torch.int64, device="cuda")
+    logp, h, norm, tl, tc = ops.class_logprobs(score, labels, top=3)
+    assert logp.shape == rows and h.shape == rows and norm.shape == rows + (2,) and tl.shape == tc.shape == rows + (3,)
+    assert ops.class_logprobs_backward(score, labels, norm, h, logp, h).shape == shape
+    kept, cls = torch.empty(rows + (4,), device="cuda"), torch.empty(rows + (4,), dtype=torch.int64, device="cuda")
+    loss, n2 = ops.distill_loss(score, kept, cls, 2.0)
+    assert loss.shape == rows and ops.distill_loss_backward(score, kept, cls, n2, loss, 2.0).shape == shape
