@@ -222,9 +222,11 @@ template <bool ENT> struct Soft {
 
 // The same sums for one lane of a long row, x = l c2 - M in one fused operation (its rounding is that of x; one of M would be common to all
 // classes and cancels).  M, in units of x, need only be near the largest: it follows it when it is exceeded by more than 2.  It starts at
-// -NEAR: scores that far below 0 (masks) add 0.  Where the largest lies outside +-NEAR the rounding of M itself is no longer small in x; such
-// rows, masked ones and those that are not finite end in a sum of 0, inf or NaN and are taken again class by class.
+// -NEAR: scores that far below 0 (masks) add 0.  Where the largest lies above NEAR the rounding of M itself is no longer small in x; where it
+// lies below -NEAR, which M does not follow, the largest term may be a number and smaller ones that count beside it may not.  Such rows,
+// masked ones and those that are not finite end in a sum of 0, inf or NaN and are taken again class by class.
 constexpr float NEAR = 4194304.f;          // 2^22: M is rounded by at most 1/4
+__device__ inline bool sums_hold(float m, float c2) { return fabsf(mul_rounded(m, c2)) < NEAR; }        // m: a row's largest score
 template <bool ENT> struct Lane {
     float M, s, t;
     __device__ void init() { M = -NEAR; s = t = 0.f; }
@@ -255,7 +257,7 @@ template <bool ENT> struct Lane {
         if constexpr (ENT) t = lanes_sum<L>(t);
         if (s == 0.f) return Soft<ENT>{LOWEST, 0.f, 0.f};              // nothing but masks here
         const float x = fmaf(m, c2, -M), e = exp2_(x);
-        return Soft<ENT>{m, M < NEAR ? s / e : NAN, ENT ? fmaf(-x, s, t) / e : 0.f};
+        return Soft<ENT>{m, sums_hold(m, c2) ? s / e : NAN, ENT ? fmaf(-x, s, t) / e : 0.f};
     }
 };
 
@@ -580,7 +582,7 @@ template <typename T, int MODE, int HOW, int TK> __global__ __launch_bounds__(25
     so.t = MODE == LP ? group_sum(ln.t, g) : 0.f;
     so.t = fmaf(-x0, so.s, so.t) / e0;
     so.s = so.s / e0;
-    if (!(so.s > 0.f && so.s < INFINITY && ln.M < NEAR)) {
+    if (!(so.s > 0.f && so.s < INFINITY && sums_hold(so.m, a.c2))) {
         so.init();
         for (int i = 0; i < t.n; ++i) so.m = fmaxf(so.m, score(t.lo + i));
         so.m = group_max(so.m, g);

@@ -658,3 +658,42 @@ def test_empty_batches(shape):
     kept, cls = torch.empty(rows + (4,), device="cuda"), torch.empty(rows + (4,), dtype=torch.int64, device="cuda")
     loss, n2 = ops.distill_loss(score, kept, cls, 2.0)
     assert loss.shape == rows and ops.distill_loss_backward(score, kept, cls, n2, loss, 2.0).shape == shape
+
+
+# rows whose largest score is a little below the lower end of the range that the fast sums take (l log2(e) / T = -2^22): the largest term is
+# still a number there, terms within 2^24 of it are not any more.  How far below, in powers of two; 0 and less: still inside
+BELOW = [-3, -0.25, 0.25, 1, 24, 64, 90, 99, 102, 105, 108, 112, 116, 120, 124, 126, 128, 140, 149, 151, 200, 1000]
+
+
+def rows_below_the_range(K, T):
+    """a row for each of BELOW: neighbouring numbers, at most 12 powers of two apart"""
+    c2 = 1.4426950408889634 / T
+    top = torch.tensor([-(2.0 ** 22 + b) / c2 for b in BELOW], dtype=torch.float64)
+    g = torch.Generator().manual_seed(K)
+    down = 12 / c2 * torch.rand(len(BELOW), K, generator=g, dtype=torch.float64)
+    down[:, K // 2] = 0
+    return (top[:, None] - down).float().cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [2, 19, 41, 64, 300, 530, 1000, 1025, 4096, 5000, 20011, 65536])
+@pytest.mark.parametrize("how", ["rows", "wide", "planar"])
+def test_rows_just_below_the_range_of_the_fast_sums(K, how):
+    if how == "planar" and K > 1024:
+        how = "channels_last"
+    R = len(BELOW)
+    labels = (torch.arange(R, device="cuda") * 7) % K
+    ga, ge = torch.ones(R, device="cuda"), torch.full((R,), 0.5, device="cuda")
+    l = rows_below_the_range(K, 1.0)
+    for top in (0, min(K, 3)):
+        check_logprobs(l, labels, ga, ge, top, torch.float32, how)
+    # so many rows that a lane, 16 lanes or a wave has one
+    n = max(1, min(200, int(4e6) // (K * R)))
+    check_logprobs(l.repeat(n, 1), labels.repeat(n), ga.repeat(n), ge.repeat(n), 1, torch.float32, how)
+    for T in (1.0, 1e-3, 2.0 ** -9):
+        l = rows_below_the_range(K, T)
+        g = torch.Generator(device="cuda").manual_seed(K)
+        cls = torch.randint(0, K, (R, 5), device="cuda", generator=g)
+        kept = l.gather(1, cls) + 2 * T * torch.randn(R, 5, device="cuda", generator=g)
+        check_distill(l, kept, cls, T, torch.float32, how)
+        check_distill(l.repeat(n, 1), kept.repeat(n, 1), cls.repeat(n, 1), T, torch.float32, how)
