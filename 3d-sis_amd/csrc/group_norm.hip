@@ -15,8 +15,11 @@
 // workgroup numbers from  floor(off[s] / T) + s  on, which leaves it at least ceil(n_s / T) of them whatever the lengths are, so the grid
 // and the workspace depend on the row count and the number of samples alone and the call captures into a graph.
 //
-// Sums: a thread adds d = x - K and d^2 in 32 bits over its rows (at most 2048, a few hundred mostly), K its own first row, so a mean that is large
-// against the deviation does not cancel; everything across threads is added in 64 bits.
+// Statistics: a thread adds d = x - K and d^2 in 32 bits over its rows (at most 2048, a few hundred mostly), K its own first row, and leaves
+// the mean and the sum M2 of squared deviations from it.  Threads, then tiles, are joined in 64 bits as such pairs, relative to the first one's
+// mean c:  mean = c + sum n_i (mean_i - c) / n,  M2 = sum M2_i + sum n_i (mean_i - c)^2 - (sum n_i (mean_i - c))^2 / n.  c is the mean of n_1
+// of the n values, so the two sides of the last difference are at most n / n_1 times their result: no level of the map, however large,
+// cancels in it, and a constant map has variance 0.
 //
 // Measured (kernel alone; rate of the bytes that it moves itself, the rows' second reading included):
 //   96 x 48 x 96 x 32 fp32, ReLU   gn_stats 13.1 us (4.3 TB/s), gn_apply 17.4 (6.5), gn_back_sums 22.6 (5.0), gn_back_apply 25.2 (6.7):  78 us
@@ -40,7 +43,7 @@ struct GnArgs {
     int64_t x_n, x_v, d_n, d_v, y_n, y_v;     // element strides between samples and rows of x, dy, y / dx
     int S, C, G, cpg, gpb, T, t_log, tiles, zero_tail;     // T rows a tile; ragged: T = 1 << t_log
     float eps;
-    double2 *part;                // forward: [G][workgroups] (sum, sum of squares)
+    double2 *part;                // forward: [G][workgroups] (mean, sum of squared deviations from it)
     float2 *part_g, *part_c;      // backward: [G][workgroups] and [workgroups][C]
     float *dw, *db;
 };
@@ -136,15 +139,14 @@ template <typename F> __device__ inline void finish_group(double s0, double s1, 
     if (l == 0) out(g, s0, s1);
 }
 
-// Adds, per group of the column block, pairs that the threads left in LDS: `epg` entries a group and row lane
-template <typename P, typename F> __device__ inline void reduce_groups(const P *lds, int rpb, int gl, int epg, F out)
+// Adds the weighted channel sums (backward) of a column block's groups, `cpg` pairs a group in LDS
+template <typename F> __device__ inline void reduce_channels(const float2 *lds, int gl, int cpg, F out)
 {
-    const int lp = lanes_per_group(gl), per = rpb * epg, l = threadIdx.x & (lp - 1);
+    const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
         double s0 = 0, s1 = 0;
-        for (int i = l; i < per; i += lp) {
-            const int r = i / epg;
-            const P v = lds[(r * gl + g) * epg + (i - r * epg)];
+        for (int i = l; i < cpg; i += lp) {
+            const float2 v = lds[g * cpg + i];
             s0 += v.x;
             s1 += v.y;
         }
@@ -152,34 +154,100 @@ template <typename P, typename F> __device__ inline void reduce_groups(const P *
     }
 }
 
-// p[i * stride] for i = from, from + step, ...: added in that order, eight of them on their way at a time
-template <typename P> __device__ inline void sum_pairs(const P *p, int64_t stride, int from, int n, int step, double &s0, double &s1)
+// f(there, p[i * stride]) for i = from, from + step, ...: in that order, N of them on their way at a time, the last ones perhaps not there
+template <int N, typename P, typename F> __device__ inline void each_pair(const P *p, int64_t stride, int from, int n, int step, F f)
 {
     int i = from;
-    for (; i + step < n; i += 8 * step) {
-        P v[8];
+    for (; i + step < n; i += N * step) {
+        P v[N];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = p[min(i + u * step, n - 1) * stride];
+        for (int u = 0; u < N; ++u) v[u] = p[min(i + u * step, n - 1) * stride];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            s0 += i + u * step < n ? v[u].x : 0;
-            s1 += i + u * step < n ? v[u].y : 0;
-        }
+        for (int u = 0; u < N; ++u) f(i + u * step < n, v[u]);
     }
-    if (i < n) {                                     // all there is, mostly, where samples are small
-        s0 += p[i * stride].x;
-        s1 += p[i * stride].y;
-    }
+    if (i < n) f(true, p[i * stride]);               // all there is, mostly, where samples are small
 }
 
-// The same over the tiles of one sample: part[g * tiles + first + p], so that a wave reads neighbouring tiles
-template <typename P, typename F> __device__ inline void reduce_tiles(const P *part, int tiles, int first, int ntiles, int g0, int gl, F out)
+// The sums of a sample's tiles: part[g * tiles + first + p], so that a wave reads neighbouring tiles
+template <typename F> __device__ inline void reduce_tiles(const float2 *part, int tiles, int first, int ntiles, int g0, int gl, F out)
 {
     const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
         double s0 = 0, s1 = 0;
-        sum_pairs(part + (size_t)(g0 + g) * tiles + first, 1, l, ntiles, lp, s0, s1);
+        each_pair<8>(part + (size_t)(g0 + g) * tiles + first, 1, l, ntiles, lp, [&](bool there, float2 v) {
+            s0 += there ? v.x : 0.f;
+            s1 += there ? v.y : 0.f;
+        });
         finish_group(s0, s1, lp, l, g, out);
+    }
+}
+
+// 1 / n of a count of values: Newton's iteration from an estimate of 23 bits or more, two steps
+__device__ inline double inverse(double n)
+{
+    double r = __builtin_amdgcn_rcp(n);
+    r = __builtin_fma(r, __builtin_fma(-n, r, 1.0), r);
+    return __builtin_fma(r, __builtin_fma(-n, r, 1.0), r);
+}
+
+__device__ inline float inverse(float n)
+{
+    const float r = __builtin_amdgcn_rcpf(n);
+    return fmaf(r, fmaf(-n, r, 1.f), r);
+}
+
+// (mean, M2) of several such pairs with their numbers of values, joined relative to c, the mean of the first one
+struct Joined {
+    double c, s0, s1;
+    __device__ Joined(double c_) : c(c_), s0(0), s1(0) {}
+    __device__ void add(double n, double2 v)
+    {
+        const double d = v.x - c, nd = n * d;
+        s0 += nd;
+        s1 += v.y + nd * d;
+    }
+};
+__device__ inline double2 joined(double c, double s0, double s1, double inv_n) { return make_double2(c + s0 * inv_n, s1 - s0 * (s0 * inv_n)); }
+
+// Joins, per group of the column block, what the threads left in LDS for `n` rows: `epg` entries a group and row lane, each of `chans` channels
+template <typename F> __device__ inline void join_groups(const double2 *lds, int rpb, int n, int gl, int epg, int chans, F out)
+{
+    const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1), all = n / rpb, more = n - all * rpb;      // a lane's rows: all, or one more
+    const int per = min(rpb, n) * epg;               // lanes without a row have left nothing
+    for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
+        Joined j(n ? lds[g * epg].x : 0);
+        for (int i = l; i < per; i += lp) {
+            const int r = i / epg;
+            j.add((double)((all + (r < more)) * chans), lds[(r * gl + g) * epg + (i - r * epg)]);
+        }
+        const double c = j.c, inv = inverse((double)n * epg * chans);
+        finish_group(j.s0, j.s1, lp, l, g, [&](int g_, double s0, double s1) { out(g_, joined(c, s0, s1, inv)); });
+    }
+}
+
+// The same over the tiles of one sample of `len` rows: all have T rows but the last one, which its lane adds by itself (an empty sample's one
+// place is read and not used).  Four pairs on their way: with eight, one channel a thread, two workgroups fit a CU and not three (5000 samples,
+// C 18, fp32: 85 us, 75 with four; elsewhere alike).
+template <typename F> __device__ inline void join_tiles(const GnArgs &a, int first, int ntiles, int64_t len, int g0, int gl, F out)
+{
+    const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1), before = max(ntiles - 1, 0);
+    for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
+        const double2 *p = a.part + (size_t)(g0 + g) * a.tiles + first;
+        Joined j(p[0].x);
+        const double2 end = p[before];
+        double d0 = 0, d1 = 0;
+        each_pair<4>(p, 1, l, before, lp, [&](bool there, double2 v) {
+            const double d = there ? v.x - j.c : 0;
+            d0 += d;
+            d1 = __builtin_fma(d, d, d1);
+            j.s1 += there ? v.y : 0;
+        });
+        const double whole = (double)a.T * a.cpg;
+        j.s0 = whole * d0;
+        j.s1 = __builtin_fma(whole, d1, j.s1);
+        if (l == (before & (lp - 1))) j.add((double)(len - (int64_t)before * a.T) * a.cpg, end);
+        const double c = j.c, inv = inverse((double)len * a.cpg);
+        finish_group(j.s0, j.s1, lp, l, g, [&](int g_, double s0, double s1) { out(g_, joined(c, s0, s1, inv)); });
     }
 }
 
@@ -273,7 +341,7 @@ template <int VEC> struct GroupOf {
     }
 };
 
-// Sums of one tile's rows, left per group in out(group, sum, sum of squares)
+// One tile's rows: mean and sum of squared deviations of every group, to out(group, pair); n = 0: not a number
 template <typename T, int VEC, typename F> __device__ inline void tile_sums(const GnArgs &a, const Cols &k, const T *px, int n, double2 *lds, F out)
 {
     const bool fold = a.cpg % VEC == 0;              // a vector's channels are of one group: one entry a thread
@@ -295,30 +363,43 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
                 s2[i] = fmaf(d, d, s2[i]);
             }
         });
-        double f0 = 0, f1 = 0;
+        if (m > 0) {
+            const float im = inverse((float)m);
+            float mean[VEC], M2[VEC];                // of each channel; the mean relative to the first channel's K, or, not folded, to its own
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const double kk = K[i], t0 = m * kk + s1[i], t1 = s2[i] + kk * (2.0 * s1[i] + m * kk);
-            f0 += t0;
-            f1 += t1;
-            if (!fold) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2(t0, t1);
+            for (int i = 0; i < VEC; ++i) {
+                mean[i] = s1[i] * im;
+                M2[i] = fmaf(-s1[i], mean[i], s2[i]);
+                if (!fold) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2((double)K[i] + mean[i], M2[i]);
+            }
+            if (fold) {
+                float all = 0.f, sq = 0.f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    mean[i] += K[i] - K[0];
+                    all += mean[i];
+                }
+                all *= 1.f / VEC;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = mean[i] - all;
+                    sq = fmaf(d * m, d, sq) + M2[i];
+                }
+                lds[k.ri * k.nv + k.cv] = make_double2((double)K[0] + all, sq);
+            }
         }
-        if (fold) lds[k.ri * k.nv + k.cv] = make_double2(f0, f1);
-    } else if (k.live) {
-        for (int i = 0; i < (fold ? 1 : VEC); ++i) lds[fold ? k.ri * k.nv + k.cv : (k.ri * k.nv + k.cv) * VEC + i] = make_double2(0, 0);
     }
     __syncthreads();
-    reduce_groups(lds, k.rpb, k.gl, fold ? a.cpg / VEC : a.cpg, out);
+    join_groups(lds, k.rpb, n, k.gl, fold ? a.cpg / VEC : a.cpg, fold ? VEC : 1, out);
 }
 
-// mean and r of a group from its sums
-__device__ inline void group_stats(const GnArgs &a, const Cols &k, const Tile &t, float *st, int g, double s0, double s1)
+// mean and r of a group from its mean and sum of squared deviations; 0 for an empty sample
+__device__ inline void group_stats(const GnArgs &a, const Cols &k, const Tile &t, float *st, int g, double2 v)
 {
-    const double m = (double)t.len * a.cpg;
     double mu = 0, r = 0;
-    if (m > 0) {
-        mu = s0 / m;
-        const double var = s1 / m - mu * mu;
+    if (t.len > 0) {
+        mu = v.x;
+        const double var = v.y * inverse((double)t.len * a.cpg);
         r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)a.eps);      // NaN passes
     }
     st[g] = (float)mu;
@@ -381,10 +462,11 @@ template <typename T, int VEC> __global__ __launch_bounds__(NT) void gn_stats(Gn
     if (t.s < 0 || t.s >= a.S || t.n == 0) return;
     const Cols k = columns<VEC>(a);
     tile_sums<T, VEC>(a, k, rows_at<T>(a.x, a, k, t, a.x_n, a.x_v), t.n, lds,
-                      [&](int g, double s0, double s1) { a.part[(size_t)(k.g0 + g) * a.tiles + blockIdx.x] = make_double2(s0, s1); });
+                      [&](int g, double2 v) { a.part[(size_t)(k.g0 + g) * a.tiles + blockIdx.x] = v; });
 }
 
-// ONCE: x and y are more than the L2 holds, they are read and written past it
+// ONCE: x and y are more than the L2 holds, they are read and written past it.  With one channel a thread three workgroups fit a CU, if the
+// compiler is held to their registers (5000 samples, C 18, fp32: PLACEHOLDER).
 template <typename T, int VEC, int ACT, bool ONCE> __global__ __launch_bounds__(NT) void gn_apply(GnArgs a)
 {
     extern __shared__ double2 ldsd[];
@@ -395,13 +477,13 @@ template <typename T, int VEC, int ACT, bool ONCE> __global__ __launch_bounds__(
     T *y = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
     if (t.s >= a.S) { zero_rows<T, VEC>(a, k, y, t.n); return; }
     if (t.n == 0) {                                  // an empty sample has statistics only
-        reduce_tiles(a.part, a.tiles, t.first, 0, k.g0, k.gl, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
+        join_tiles(a, t.first, 0, 0, k.g0, k.gl, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
         return;
     }
     Cols safe = k;                                   // threads beyond the block's vectors read its first and write nothing
     if (!k.live) safe.ri = safe.cv = 0, safe.c = k.g0 * a.cpg;
     Apply<T, VEC, ACT, ONCE> ap(a, safe, rows_at<T>(a.x, a, safe, t, a.x_n, a.x_v), t.n);
-    reduce_tiles(a.part, a.tiles, t.first, t.ntiles, k.g0, k.gl, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
+    join_tiles(a, t.first, t.ntiles, t.len, k.g0, k.gl, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
     __syncthreads();
     if (k.live) ap.run(a, k, st, y);
 }
@@ -417,7 +499,7 @@ template <typename T, int VEC, int ACT> __global__ __launch_bounds__(NT) void gn
     T *y = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
     if (t.s >= a.S) { zero_rows<T, VEC>(a, k, y, t.n); return; }
     const T *x = rows_at<T>(a.x, a, k, t, a.x_n, a.x_v);
-    tile_sums<T, VEC>(a, k, x, t.n, lds, [&](int g, double s0, double s1) { group_stats(a, k, t, st, g, s0, s1); });
+    tile_sums<T, VEC>(a, k, x, t.n, lds, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
     __syncthreads();
     if (k.live && t.n > 0) Apply<T, VEC, ACT, false>(a, k, x, t.n).run(a, k, st, y);
 }
@@ -491,7 +573,7 @@ __device__ inline void tile_grad_sums(const GnArgs &a, const Cols &k, const Tile
         lds[c] = make_float2((float)(w * s0), (float)(w * s1));
     }
     __syncthreads();
-    reduce_groups(lds, 1, k.gl, a.cpg, group);
+    reduce_channels(lds, k.gl, a.cpg, group);
 }
 
 template <typename T, int VEC, int ACT, bool ONCE> struct ApplyGrad {
@@ -548,7 +630,10 @@ template <typename T, int VEC, int ACT, bool ONCE> __global__ __launch_bounds__(
         const int c = ((int)blockIdx.x - a.tiles) * 32 + (threadIdx.x & 31), l = threadIdx.x >> 5;
         double s0 = 0, s1 = 0;
         if (c < a.C)
-            sum_pairs(a.part_c + c, a.C, l, a.tiles, NT / 32, s0, s1);
+            each_pair<8>(a.part_c + c, a.C, l, a.tiles, NT / 32, [&](bool there, float2 v) {
+                s0 += there ? v.x : 0.f;
+                s1 += there ? v.y : 0.f;
+            });
         acc[threadIdx.x][0] = s0;
         acc[threadIdx.x][1] = s1;
         __syncthreads();

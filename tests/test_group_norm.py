@@ -532,3 +532,51 @@ def test_reference_gradients_are_slopes():
         got = reference(x.detach(), dy, [0, 9, 23], 3, w.detach(), b.detach(), act)
         for k, v in (("y", y.detach()), ("dx", dx), ("dw", dw), ("db", db)):
             assert torch.allclose(got[k], v, rtol=1e-10, atol=1e-12), (act, k)
+
+
+def stats_of(rows, offsets, G):
+    """mean, variance and 1 / sqrt(var + eps) of float64 rows, per sample and group: deviations from the mean itself"""
+    C = rows.shape[1]
+    mean, rstd = [], []
+    for lo, hi in zip(offsets, offsets[1:]):
+        v = rows[lo:hi].reshape(hi - lo, G, C // G)
+        mu = v[:1, :, :1] + (v - v[:1, :, :1]).mean((0, 2), keepdim=True)
+        mean.append(mu.flatten())
+        rstd.append(1 / torch.sqrt(((v - mu) ** 2).mean((0, 2)) + EPS))
+    return torch.stack(mean), torch.stack(rstd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("level", [0.0, 1.7, 1e5, 3e5, 1e6, -1.2345e7])
+@pytest.mark.parametrize("C,G", [(16, 4), (32, 8), (20, 4), (19, 19), (64, 1), (6, 3), (1024, 4)])
+def test_statistics_of_a_large_mean_do_not_cancel(level, C, G):
+    """Constant maps and maps of two neighbouring numbers at a level that is far from 0: the variance is 0, or the square of a step.
+    rstd: a thread's variance of n rows has a relative error of a few n u at most (differences of neighbours are exact), joined in 64 bits:
+    32 u as everywhere here.  The mean, rounded to 32 bits, is off by u |mean| and a few u deviations."""
+    from sis3d import ops
+    g = torch.Generator(device="cuda").manual_seed(C)
+    lens = [13825, 1, 0, 300, 4097]
+    offsets = [0]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    R = offsets[-1]
+    live = [i for i, n in enumerate(lens) if n]
+    base = torch.full((R, C), level, device="cuda")
+    step = torch.nextafter(base[0, 0].cpu(), torch.tensor(float("inf"))).item() - base[0, 0].item()
+    one = base + (torch.rand(R, C, device="cuda", generator=g) < 0.3) * step
+    ramp = base + torch.randint(0, 16, (R, C), device="cuda", generator=g) * step
+    corner = base.clone()                                        # a map that is constant but for the first row
+    corner[0] += 64 * step
+    cases = [(base, torch.float32), (one, torch.float32), (ramp, torch.float32), (corner, torch.float32)]
+    cases += [(base, d) for d in (torch.bfloat16, torch.float16) if abs(level) < torch.finfo(d).max]
+    for x, dtype in cases:
+        x = x.to(dtype)
+        _, mean, rstd = ops.group_norm(x, G, offsets=torch.tensor(offsets, device="cuda"), want_stats=True)
+        wm, wr = stats_of(x.double(), [offsets[i] for i in live] + [R], G)
+        check_close(rstd[live], wr, 32 * U * wr, "rstd")
+        check_close(mean[live], wm, 4 * U * wm.abs() + 4 * U / wr, "mean")
+        for lo, n in ((0, 13825), (offsets[3], 300)):            # dense: two launches and one
+            _, mean, rstd = ops.group_norm(x[lo:lo + n][None].permute(0, 2, 1), G, want_stats=True)
+            wm, wr = stats_of(x[lo:lo + n].double(), [0, n], G)
+            check_close(rstd, wr, 32 * U * wr, "dense rstd")
+            check_close(mean, wm, 4 * U * wm.abs() + 4 * U / wr, "dense mean")
