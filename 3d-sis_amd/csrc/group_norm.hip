@@ -15,9 +15,11 @@
 // workgroup numbers from  floor(off[s] / T) + s  on, which leaves it at least ceil(n_s / T) of them whatever the lengths are, so the grid
 // and the workspace depend on the row count and the number of samples alone and the call captures into a graph.
 //
-// Statistics: a thread adds d = x - K and d^2 in 32 bits over its rows (at most 2048, a few hundred mostly), K its own first row, and leaves
-// the mean and the sum M2 of squared deviations from it.  Threads, then tiles, are joined in 64 bits as such pairs, relative to the first one's
-// mean c:  mean = c + sum n_i (mean_i - c) / n,  M2 = sum M2_i + sum n_i (mean_i - c)^2 - (sum n_i (mean_i - c))^2 / n.  c is the mean of n_1
+// Statistics: a thread keeps the mean a of its rows so far, in 32 bits and relative to its first row K, and the sum M2 of squared deviations
+// from it.  Four rows at a time: with s = sum d and q = sum d^2 of d = x - K - a, and n rows now, a += s / n, M2 += q - s^2 / n.  No row, the
+// first one included, stands so far out that the others are lost beside it (sums about K alone: 5e-4 of the variance of a flat map of 118
+// rows a thread with one peak).  Threads, then tiles, are joined in 64 bits as such pairs, relative to the first one's mean c:
+//     mean = c + sum n_i (mean_i - c) / n,  M2 = sum M2_i + sum n_i (mean_i - c)^2 - (sum n_i (mean_i - c))^2 / n.  c is the mean of n_1
 // of the n values, so the two sides of the last difference are at most n / n_1 times their result: no level of the map, however large,
 // cancels in it, and a constant map has variance 0.
 //
@@ -294,17 +296,23 @@ template <typename T, int VEC, bool ONCE> struct Rows {
     }
     __device__ const SisVec<T, VEC> &first() const { return cur[0]; }
 };
-template <typename T, int VEC, bool ONCE, typename F> __device__ inline void each_row(Rows<T, VEC, ONCE> &x, F f)
+template <typename T, int VEC, bool ONCE, typename F> __device__ inline void each_batch(Rows<T, VEC, ONCE> &x, F f)        // f(U vectors from row x.r on)
 {
     SisVec<T, VEC> next[U];
     const int step = U * x.rpb;
     for (; x.r < x.n; x.r += step) {
         if (x.r + step < x.n) x.load(next, x.r + step);
-#pragma unroll
-        for (int u = 0; u < U; ++u) f(x.r + u * x.rpb, x.r + u * x.rpb < x.n, x.cur[u]);
+        f(x.cur);
 #pragma unroll
         for (int u = 0; u < U; ++u) x.cur[u] = next[u];
     }
+}
+template <typename T, int VEC, bool ONCE, typename F> __device__ inline void each_row(Rows<T, VEC, ONCE> &x, F f)
+{
+    each_batch(x, [&](const SisVec<T, VEC> (&v)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(x.r + u * x.rpb, x.r + u * x.rpb < x.n, v[u]);
+    });
 }
 template <typename T, int VEC, bool ONCE, typename F> __device__ inline void each_row2(Rows<T, VEC, ONCE> &x, Rows<T, VEC, ONCE> &d, F f)
 {
@@ -347,31 +355,46 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
     const bool fold = a.cpg % VEC == 0;              // a vector's channels are of one group: one entry a thread
     if (k.live && n > 0) {
         Rows<T, VEC, false> x(px, a.x_v, k, n);
-        float K[VEC], s1[VEC], s2[VEC];
+        float K[VEC], mean[VEC], M2[VEC];            // of each channel's m rows so far, the mean relative to K
         int m = 0;
         sis3d_unpack<T, VEC>(x.first(), K);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = 0.f;
-        each_row(x, [&](int, bool there, const SisVec<T, VEC> &v) {
-            m += there;
-            float f[VEC];
-            sis3d_unpack<T, VEC>(v, f);
+        for (int i = 0; i < VEC; ++i) mean[i] = M2[i] = 0.f;
+        each_batch(x, [&](const SisVec<T, VEC> (&v)[U]) {
+            float s[VEC], q[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s[i] = q[i] = 0.f;
+            auto add = [&](const SisVec<T, VEC> &row) {
+                float f[VEC];
+                sis3d_unpack<T, VEC>(row, f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = f[i] - K[i] - mean[i];
+                    s[i] += d;
+                    q[i] = fmaf(d, d, q[i]);
+                }
+            };
+            if (x.r + (U - 1) * x.rpb < x.n) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) add(v[u]);
+                m += U;
+            } else {
+#pragma unroll
+                for (int u = 0; u + 1 < U; ++u)
+                    if (x.r + u * x.rpb < x.n) add(v[u]), ++m;
+            }
+            const float im = inverse((float)m);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float d = there ? f[i] - K[i] : 0.f;
-                s1[i] += d;
-                s2[i] = fmaf(d, d, s2[i]);
+                const float t = s[i] * im;
+                mean[i] += t;
+                M2[i] += fmaf(-s[i], t, q[i]);
             }
         });
         if (m > 0) {
-            const float im = inverse((float)m);
-            float mean[VEC], M2[VEC];                // of each channel; the mean relative to the first channel's K, or, not folded, to its own
+            if (!fold)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                mean[i] = s1[i] * im;
-                M2[i] = fmaf(-s1[i], mean[i], s2[i]);
-                if (!fold) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2((double)K[i] + mean[i], M2[i]);
-            }
+                for (int i = 0; i < VEC; ++i) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2((double)K[i] + mean[i], M2[i]);
             if (fold) {
                 float all = 0.f, sq = 0.f;
 #pragma unroll

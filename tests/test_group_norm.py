@@ -580,3 +580,25 @@ def test_statistics_of_a_large_mean_do_not_cancel(level, C, G):
             wm, wr = stats_of(x[lo:lo + n].double(), [0, n], G)
             check_close(rstd, wr, 32 * U * wr, "dense rstd")
             check_close(mean, wm, 4 * U * wm.abs() + 4 * U / wr, "dense mean")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,G,R,dtype", [(511, 1, 60000, torch.float32), (511, 7, 60000, torch.float32), (2048, 1, 20000, torch.float32), (2048, 8, 40000, torch.float16),
+                                         (256, 1, 40000, torch.float32), (32, 8, 200000, torch.float32), (19, 19, 40000, torch.bfloat16), (128, 16, 864, torch.float32)])
+@pytest.mark.parametrize("level,peak", [(0.1, 10.0), (-0.37, 7.3), (0.1, 1234.567), (100.3, 0.1)])
+def test_statistics_of_a_flat_map_with_a_few_peaks(C, G, R, dtype, level, peak):
+    """Rows that stand out from a flat map, wherever in a tile they are, the first row of a thread among them: none may spoil the sums of the
+    rows behind it.  A thread of n rows joins n / 4 batches, each off by a few u of its squared deviations, to the sum so far, one rounding
+    each: (n / 4 + 16) u of the variance and half of it of rstd, with n <= 128 here: 24 u, and a rounding; 32 u as everywhere."""
+    from sis3d import ops
+    for first in (0, 1, R // 2, R - 1):
+        x = torch.full((R, C), level, device="cuda")
+        x[first] = peak
+        if first == 1:
+            x[::3001] = peak
+        x = x.to(dtype)
+        want = stats_of(x.double(), [0, R], G)
+        for off in (None, torch.tensor([0, R], device="cuda")):
+            _, mean, rstd = ops.group_norm(x if off is not None else x[None].permute(0, 2, 1), G, offsets=off, want_stats=True)
+            check_close(rstd, want[1], 32 * U * want[1], "rstd, row %d" % first)
+            check_close(mean, want[0], 4 * U * want[0].abs() + 4 * U / want[1], "mean, row %d" % first)
