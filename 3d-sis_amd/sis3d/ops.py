@@ -1608,7 +1608,10 @@ class RaggedBatch:
         return hit
 
     def group_norm(self, src, groups, weight=None, bias=None, eps=1e-5, act=None):
-        """(voxels, C) -> (voxels, C): every crop normalised by its own statistics"""
+        """(voxels, C) -> (voxels, C): every crop normalised by its own statistics; differentiable"""
+        if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (src, weight, bias)):
+            from .layer_utils.group_norm import GroupNormAct                 # which is built on this module
+            return GroupNormAct.apply(src, weight, bias, groups, eps, act, self.offsets())
         return group_norm(src, groups, weight, bias, eps, act=act, offsets=self.offsets())
 
     def views(self, out):

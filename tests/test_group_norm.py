@@ -602,3 +602,31 @@ def test_statistics_of_a_flat_map_with_a_few_peaks(C, G, R, dtype, level, peak):
             _, mean, rstd = ops.group_norm(x if off is not None else x[None].permute(0, 2, 1), G, offsets=off, want_stats=True)
             check_close(rstd, want[1], 32 * U * want[1], "rstd, row %d" % first)
             check_close(mean, want[0], 4 * U * want[0].abs() + 4 * U / want[1], "mean, row %d" % first)
+
+
+@pytest.mark.gpu
+def test_crops_of_the_mask_head_in_training():
+    """RaggedBatch.group_norm is differentiable: gradients of the source, the weight and the bias are the operator's"""
+    from sis3d import ops
+    windows = [(0, 0, 0, 9, 10, 11), (3, 2, 1, 4, 3, 2), (5, 5, 5, 17, 20, 14)]
+    rb = ops.RaggedBatch(windows, torch.device("cuda"))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    src = torch.randn(rb.voxels, 64, device="cuda", generator=g)
+    w, b = torch.rand(64, device="cuda", generator=g), torch.rand(64, device="cuda", generator=g)
+    dy = torch.randn(rb.voxels, 64, device="cuda", generator=g)
+    y, mean, rstd = ops.group_norm(src, 16, w, b, act="silu", offsets=rb.offsets(), want_stats=True)
+    want = ops.group_norm_backward(dy, src, mean, rstd, 16, w, b, act="silu", offsets=rb.offsets())
+    for which in ((0, 1, 2), (0,), (1, 2)):                     # a leaf each, and constants beside it
+        leaves = [t.clone().requires_grad_(i in which) for i, t in enumerate((src, w, b))]
+        got = rb.group_norm(leaves[0], 16, leaves[1], leaves[2], act="silu")
+        assert got.requires_grad and torch.equal(got.detach(), y)
+        got.backward(dy)
+        for i, t in enumerate(leaves):
+            assert torch.equal(t.grad, want[i]) if i in which else t.grad is None
+    leaf = src.clone().requires_grad_(True)
+    rb.group_norm(leaf, 16).backward(dy)                        # no weight, no bias
+    y, mean, rstd = ops.group_norm(src, 16, offsets=rb.offsets(), want_stats=True)
+    assert torch.equal(leaf.grad, ops.group_norm_backward(dy, src, mean, rstd, 16, offsets=rb.offsets())[0])
+    with torch.no_grad():
+        got = rb.group_norm(leaf, 16)
+    assert not got.requires_grad and torch.equal(got, y)
