@@ -75,7 +75,9 @@ class HipGroupNorm(nn.GroupNorm):
         self.act = act
 
     def forward(self, x, offsets=None):
-        return GroupNormAct.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.act, offsets)
+        # the operator's parameters are fp32; after .bfloat16() / .half() they are taken at their value, and the cast carries the gradient
+        weight, bias = (p.float() if p is not None and p.dtype in (torch.bfloat16, torch.float16) else p for p in (self.weight, self.bias))
+        return GroupNormAct.apply(x, weight, bias, self.num_groups, self.eps, self.act, offsets)
 
 
 class Bottleneck(nn.Module):

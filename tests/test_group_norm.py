@@ -630,3 +630,39 @@ def test_crops_of_the_mask_head_in_training():
     with torch.no_grad():
         got = rb.group_norm(leaf, 16)
     assert not got.requires_grad and torch.equal(got, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("affine", [True, False])
+def test_module_in_16_bits(dtype, affine):
+    """HipGroupNorm after .bfloat16() / .half(), as nn.GroupNorm: 16-bit parameters, taken at their value, and their gradients in 16 bits"""
+    from sis3d import ops
+    from sis3d.nets.backbones import HipGroupNorm
+    g = torch.Generator(device="cuda").manual_seed(6)
+    m = HipGroupNorm(8, 64, act="relu", affine=affine).cuda()
+    if affine:
+        with torch.no_grad():
+            m.weight.normal_(1, 0.2, generator=g)
+            m.bias.normal_(0, 0.2, generator=g)
+    m = m.to(dtype)
+    assert all(p.dtype is dtype for p in m.parameters()) and len(list(m.parameters())) == 2 * affine
+    w, b = (m.weight.detach().float(), m.bias.detach().float()) if affine else (None, None)
+    rows = torch.randn(700, 64, device="cuda", generator=g).to(dtype)
+    dy = torch.randn(700, 64, device="cuda", generator=g).to(dtype)
+    off = torch.tensor([0, 300, 700], device="cuda")
+    for x, d, offsets in ((rows, dy, off), (rows[None].permute(0, 2, 1), dy[None].permute(0, 2, 1), None)):
+        m.zero_grad()
+        x = x.detach().requires_grad_(True)
+        y = m(x, offsets)
+        y.backward(d)
+        want, mean, rstd = ops.group_norm(x.detach(), 8, w, b, m.eps, act="relu", offsets=offsets, want_stats=True)
+        dx, dw, db = ops.group_norm_backward(d, x.detach(), mean, rstd, 8, w, b, act="relu", offsets=offsets)
+        assert y.dtype is dtype and torch.equal(y.detach(), want) and torch.equal(x.grad, dx)
+        if affine:
+            assert torch.equal(m.weight.grad, dw.to(dtype)) and torch.equal(m.bias.grad, db.to(dtype))
+    with torch.no_grad():
+        assert torch.equal(m(rows, off), ops.group_norm(rows, 8, w, b, m.eps, act="relu", offsets=off))
+    # fp32 maps between 16-bit parameters, and fp32 parameters at 16-bit maps
+    assert torch.equal(m(rows.float(), off).detach(), ops.group_norm(rows.float(), 8, w, b, m.eps, act="relu", offsets=off))
+    assert torch.equal(m.float()(rows, off).detach(), ops.group_norm(rows, 8, w, b, m.eps, act="relu", offsets=off))
