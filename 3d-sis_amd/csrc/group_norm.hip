@@ -24,11 +24,11 @@
 // cancels in it, and a constant map has variance 0.
 //
 // Measured (kernel alone; rate of the bytes that it moves itself, the rows' second reading included):
-//   96 x 48 x 96 x 32 fp32, ReLU   gn_stats 13.1 us (4.3 TB/s), gn_apply 17.4 (6.5), gn_back_sums 22.6 (5.0), gn_back_apply 25.2 (6.7):  78 us
+//   96 x 48 x 96 x 32 fp32, ReLU   gn_stats 13.1 us (4.3 TB/s), gn_apply 17.8 (6.4), gn_back_sums 22.0 (5.1), gn_back_apply 25.1 (6.8):  78 us
 //                                  for 226 MB that have to move once
 //   24 x 12 x 24 x 128 fp32, ReLU  4.9, 5.6, 7.0, 7.0 us: the loads' way and back, twice a launch; the calls take the host 35 us
-//   16 crops, 43995 x 64 in all    7.3, 8.0, 9.2, 9.2 us
-//   12 x 6 x 12 x 128 fp32         gn_one 6.9 us
+//   16 crops, 43995 x 64 in all    7.4, 7.7, 10.3, 8.7 us
+//   12 x 6 x 12 x 128 fp32         gn_one 7.0 us
 #include "elem.h"
 
 namespace {
@@ -396,19 +396,22 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2((double)K[i] + mean[i], M2[i]);
             if (fold) {
-                float all = 0.f, sq = 0.f;
+                // the mean is made of the channels' K in 64 bits, so that it is rounded no more than they are; deviations from it need no more than 32
+                double k_all = 0;
+                float a_all = 0.f, sq = 0.f;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    mean[i] += K[i] - K[0];
-                    all += mean[i];
+                    k_all += K[i];
+                    a_all += mean[i];
                 }
-                all *= 1.f / VEC;
+                const double all = (k_all + a_all) * (1.0 / VEC);
+                const float near = (float)(all - K[0]);          // relative to the first channel's K, as the channels' means below
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = mean[i] - all;
+                    const float d = K[i] - K[0] + mean[i] - near;
                     sq = fmaf(d * m, d, sq) + M2[i];
                 }
-                lds[k.ri * k.nv + k.cv] = make_double2((double)K[0] + all, sq);
+                lds[k.ri * k.nv + k.cv] = make_double2(all, sq);
             }
         }
     }

@@ -666,3 +666,20 @@ def test_module_in_16_bits(dtype, affine):
     # fp32 maps between 16-bit parameters, and fp32 parameters at 16-bit maps
     assert torch.equal(m(rows.float(), off).detach(), ops.group_norm(rows.float(), 8, w, b, m.eps, act="relu", offsets=off))
     assert torch.equal(m.float()(rows, off).detach(), ops.group_norm(rows, 8, w, b, m.eps, act="relu", offsets=off))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,G", [(512, 8), (64, 1), (128, 16), (48, 16), (130, 10)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_mean_of_few_rows_is_rounded_once(C, G, dtype):
+    """A thread's only row enters the mean in 64 bits: what comes out is the mean of the group rounded to 32 bits, however much of it cancels
+    (u of it, and 2^-40 of the largest value for the additions in 64 bits)."""
+    from sis3d import ops
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x = torch.randn(3, C, device="cuda", generator=g) * 20
+    x = (x - x.view(3, G, C // G).mean(2, keepdim=True).expand(-1, -1, C // G).reshape(3, C)).to(dtype)          # means of nearly 0
+    for off in ([0, 1, 2, 3], [0, 3], [0, 1, 3]):
+        want = stats_of(x.double(), off, G)
+        _, mean, rstd = ops.group_norm(x, G, offsets=torch.tensor(off, device="cuda"), want_stats=True)
+        check_close(mean, want[0], U * want[0].abs() + 2.0 ** -40 * 100, "mean")
+        check_close(rstd, want[1], 32 * U * want[1], "rstd")
