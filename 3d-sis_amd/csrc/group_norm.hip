@@ -228,9 +228,9 @@ template <typename F> __device__ inline void join_groups(const double2 *lds, int
 }
 
 // The same over the tiles of one sample of `len` rows: all have T rows but the last one, which its lane adds by itself (an empty sample's one
-// place is read and not used).  Four pairs on their way: with eight, one channel a thread, two workgroups fit a CU and not three (5000 samples,
-// C 18, fp32: 85 us, 75 with four; elsewhere alike).
-template <typename F> __device__ inline void join_tiles(const GnArgs &a, int first, int ntiles, int64_t len, int g0, int gl, F out)
+// place is read and not used).  N pairs on their way: four with one channel a thread, so that three workgroups fit a CU (5000 samples, C 18,
+// fp32: 75 us, 85 with eight), else eight, where two fit either way (40 MB fp32, one group: 22.2 us, 23.0 with four).
+template <int N, typename F> __device__ inline void join_tiles(const GnArgs &a, int first, int ntiles, int64_t len, int g0, int gl, F out)
 {
     const int lp = lanes_per_group(gl), l = threadIdx.x & (lp - 1), before = max(ntiles - 1, 0);
     for (int g = threadIdx.x / lp; g < gl; g += NT / lp) {
@@ -238,7 +238,7 @@ template <typename F> __device__ inline void join_tiles(const GnArgs &a, int fir
         Joined j(p[0].x);
         const double2 end = p[before];
         double d0 = 0, d1 = 0;
-        each_pair<4>(p, 1, l, before, lp, [&](bool there, double2 v) {
+        each_pair<N>(p, 1, l, before, lp, [&](bool there, double2 v) {
             const double d = there ? v.x - j.c : 0;
             d0 += d;
             d1 = __builtin_fma(d, d, d1);
@@ -503,13 +503,13 @@ template <typename T, int VEC, int ACT, bool ONCE> __global__ __launch_bounds__(
     T *y = (T *)rows_at<T>(a.y, a, k, t, a.y_n, a.y_v);
     if (t.s >= a.S) { zero_rows<T, VEC>(a, k, y, t.n); return; }
     if (t.n == 0) {                                  // an empty sample has statistics only
-        join_tiles(a, t.first, 0, 0, k.g0, k.gl, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
+        join_tiles<VEC == 1 ? 4 : 8>(a, t.first, 0, 0, k.g0, k.gl, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
         return;
     }
     Cols safe = k;                                   // threads beyond the block's vectors read its first and write nothing
     if (!k.live) safe.ri = safe.cv = 0, safe.c = k.g0 * a.cpg;
     Apply<T, VEC, ACT, ONCE> ap(a, safe, rows_at<T>(a.x, a, safe, t, a.x_n, a.x_v), t.n);
-    join_tiles(a, t.first, t.ntiles, t.len, k.g0, k.gl, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
+    join_tiles<VEC == 1 ? 4 : 8>(a, t.first, t.ntiles, t.len, k.g0, k.gl, [&](int g, double2 v) { group_stats(a, k, t, st, g, v); });
     __syncthreads();
     if (k.live) ap.run(a, k, st, y);
 }
