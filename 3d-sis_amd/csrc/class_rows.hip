@@ -1536,7 +1536,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void four_back
 // a launch has at most 2^32 - 1 threads
 bool too_many(int64_t workgroups) { return workgroups > 0xffffffffll / 256; }
 
-// 50000 x 1000 fp16, log probabilities: 0.81 TB/s as a short row, 2.5 TB/s as a longer one
+// fp16, log probabilities, forward / backward: 50000 x 1000 48 / 59 us as short rows, 35 / 37 as longer ones; 83000 x 600 44 / 42 and 52 / 41
 bool is_short(int K, int64_t s_c, int es) { return s_c != 1 ? K <= K_STRIDED : K <= 64 * (16 / es) + 16; }
 
 // few long rows: parts of at least 4096 classes, enough for two workgroups per CU, at most one per lane of the joining wave

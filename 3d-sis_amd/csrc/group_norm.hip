@@ -24,10 +24,10 @@
 // cancels in it, and a constant map has variance 0.
 //
 // Measured (kernel alone; rate of the bytes that it moves itself, the rows' second reading included):
-//   96 x 48 x 96 x 32 fp32, ReLU   gn_stats 13.1 us (4.3 TB/s), gn_apply 17.8 (6.4), gn_back_sums 22.0 (5.1), gn_back_apply 25.1 (6.8):  78 us
+//   96 x 48 x 96 x 32 fp32, ReLU   gn_stats 13.2 us (4.3 TB/s), gn_apply 17.3 (6.5), gn_back_sums 22.6 (5.0), gn_back_apply 24.9 (6.8):  78 us
 //                                  for 226 MB that have to move once
-//   24 x 12 x 24 x 128 fp32, ReLU  4.9, 5.6, 7.0, 7.0 us: the loads' way and back, twice a launch; the calls take the host 35 us
-//   16 crops, 43995 x 64 in all    7.4, 7.7, 10.3, 8.7 us
+//   24 x 12 x 24 x 128 fp32, ReLU  5.0, 5.6, 6.8, 7.0 us: the loads' way and back, twice a launch; the calls take the host 34 us
+//   16 crops, 43995 x 64 in all    7.2, 8.0, 9.1, 9.0 us
 //   12 x 6 x 12 x 128 fp32         gn_one 7.0 us
 #include "elem.h"
 

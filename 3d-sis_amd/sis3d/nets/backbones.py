@@ -30,7 +30,7 @@ class _Packed(object):
 
 
 class HipConv3d(nn.Conv3d):
-    """nn.Conv3d parameters, HIP forward.  k in {1, 3 (pad 1), 2 (stride 2)}; fuse_relu folds the
+    """nn.Conv3d parameters, HIP forward (no gradient: the result has no history).  k in {1, 3 (pad 1), 2 (stride 2)}; fuse_relu folds the
     following nn.ReLU into the epilogue."""
 
     def __init__(self, cin, cout, kernel_size, stride=1, padding=0, bias=True, fuse_relu=False, fuse_sigmoid=False):
@@ -67,8 +67,10 @@ class HipMaxPool3d(nn.Module):
 
 class HipGroupNorm(nn.GroupNorm):
     """nn.GroupNorm parameters and state_dict keys on channels-last activations, with the activation behind it fused (act: None,
-    'relu', 'silu'): the normalisation for training on one chunk per GPU.  Differentiable; `offsets` (RaggedBatch.offsets) normalises
-    every crop of a packed (voxels, C) batch by itself."""
+    'relu', 'silu'): a normalisation that does not look at the batch, for one chunk per GPU.  Differentiable, between layers that are: torch's own
+    (nn.Conv3d in channels_last_3d).  HipConv3d and the other layers of this module are the detector's forward path: what they return has no
+    history, so no gradient passes through them.  `offsets` (RaggedBatch.offsets) normalises every crop of a packed (voxels, C) batch by
+    itself."""
 
     def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, act=None):
         super().__init__(num_groups, num_channels, eps=eps, affine=affine)

@@ -1601,7 +1601,8 @@ class RaggedBatch:
         return out
 
     def offsets(self):
-        """first row of every crop and the row count, int64 on the device: what group_norm takes to normalise each crop by itself"""
+        """first row of every crop and the row count, int64 on the device: what group_norm takes to normalise each crop by itself (copied
+        there at the first call, which therefore comes before a capture, as with `table`)"""
         hit = self._tables.get("offsets")
         if hit is None:
             hit = self._tables["offsets"] = torch.from_numpy(self.voffs).to(self.device)
@@ -1795,7 +1796,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act=None, offsets=No
     x: (N,C,*spatial), fp32 / bf16 / fp16, channels-last (dense, or a channel range of a wider tensor), statistics per sample and
     group; or, with offsets (S+1,) int64 on the device, (rows, C) of which sample s is [offsets[s], offsets[s+1]) -- the packing of
     RaggedBatch.  weight / bias (C,) fp32 or None; act: None / 'none', 'relu', 'silu'.  out: where to write (x itself is allowed, any
-    other overlap is not); rows behind offsets[-1] are left as they are in `out`, and zero without it.
+    other overlap is not); rows behind offsets[-1] are left as they are in `out`, and zero without it.  No history: the differentiable
+    form is layer_utils.group_norm.GroupNormAct.
     -> y, or (y, mean, rstd) with want_stats: (samples, groups) fp32 for group_norm_backward."""
     (code, S, V, C, sn, sv, groups, actc, dense, wsb, _), samples, offsets, weight, bias = _norm_args(x, groups, weight, bias, act, offsets)
     if out is None:
@@ -1893,6 +1895,7 @@ def class_logprobs(score, labels, top=0, num=None):
 
     score (R,K), or (N,K,*spatial) planar or channels-last, fp32 / bf16 / fp16; labels int64 (R,) or (N,*spatial): a negative label is
     none (log probability 0).  num: int32 tensor with the number of live rows (detection passes pad theirs): outputs behind are 0.
+    No history: the differentiable form is layer_utils.class_losses.ClassLogProbs.
     -> (logp, entropy, norm, top_logp, top_class): logp / entropy fp32 like labels; norm (...,2) for the backward pass (a row's
     largest score m and the sum s of exp(score - m): m + log s is the row's log-sum-exp); top_logp fp32 / top_class int64
     (...,top), best first, the lowest class first among equal scores; top <= min(32, K)."""
@@ -1952,7 +1955,8 @@ def distill_loss(score, kept, classes, temperature=1.0, num=None):
 
     score: the student's scores, as class_logprobs takes them; kept (R,k) / (N,*spatial,k) fp32 teacher logits of `classes` (same shape,
     int64; negative = absent, equal classes add up), k <= 128.  The teacher's distribution is the softmax of kept / T over the entries
-    that are present, the student's the softmax of score / T over all classes; a row without entries has loss 0.
+    that are present, the student's the softmax of score / T over all classes; a row without entries has loss 0.  No history: the
+    differentiable form is layer_utils.class_losses.DistillLoss.
     -> (loss fp32 (R,) / (N,*spatial), norm for the backward pass)."""
     _gpu(score, "score")
     code, rows, N, V, K, sn, sv, sc, _, _, _, _, wsb = _score_plan(score.dtype, score.shape, score.stride(), 0)

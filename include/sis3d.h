@@ -566,7 +566,8 @@ int sis3d_maxpool3d_3x3x3(const float *in, int X, int Y, int Z, int C, float *ou
  * rows in one buffer, sample s = rows [offsets[s], offsets[s+1]), offsets [S+1] int64 on the DEVICE, ascending from 0; rows from
  * offsets[S] on are left as they are (zero_tail = 0) or zeroed (1; what backward does with dx).  Samples may be empty (mean = rstd = 0).
  * weight / bias [C] fp32, each may be NULL (1 / 0).  mean / rstd [S][G] fp32: forward writes them (both may be NULL), backward reads them.
- * Statistics: 32-bit sums of differences to a nearby value per thread, 64-bit across threads; no atomics, results do not vary.
+ * Statistics: a running mean and squared deviations from it, in 32 bits per thread, joined as such in 64 bits (no level of x and no row that
+ * stands out cancels in the variance); no atomics, results do not vary.
  * backward also writes dweight / dbias [C] fp32 (each may be NULL), summed over all samples.  y may be x (in place); dx may be dy, not x.
  * SIS3D_EUNSUPPORTED: more than 512 * (16 bytes / element) channels per group (512 where a pointer, a stride or C is not a multiple of
  * 16 bytes), or more samples than a launch has workgroups (millions).  workspace: 16-byte aligned, sis3d_group_norm_workspace_bytes (ragged: 0 / 1), any content. */
