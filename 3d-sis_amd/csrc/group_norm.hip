@@ -396,9 +396,10 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) lds[(k.ri * k.nv + k.cv) * VEC + i] = make_double2((double)K[i] + mean[i], M2[i]);
             if (fold) {
-                // the mean is made of the channels' K in 64 bits, so that it is rounded no more than they are; deviations from it need no more than 32
-                double k_all = 0;
-                float a_all = 0.f, sq = 0.f;
+                // the mean is made of the channels' K in 64 bits, so that it is rounded no more than they are; deviations from it need no more
+                // than 32, but their squares may leave them
+                double k_all = 0, sq = 0;
+                float a_all = 0.f;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     k_all += K[i];
@@ -408,8 +409,8 @@ template <typename T, int VEC, typename F> __device__ inline void tile_sums(cons
                 const float near = (float)(all - K[0]);          // relative to the first channel's K, as the channels' means below
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = K[i] - K[0] + mean[i] - near;
-                    sq = fmaf(d * m, d, sq) + M2[i];
+                    const double d = K[i] - K[0] + mean[i] - near;
+                    sq = __builtin_fma(d * m, d, sq) + M2[i];
                 }
                 lds[k.ri * k.nv + k.cv] = make_double2(all, sq);
             }
@@ -491,8 +492,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(NT) void gn_stats(Gn
                       [&](int g, double2 v) { a.part[(size_t)(k.g0 + g) * a.tiles + blockIdx.x] = v; });
 }
 
-// ONCE: x and y are more than the L2 holds, they are read and written past it.  With one channel a thread three workgroups fit a CU, if the
-// compiler is held to their registers (5000 samples, C 18, fp32: PLACEHOLDER).
+// ONCE: x and y are more than the L2 holds, they are read and written past it
 template <typename T, int VEC, int ACT, bool ONCE> __global__ __launch_bounds__(NT) void gn_apply(GnArgs a)
 {
     extern __shared__ double2 ldsd[];

@@ -683,3 +683,16 @@ def test_mean_of_few_rows_is_rounded_once(C, G, dtype):
         _, mean, rstd = ops.group_norm(x, G, offsets=torch.tensor(off, device="cuda"), want_stats=True)
         check_close(mean, want[0], U * want[0].abs() + 2.0 ** -40 * 100, "mean")
         check_close(rstd, want[1], 32 * U * want[1], "rstd")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,G", [(512, 8), (64, 1), (48, 16), (130, 10)])
+def test_one_row_whose_squares_are_beyond_32_bits(C, G):
+    """a thread's only row needs no square in 32 bits: deviations of 1e25 and more still have their variance (rstd to 32 u)"""
+    from sis3d import ops
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x = torch.randn(2, C, device="cuda", generator=g) * 1e25
+    want = stats_of(x.double(), [0, 1, 2], G)
+    y, mean, rstd = ops.group_norm(x, G, offsets=torch.tensor([0, 1, 2], device="cuda"), want_stats=True)
+    check_close(rstd, want[1], 32 * U * want[1], "rstd")
+    check_close(mean, want[0], U * want[0].abs() + 2.0 ** -40 * 1e26, "mean")
